@@ -1,0 +1,513 @@
+// Linear layer whose backward works from an 8-bit checkpoint of its input (CDNA4, gfx950).
+//
+//   y  = act(x) w^T + b             act: identity or gelu_tanh; from x itself
+//   c  = what the checkpoint of x stands for
+//   dx = (dy w) act'(c)     dw = dy^T act(c)     db = sum dy
+//
+// Checkpoint: blocks of 32 features of one row, each e4m3 times the smallest power of two 2^e,
+// e >= -126, with the block's largest finite |x| <= 448 2^e.  The scaling is exact, so the one rounding
+// is e4m3's (at most 2^-4 of the value, or 2^(e-10) for the smallest), and nothing saturates.  Infinite
+// and NaN elements are held as NaN.  33 bytes for 32 features against 64 (bf16) or 128 (fp32).
+//
+//  * act8_pack reads x once and writes the checkpoint and, where the product cannot take x as it is,
+//    act(x) as the product's operand (bf16, or the two fp16 planes of fp32).  It moves 8 features a
+//    thread; a block's maximum is two shuffles inside a quad of lanes.
+//  * act8_unpack writes act(c) for dw's product: the GELU is then computed once an element, not once
+//    for each of dw's row tiles.  bf16 holds an identity c exactly (four significant bits).
+//  * The three products are gemm_tile.h's; gelu'(c) is applied in dx's epilogue from the checkpoint.
+//    fp32: x, w and dy as two fp16 planes, three 16-bit products; an identity c fits one plane, so
+//    its dw takes two.
+#include "gemm_tile.h"
+#include "ops.h"
+
+namespace voda {
+
+namespace {
+
+using namespace gt;
+
+struct PackArgs {
+  const void* x;
+  int64_t ldx;
+  int rows, width, vec, gelu;
+  uint8_t* q;       // [rows][kq], kq = width up to whole blocks of 32; null: no checkpoint
+  uint8_t* qs;      // [rows][kq / 32]
+  int kq;
+  uint16_t* o;      // act(x): [rows][kq] bf16, or two fp16 planes; or null
+  int64_t plane;
+  const float* amax;
+  float* inv;
+};
+
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.4028235e38f; }
+
+__device__ __forceinline__ void load8(const PackArgs& p, bool f32, int64_t r, int c, float (&v)[8]) {
+  if (f32) {
+    const float* row = static_cast<const float*>(p.x) + r * p.ldx + c;
+    if (p.vec && c < p.width) {
+      const float4 a = *reinterpret_cast<const float4*>(row), b = *reinterpret_cast<const float4*>(row + 4);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = c + e < p.width ? row[e] : 0.f;
+    }
+  } else {
+    const uint16_t* row = static_cast<const uint16_t*>(p.x) + r * p.ldx + c;
+    if (p.vec && c < p.width) {
+      const uint4 u = *reinterpret_cast<const uint4*>(row);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[2 * e] = bf2f(w[e] & 0xffff);
+        v[2 * e + 1] = bf2f(w[e] >> 16);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = c + e < p.width ? bf2f(row[e]) : 0.f;
+    }
+  }
+}
+
+__device__ __forceinline__ uint4 pack8_bf16(const float (&v)[8]) {
+  uint32_t u[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) u[e] = uint32_t(f2bf(v[2 * e])) | (uint32_t(f2bf(v[2 * e + 1])) << 16);
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+
+// planes of 8 values; ``lo`` may be null (one plane)
+__device__ __forceinline__ void store8_planes(const float (&v)[8], float s, uint16_t* hi, uint16_t* lo) {
+  uint16_t h[8], l[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) split_safe(v[e], s, h[e], l[e]);
+  auto quad = [](const uint16_t* a) {
+    return make_uint4(a[0] | (uint32_t(a[1]) << 16), a[2] | (uint32_t(a[3]) << 16), a[4] | (uint32_t(a[5]) << 16),
+                      a[6] | (uint32_t(a[7]) << 16));
+  };
+  *reinterpret_cast<uint4*>(hi) = quad(h);
+  if (lo) *reinterpret_cast<uint4*>(lo) = quad(l);
+}
+
+template <bool F32>
+__global__ __launch_bounds__(256) void act8_pack_kernel(PackArgs p) {
+  __shared__ float lds[4];
+  float scale = 1.f;
+  if constexpr (F32) {
+    if (p.o) {  // |gelu(x)| <= |x|: x's scale serves act(x)
+      scale = split_scale(amax_of(p.amax, lds));
+      if (blockIdx.x == 0 && threadIdx.x == 0) *p.inv = pow2_inverse(scale);
+    }
+  }
+  const int eights = p.kq >> 3;  // a multiple of 4: a quad of lanes is one block of 32
+  const int64_t n = int64_t(p.rows) * eights;
+  const int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (t >= n) return;
+  const int64_t r = t / eights;
+  const int c = 8 * int(t - r * eights);
+  float v[8];
+  load8(p, F32, r, c, v);
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = fmaxf(m, finite(v[e]) ? fabsf(v[e]) : 0.f);
+  m = fmaxf(m, __shfl_xor(m, 1, 64));
+  m = fmaxf(m, __shfl_xor(m, 2, 64));
+  // m = 1.f 2^E <= 1.75 2^8 2^e
+  const uint32_t bits = __float_as_uint(m);
+  const int ex = max(int(bits >> 23) - 127 - 8 + int((bits & 0x7fffff) > 0x600000), -126);
+  const float inv = __uint_as_float(uint32_t(127 - ex) << 23);
+  float w[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = finite(v[e]) ? v[e] * inv : NAN;
+  uint32_t q0 = 0, q1 = 0;
+  q0 = __builtin_amdgcn_cvt_pk_fp8_f32(w[0], w[1], q0, false);
+  q0 = __builtin_amdgcn_cvt_pk_fp8_f32(w[2], w[3], q0, true);
+  q1 = __builtin_amdgcn_cvt_pk_fp8_f32(w[4], w[5], q1, false);
+  q1 = __builtin_amdgcn_cvt_pk_fp8_f32(w[6], w[7], q1, true);
+  if (p.q) {
+    *reinterpret_cast<uint2*>(p.q + 8 * t) = make_uint2(q0, q1);
+    if ((c & 31) == 0) p.qs[t >> 2] = uint8_t(ex + 127);
+  }
+  if (!p.o) return;
+  if (p.gelu) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = gelu_tanh_f(v[e]);
+  }
+  if constexpr (F32) store8_planes(v, scale, p.o + 8 * t, p.o + p.plane + 8 * t);
+  else *reinterpret_cast<uint4*>(p.o + 8 * t) = pack8_bf16(v);
+}
+
+struct UnpackArgs {
+  const uint8_t* q;
+  const uint8_t* qs;
+  int64_t n;       // groups of 8
+  int gelu, planes;
+  uint16_t* o;     // act(c): bf16, or one or two fp16 planes
+  int64_t plane;
+  const float* amax;
+  float* inv;
+};
+
+__device__ __forceinline__ void unpack8(const uint8_t* q, const uint8_t* qs, int64_t t, float (&v)[8]) {
+  const uint2 u = *reinterpret_cast<const uint2*>(q + 8 * t);
+  const float s = __uint_as_float(uint32_t(qs[t >> 2]) << 23);
+  v[0] = __builtin_amdgcn_cvt_f32_fp8(u.x, 0) * s;
+  v[1] = __builtin_amdgcn_cvt_f32_fp8(u.x, 1) * s;
+  v[2] = __builtin_amdgcn_cvt_f32_fp8(u.x, 2) * s;
+  v[3] = __builtin_amdgcn_cvt_f32_fp8(u.x, 3) * s;
+  v[4] = __builtin_amdgcn_cvt_f32_fp8(u.y, 0) * s;
+  v[5] = __builtin_amdgcn_cvt_f32_fp8(u.y, 1) * s;
+  v[6] = __builtin_amdgcn_cvt_f32_fp8(u.y, 2) * s;
+  v[7] = __builtin_amdgcn_cvt_f32_fp8(u.y, 3) * s;
+}
+
+template <bool F32>
+__global__ __launch_bounds__(256) void act8_unpack_kernel(UnpackArgs p) {
+  __shared__ float lds[4];
+  float scale = 1.f;
+  if constexpr (F32) {
+    scale = split_scale(amax_of(p.amax, lds));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.inv = pow2_inverse(scale);
+  }
+  const int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (t >= p.n) return;
+  float v[8];
+  unpack8(p.q, p.qs, t, v);
+  if (p.gelu) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = gelu_tanh_f(v[e]);
+  }
+  if constexpr (F32) store8_planes(v, scale, p.o + 8 * t, p.planes == 2 ? p.o + p.plane + 8 * t : nullptr);
+  else *reinterpret_cast<uint4*>(p.o + 8 * t) = pack8_bf16(v);
+}
+
+// checkpoint -> values in dt, [rows][width] contiguous
+template <bool F32>
+__global__ __launch_bounds__(256) void act8_values_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ qs,
+                                                          int64_t n, int kq, int width, void* __restrict__ out) {
+  const int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (t >= n) return;
+  float v[8];
+  unpack8(q, qs, t, v);
+  const int eights = kq >> 3;
+  const int64_t r = t / eights;
+  const int c = 8 * int(t - r * eights);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (c + e >= width) break;
+    if constexpr (F32) static_cast<float*>(out)[r * width + c + e] = v[e];
+    else static_cast<uint16_t*>(out)[r * width + c + e] = f2bf(v[e]);
+  }
+}
+
+unsigned blocks(int64_t threads) { return unsigned((threads + 255) / 256); }
+
+struct Act8Plan {
+  int kq, np8, kp;               // features up to 32, outputs up to 8, features up to 8
+  int y_tile, dx_tile, y_s, dx_s, dw_s;
+  bool copy;                     // the forward's product reads a copy that act8_pack writes
+  // forward workspace: planes' inverse scales, x's operand, w's planes, slab
+  int64_t f_inv, f_x, f_w, f_slab, fwd;
+  // backward workspace: dy's maxima, inverse scales, dy's planes, w's planes, act(c), slabs
+  int64_t b_amax, b_inv, b_dy, b_w, b_c, b_dx, b_dw, b_db, bwd;
+};
+
+Act8Plan act8_plan(int64_t rows, int64_t width, int64_t out, bool f32, bool copy) {
+  Act8Plan q{};
+  q.kq = int(up(width, 32));
+  q.kp = int(up(width, 8));
+  q.np8 = int(up(out, 8));
+  q.copy = copy;
+  // a product's tile and the splits of its reduction: whole reductions where the tiles alone give
+  // every other CU one
+  auto tile = [&](int64_t ni) { return ni <= 32 ? kFew : kBig; };
+  auto splits = [&](int64_t tiles, int64_t nk, int64_t least) { return tiles >= 192 ? 1 : splits_for(tiles, nk, least); };
+  q.y_tile = q.dx_tile = tile(rows);
+  q.y_s = splits(tiles_of(q.y_tile, rows, out), width, 256);
+  q.dx_s = splits(tiles_of(q.dx_tile, rows, width), out, 256);
+  q.dw_s = splits(tiles_of(kBig, out, width), rows, 256);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at = up(at + bytes, 256);
+    return o;
+  };
+  q.f_inv = take(f32 ? 16 : 0);
+  q.f_x = take(copy ? rows * q.kq * (f32 ? 4 : 2) : 0);
+  q.f_w = take(f32 ? out * q.kp * 4 : 0);
+  q.f_slab = take(q.y_s > 1 ? q.y_s * rows * up(out, 4) * 4 : 0);
+  q.fwd = at;
+  at = 0;
+  q.b_amax = take(f32 ? kAmaxBlocks * 4 : 0);
+  q.b_inv = take(f32 ? 16 : 0);
+  q.b_dy = take(f32 ? rows * q.np8 * 4 : 0);
+  q.b_w = take(f32 ? out * q.kp * 4 : 0);
+  q.b_c = take(rows * q.kq * (f32 ? 4 : 2));
+  q.b_dx = take(q.dx_s > 1 ? q.dx_s * rows * q.kp * 4 : 0);
+  q.b_dw = take(q.dw_s > 1 ? q.dw_s * out * q.kp * 4 : 0);
+  q.b_db = take(q.dw_s > 1 ? q.dw_s * out * 4 : 0);
+  q.bwd = at;
+  return q;
+}
+
+void check_act8(int64_t rows, int64_t width, int64_t out, int dt) {
+  VODA_CHECK(rows > 0 && rows < (1 << 30) && width > 0 && width <= (1 << 20) && out > 0 && out <= (1 << 20),
+             "linear_act8: sizes out of range");
+  VODA_CHECK(up(rows, 32) / 32 * (up(width > out ? width : out, 128) / 128) < (int64_t(1) << 31) &&
+                 up(rows * up(width, 32), 256) / 256 < (int64_t(1) << 31),
+             "linear_act8: rows x features too large");
+  VODA_CHECK(dt == kF32 || dt == kBF16, "linear_act8: fp32 or bf16");
+}
+
+FinishArgs finish_args(const GemmArgs& a, int splits) {
+  FinishArgs f{};
+  f.slab = a.slab;
+  f.lds = a.lds;
+  f.splits = splits;
+  f.slab_rows = f.rows = a.I.n;
+  f.bslab = a.bslab;
+  f.e = a.e;
+  return f;
+}
+
+}  // namespace
+
+// (forward workspace, backward workspace) bytes, features up to 32, outputs up to 8
+std::vector<int64_t> linear_act8_sizes(int64_t rows, int64_t width, int64_t out, int dt, bool copy) {
+  check_act8(rows, width, out, dt);
+  const Act8Plan q = act8_plan(rows, width, out, dt == kF32, copy);
+  return {q.fwd, q.bwd, q.kq, q.np8};
+}
+
+void act8_pack(uintptr_t x, int64_t ldx, int64_t rows, int64_t width, int dt, uintptr_t qp, uintptr_t qs,
+               uintptr_t stream) {
+  check_act8(rows, width, 1, dt);
+  VODA_CHECK(qp % 16 == 0, "act8: checkpoint must be 16-byte aligned");
+  PackArgs p{};
+  p.x = reinterpret_cast<const void*>(x);
+  p.ldx = ldx;
+  p.rows = int(rows);
+  p.width = int(width);
+  p.vec = x % 16 == 0 && ldx % 8 == 0 && width % 8 == 0;
+  p.q = reinterpret_cast<uint8_t*>(qp);
+  p.qs = reinterpret_cast<uint8_t*>(qs);
+  p.kq = int(up(width, 32));
+  const dim3 grid(blocks(rows * (p.kq >> 3)));
+  if (dt == kF32) hipLaunchKernelGGL((act8_pack_kernel<true>), grid, dim3(256), 0, as_stream(stream), p);
+  else hipLaunchKernelGGL((act8_pack_kernel<false>), grid, dim3(256), 0, as_stream(stream), p);
+  check_launch();
+}
+
+void act8_values(uintptr_t qp, uintptr_t qs, int64_t rows, int64_t width, int dt, uintptr_t out, uintptr_t stream) {
+  check_act8(rows, width, 1, dt);
+  VODA_CHECK(qp % 16 == 0, "act8: checkpoint must be 16-byte aligned");
+  const int kq = int(up(width, 32));
+  const int64_t n = rows * (kq >> 3);
+  if (dt == kF32)
+    hipLaunchKernelGGL((act8_values_kernel<true>), dim3(blocks(n)), dim3(256), 0, as_stream(stream),
+                       reinterpret_cast<const uint8_t*>(qp), reinterpret_cast<const uint8_t*>(qs), n, kq, int(width),
+                       reinterpret_cast<void*>(out));
+  else
+    hipLaunchKernelGGL((act8_values_kernel<false>), dim3(blocks(n)), dim3(256), 0, as_stream(stream),
+                       reinterpret_cast<const uint8_t*>(qp), reinterpret_cast<const uint8_t*>(qs), n, kq, int(width),
+                       reinterpret_cast<void*>(out));
+  check_launch();
+}
+
+// y [rows][out] contiguous; the checkpoint (q, qs) is written where q is not null; ``amax`` (fp32):
+// 2 kAmaxBlocks floats, kept for the backward.
+void linear_act8_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr_t bias, int bias_dt, uintptr_t y,
+                     uintptr_t qp, uintptr_t qs, int64_t rows, int64_t width, int64_t out, int dt, bool gelu, bool copy,
+                     uintptr_t amax, uintptr_t ws, uintptr_t stream) {
+  check_act8(rows, width, out, dt);
+  const bool f32 = dt == kF32;
+  VODA_CHECK(f32 || (w % 16 == 0 && ldw % 8 == 0 && ldw >= up(width, 8)),
+             "linear_act8: bf16 weight rows must be 16-byte aligned and whole 16-byte vectors");
+  VODA_CHECK(copy || (!f32 && !gelu && x % 16 == 0 && ldx % 8 == 0 && width % 8 == 0),
+             "linear_act8: this input needs a copy");
+  VODA_CHECK(qp % 16 == 0 && ws % 256 == 0, "linear_act8: workspaces must be aligned");
+  const Act8Plan q = act8_plan(rows, width, out, f32, copy);
+  hipStream_t st = as_stream(stream);
+  uint8_t* base = reinterpret_cast<uint8_t*>(ws);
+  float* inv = reinterpret_cast<float*>(base + q.f_inv);
+  float* am = reinterpret_cast<float*>(amax);
+  const Rows rw = {reinterpret_cast<const float*>(w), ldw, int(out), int(width)};
+  if (f32) gt::amax({reinterpret_cast<const float*>(x), ldx, int(rows), int(width)}, &rw, nullptr, 0, 0, am, st);
+  PackArgs p{};
+  p.x = reinterpret_cast<const void*>(x);
+  p.ldx = ldx;
+  p.rows = int(rows);
+  p.width = int(width);
+  p.vec = x % 16 == 0 && ldx % 8 == 0 && width % 8 == 0;
+  p.gelu = gelu;
+  p.q = reinterpret_cast<uint8_t*>(qp);
+  p.qs = reinterpret_cast<uint8_t*>(qs);
+  p.kq = q.kq;
+  p.o = copy ? reinterpret_cast<uint16_t*>(base + q.f_x) : nullptr;
+  p.plane = rows * q.kq;
+  p.amax = am;
+  p.inv = inv;
+  if (p.q || p.o) {
+    const dim3 grid(blocks(rows * (q.kq >> 3)));
+    if (f32) hipLaunchKernelGGL((act8_pack_kernel<true>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((act8_pack_kernel<false>), grid, dim3(256), 0, st, p);
+    check_launch();
+  }
+  GemmArgs a{};
+  a.I = copy ? Operand{p.o, q.kq, p.plane, int(rows)} : Operand{reinterpret_cast<const uint16_t*>(x), ldx, 0, int(rows)};
+  a.J = {reinterpret_cast<const uint16_t*>(w), ldw, 0, int(out)};
+  if (f32) {
+    uint16_t* wp = reinterpret_cast<uint16_t*>(base + q.f_w);
+    split(rw, wp, q.kp, out * q.kp, am + kAmaxBlocks, inv + 1, st);
+    a.J = {wp, q.kp, out * q.kp, int(out)};
+    a.e.fi = inv;
+    a.e.fj = inv + 1;
+  }
+  a.nk = q.kp;
+  a.o.gi = 8;
+  a.o.splits = q.y_s;
+  a.e.f = 1.f;
+  a.e.out = reinterpret_cast<void*>(y);
+  a.e.ldo = out;
+  a.e.bf16 = !f32;
+  a.e.nj = int(out);
+  a.e.vec = out % 4 == 0 && y % 16 == 0;
+  a.e.zero_from = 0x7fffffff;
+  a.e.bias = reinterpret_cast<const void*>(bias);
+  a.e.bias_bf16 = bias_dt == kBF16;
+  if (q.y_s > 1) {
+    a.slab = reinterpret_cast<float*>(base + q.f_slab);
+    a.lds = up(out, 4);
+  }
+  if (q.y_tile == kFew) {
+    if (f32) gemm<Few<true, 3, false, false>, false>(a, st);
+    else gemm<Few<false, 1, false, false>, false>(a, st);
+  } else {
+    if (f32) gemm<Big<true, 3, false, false>, false>(a, st);
+    else gemm<Big<false, 1, false, false>, false>(a, st);
+  }
+  if (q.y_s > 1) finish(finish_args(a, q.y_s), st);
+}
+
+// dx [rows][ldo] in x's type (added to when ``dx_add``); dw [out][ldd] and db [out] in ``grad_dt``
+// (added to when ``accumulate``); dx, db, or dw and db may be null.  dy: bf16 rows of whole 16-byte vectors.
+void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintptr_t qp, uintptr_t qs, uintptr_t dx,
+                     bool dx_add, uintptr_t dw, int64_t ldd, uintptr_t db, int grad_dt, bool accumulate, int64_t rows,
+                     int64_t width, int64_t out, int dt, bool gelu, uintptr_t amax, uintptr_t ws, uintptr_t stream) {
+  check_act8(rows, width, out, dt);
+  const bool f32 = dt == kF32;
+  VODA_CHECK(grad_dt == kF32 || grad_dt == kBF16, "linear_act8: weight gradients must be fp32 or bf16");
+  VODA_CHECK(f32 || (w % 16 == 0 && ldw % 8 == 0 && ldw >= up(width, 8)),
+             "linear_act8: bf16 weight rows must be 16-byte aligned and whole 16-byte vectors");
+  VODA_CHECK(f32 || (dy % 16 == 0 && ldy % 8 == 0 && ldy >= up(out, 8)),
+             "linear_act8: bf16 gradient rows must be 16-byte aligned and whole 16-byte vectors");
+  VODA_CHECK(qp % 16 == 0 && ws % 256 == 0, "linear_act8: workspaces must be aligned");
+  const Act8Plan q = act8_plan(rows, width, out, f32, true);
+  hipStream_t st = as_stream(stream);
+  uint8_t* base = reinterpret_cast<uint8_t*>(ws);
+  float* inv = reinterpret_cast<float*>(base + q.b_inv);  // of dy, w, act(c)
+  const float* am = reinterpret_cast<const float*>(amax);
+  const uint8_t* q8 = reinterpret_cast<const uint8_t*>(qp);
+  const uint8_t* s8 = reinterpret_cast<const uint8_t*>(qs);
+  Operand DY = {reinterpret_cast<const uint16_t*>(dy), ldy, 0, int(rows)};
+  Operand W = {reinterpret_cast<const uint16_t*>(w), ldw, 0, int(out)};
+  if (f32) {
+    const Rows rdy = {reinterpret_cast<const float*>(dy), ldy, int(rows), int(out)};
+    float* dam = reinterpret_cast<float*>(base + q.b_amax);
+    gt::amax(rdy, nullptr, nullptr, 0, 0, dam, st);
+    uint16_t* dyp = reinterpret_cast<uint16_t*>(base + q.b_dy);
+    split(rdy, dyp, q.np8, rows * q.np8, dam, inv, st);
+    DY = {dyp, q.np8, rows * q.np8, int(rows)};
+    if (dx) {
+      uint16_t* wp = reinterpret_cast<uint16_t*>(base + q.b_w);
+      split({reinterpret_cast<const float*>(w), ldw, int(out), int(width)}, wp, q.kp, out * q.kp, am + kAmaxBlocks, inv + 1,
+            st);
+      W = {wp, q.kp, out * q.kp, int(out)};
+    }
+  }
+  if (dx) {
+    GemmArgs a{};
+    a.I = DY;
+    a.J = W;
+    a.J.n = q.kp;  // columns: W is read down its rows
+    a.nk = int(out);
+    a.o.gi = 8;
+    a.o.splits = q.dx_s;
+    a.e.f = 1.f;
+    a.e.fi = f32 ? inv : nullptr;
+    a.e.fj = f32 ? inv + 1 : nullptr;
+    a.e.out = reinterpret_cast<void*>(dx);
+    a.e.ldo = width;
+    a.e.bf16 = !f32;
+    a.e.nj = int(width);
+    a.e.vec = width % 4 == 0 && dx % 16 == 0;
+    a.e.accumulate = dx_add;
+    a.e.zero_from = 0x7fffffff;
+    if (gelu) {
+      a.e.q = q8;
+      a.e.qs = s8;
+      a.e.ldq = q.kq;
+    }
+    if (q.dx_s > 1) {
+      a.slab = reinterpret_cast<float*>(base + q.b_dx);
+      a.lds = q.kp;
+    }
+    if (q.dx_tile == kFew) {
+      if (f32) gemm<Few<true, 3, false, true>, false>(a, st);
+      else gemm<Few<false, 1, false, true>, false>(a, st);
+    } else {
+      if (f32) gemm<Big<true, 3, false, true>, false>(a, st);
+      else gemm<Big<false, 1, false, true>, false>(a, st);
+    }
+    if (q.dx_s > 1) finish(finish_args(a, q.dx_s), st);
+  }
+  if (!dw) return;
+  UnpackArgs u{};
+  u.q = q8;
+  u.qs = s8;
+  u.n = rows * (q.kq >> 3);
+  u.gelu = gelu;
+  u.planes = gelu ? 2 : 1;
+  u.o = reinterpret_cast<uint16_t*>(base + q.b_c);
+  u.plane = rows * q.kq;
+  u.amax = am;
+  u.inv = inv + 2;
+  if (f32) hipLaunchKernelGGL((act8_unpack_kernel<true>), dim3(blocks(u.n)), dim3(256), 0, st, u);
+  else hipLaunchKernelGGL((act8_unpack_kernel<false>), dim3(blocks(u.n)), dim3(256), 0, st, u);
+  check_launch();
+  GemmArgs a{};
+  a.I = DY;
+  a.I.n = int(out);
+  a.J = {u.o, q.kq, u.plane, q.kq};
+  a.nk = int(rows);
+  a.o.gi = 8;
+  a.o.splits = q.dw_s;
+  a.e.f = 1.f;
+  a.e.fi = f32 ? inv : nullptr;
+  a.e.fj = f32 ? inv + 2 : nullptr;
+  a.e.out = reinterpret_cast<void*>(dw);
+  a.e.ldo = ldd;
+  a.e.bf16 = grad_dt == kBF16;
+  a.e.nj = int(width);
+  a.e.vec = ldd % 4 == 0 && dw % 16 == 0;
+  a.e.accumulate = accumulate;
+  a.e.zero_from = 0x7fffffff;
+  void* dbp = reinterpret_cast<void*>(db);
+  if (q.dw_s > 1) {
+    a.slab = reinterpret_cast<float*>(base + q.b_dw);
+    a.lds = q.kp;
+    a.bslab = db ? reinterpret_cast<float*>(base + q.b_db) : nullptr;
+  } else {
+    a.bout = dbp;
+  }
+  if (f32 && gelu) gemm<Big<true, 3, true, true>, true>(a, st);
+  else if (f32) gemm<Big<true, 2, true, true>, true>(a, st);
+  else gemm<Big<false, 1, true, true>, true>(a, st);
+  if (q.dw_s > 1) {
+    FinishArgs f = finish_args(a, q.dw_s);
+    f.bout = dbp;
+    finish(f, st);
+  }
+}
+
+}  // namespace voda

@@ -46,6 +46,14 @@ PYBIND11_MODULE(_vodahip, m) {
   m.def("masked_softmax_bwd", &masked_softmax_bwd);
   m.def("xent_fwd", &xent_fwd);
   m.def("xent_bwd", &xent_bwd);
+  m.def("linear_xent_sizes", &linear_xent_sizes);
+  m.def("linear_xent_fwd", &linear_xent_fwd);
+  m.def("linear_xent_bwd", &linear_xent_bwd);
+  m.def("linear_act8_sizes", &linear_act8_sizes);
+  m.def("act8_pack", &act8_pack);
+  m.def("act8_values", &act8_values);
+  m.def("linear_act8_fwd", &linear_act8_fwd);
+  m.def("linear_act8_bwd", &linear_act8_bwd);
 
   m.def("bn_workspace_floats", &bn_workspace_floats);
   m.def("bn_set_tuning", &bn_set_tuning, py::arg("deep") = -1, py::arg("blocks") = -1, py::arg("sweep") = -1);

@@ -1,0 +1,690 @@
+// Tiled matrix products on the 16-bit matrix cores (CDNA4, gfx950) with the epilogue left to the
+// caller: the main loop of the vocabulary head's loss (linear_xent.hip) and of the Linear layer
+// with an 8-bit input checkpoint (act8.hip).
+//
+//   C[i][j] = sum_k I(i, k) J(j, k)        fp32 accumulators, 16-bit operands
+//
+//  * An operand is "row" (k contiguous: I[i][k]) or "col" (k outermost: I[k][i]).  A row operand's
+//    stage is kept as rows of BK elements, their 16-byte chunks XOR-swizzled, and read with
+//    ds_read_b128; a col operand's as panels of 128 columns, read with the transposing
+//    ds_read_b64_tr_b16.  So x w^T (row, row), dy w (row, col) and dy^T x (col, col) share one loop
+//    and nothing is transposed in memory.
+//  * v_mfma_f32_32x32x16 with J as its first operand: a lane then holds ONE row i (lane & 31) and
+//    four consecutive columns j in each register quad, so a softmax over j is nearly all in-lane and
+//    a store moves 8 or 16 bytes.
+//  * Stages of BK reduction steps arrive in a ring of ST LDS buffers by 16-byte LDS-DMA (no staging
+//    registers); ST - 1 stages are in flight, one barrier a stage.  Chunks past the reduction's end
+//    read a zero buffer; rows past an operand's end read its last row (never stored).
+//  * fp32 operands run as two fp16 planes, x 2^a = hi + 2^-11 lo: hi is x's first 11 bits, lo the
+//    next 11, so an element is held to 2^-24 of its size, or 2^-50 of the largest element where that
+//    is more (a: the power of two that brings the tensor's largest element to [2^14, 2^15)).
+//    Three products: hi.lo and lo.hi first, one exact scaling of the accumulators by 2^-11, then
+//    hi.hi; lo.lo, 2^-24 of the result, is left out.  Half the matrix work of a three-way bf16 split.
+#pragma once
+
+#include "common.h"
+
+namespace voda {
+namespace gt {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x4_v __attribute__((__vector_size__(4 * sizeof(__bf16))));
+typedef __attribute__((address_space(3))) bf16x4_v lds_bf16x4;
+typedef __attribute__((address_space(3))) void lds_void;
+
+constexpr float kLoScale = 1.f / 2048.f;  // weight of a lo plane
+constexpr int kSplitExp = 15;             // hi planes: the largest element lies below 2^15
+
+// what chunks past a reduction's end read
+static __device__ __attribute__((aligned(16))) uint32_t zero_chunk[4];
+
+struct Operand {
+  const uint16_t* p;
+  int64_t ld;     // elements between rows (row operand: between i; col operand: between k)
+  int64_t plane;  // elements between the hi and the lo plane
+  int n;          // rows i (>= 1)
+};
+
+__device__ __forceinline__ void dma16(const void* gptr, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gptr), "s"(lds_addr) : "memory", "m0");
+}
+
+template <int N>
+__device__ __forceinline__ void wait_vm_barrier() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// byte offset of 16-byte chunk ``ch`` (0..15) of row ``r`` of a 128-column panel (col operands)
+__device__ __forceinline__ int panel_off(int r, int ch) {
+  return r * 256 + 16 * (ch ^ (((r & 3) << 2) | ((r >> 2) & 3)));
+}
+
+__device__ __forceinline__ uint2 tr_read(const uint8_t* base, int off) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(base + off)));
+}
+
+template <bool F16>
+__device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// One operand's stage in LDS: EXT rows i x BK reduction steps, filled by NW waves, read by waves
+// whose sub-tile is T 32-row tiles from row ``sub`` on.
+template <bool COL, int EXT, int BK, int NW, int T>
+struct Stage {
+  static constexpr int kBytes = EXT * BK * 2;
+  static constexpr int kInstr = kBytes / 1024;  // 1 KB wave-instructions
+  static constexpr int kPer = kInstr / NW;      // per wave
+  static_assert(kInstr % NW == 0, "a stage is whole wave-instructions for every wave");
+  static_assert(!COL || EXT % 128 == 0, "col operands come in panels of 128");
+  static constexpr int CPR = BK / 8;            // row operands: chunks a row
+  static constexpr int RPI = 64 / CPR;          // rows a wave-instruction
+
+  const uint16_t* src[kPer];
+  int off[COL ? 2 * T : BK / 16];
+
+  static __device__ __forceinline__ int swz(int row) { return (row / (8 / (CPR < 8 ? CPR : 8))) & (CPR - 1); }
+
+  // place of this lane's chunk in wave-instruction q: its row / column and k inside the stage
+  static __device__ __forceinline__ void place(int q, int lane, int& r, int& k) {
+    if constexpr (COL) {
+      const int panel = q / (BK / 4), rq = q % (BK / 4);
+      k = 4 * rq + (lane >> 4);
+      r = panel * 128 + 8 * ((lane & 15) ^ (((k & 3) << 2) | ((k >> 2) & 3)));
+    } else {
+      const int row = q * RPI + lane / CPR;
+      r = row;
+      k = 8 * ((lane % CPR) ^ swz(row));
+    }
+  }
+
+  __device__ __forceinline__ void init(const Operand& o, int r0, int k0, int wave, int lane, int sub) {
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      int r, k;
+      place(wave * kPer + u, lane, r, k);
+      if constexpr (COL)  // a chunk of 8 columns past the end: zeros, never stored
+        src[u] = r0 + r < o.n ? o.p + int64_t(k0 + k) * o.ld + r0 + r : nullptr;
+      else
+        src[u] = o.p + int64_t(min(r0 + r, o.n - 1)) * o.ld + k0 + k;
+    }
+    const int h = lane >> 5;
+    if constexpr (COL) {
+      const int g = lane >> 4, q = (lane & 15) >> 2, pp = lane & 3;
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        const int c = sub + 32 * t;  // first column of the tile inside the stage
+        const int base = (c >> 7) * (BK * 256) + 8 * (pp & 1);
+        const int ch = ((c & 127) >> 3) + 2 * (g & 1) + (pp >> 1);
+        off[2 * t] = base + panel_off(8 * h + q, ch);
+        off[2 * t + 1] = base + panel_off(8 * h + q + 4, ch);
+      }
+    } else {
+      const int row = sub + (lane & 31);
+#pragma unroll
+      for (int kk = 0; kk < BK / 16; ++kk) off[kk] = row * (BK * 2) + 16 * ((2 * kk + h) ^ swz(row));
+    }
+  }
+
+  // fill: ``shift`` elements from the stage-0 addresses, ``left`` reduction steps remain
+  __device__ __forceinline__ void issue(uint8_t* lds, int64_t shift, int left, int wave, int lane) const {
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int q = wave * kPer + u;
+      int r, k;
+      place(q, lane, r, k);
+      const bool ok = k < left && (!COL || src[u] != nullptr);
+      dma16(ok ? static_cast<const void*>(src[u] + shift) : zero_chunk, __builtin_amdgcn_readfirstlane(uint32_t(size_t((lds_void*)(lds + 1024 * q)))));
+    }
+  }
+
+  __device__ __forceinline__ uint4 frag(const uint8_t* lds, int t, int kk) const {
+    if constexpr (COL) {
+      const uint2 lo = tr_read(lds + 4096 * kk, off[2 * t]), hi = tr_read(lds + 4096 * kk, off[2 * t + 1]);
+      return make_uint4(lo.x, lo.y, hi.x, hi.y);
+    } else {
+      return *reinterpret_cast<const uint4*>(lds + off[kk] + t * (64 * BK));
+    }
+  }
+};
+
+// Tile of WJ x WI waves, each TJ x TI 32 x 32 blocks: BJ = 32 WJ TJ columns, BI = 32 WI TI rows.
+// NP products: 1 (plain 16-bit operands), 2 (I in two planes, J in one), 3 (both in two planes).
+template <bool F16, int NP, bool IT, bool JT, int WJ_, int WI_, int TJ_, int TI_, int BK_, int ST_>
+struct Tile {
+  static constexpr int WJ = WJ_, WI = WI_, TJ = TJ_, TI = TI_, BK = BK_, ST = ST_;
+  static constexpr int NW = WJ * WI, kThreads = 64 * NW;
+  static constexpr int BJ = 32 * WJ * TJ, BI = 32 * WI * TI;
+  using SI = Stage<IT, BI, BK, NW, TI>;
+  using SJ = Stage<JT, BJ, BK, NW, TJ>;
+  static constexpr int kStage = SI::kBytes + SJ::kBytes;
+  static constexpr int kLds = ST * kStage;
+  static constexpr int kPer = SI::kPer + SJ::kPer;
+  static_assert(ST >= 2 && (ST - 2) * kPer < 64, "ring depth");
+
+  struct Where {
+    int lane, wave, h, il, wi, wj;
+    __device__ __forceinline__ Where() {
+      lane = threadIdx.x & 63;
+      wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+      h = lane >> 5;
+      il = lane & 31;
+      wj = wave % WJ;
+      wi = wave / WJ;
+    }
+    // row i of block ti and first column of register quad g of block tj, inside the tile
+    __device__ __forceinline__ int i(int ti) const { return (wi * TI + ti) * 32 + il; }
+    __device__ __forceinline__ int j(int tj, int g) const { return (wj * TJ + tj) * 32 + 8 * g + 4 * h; }
+  };
+
+  // acc[tj][ti] = the tile's products over k in [k0, k1).  SUM and ``want``: also the sums of I over k
+  // (of its planes' value, in hi units) for this lane's rows i; half h of the wave holds half of them.
+  template <bool SUM>
+  static __device__ __forceinline__ void run(uint8_t* smem, const Operand& I, const Operand& J, int i0, int j0, int k0,
+                                             int k1, f32x16 (&acc)[TJ][TI], float (&isum)[TI], bool want = false) {
+    const Where w;
+    SI si;
+    SJ sj;
+    si.init(I, i0, k0, w.wave, w.lane, w.wi * TI * 32);
+    sj.init(J, j0, k0, w.wave, w.lane, w.wj * TJ * 32);
+#pragma unroll
+    for (int a = 0; a < TJ; ++a)
+#pragma unroll
+      for (int b = 0; b < TI; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
+#pragma unroll
+    for (int b = 0; b < TI; ++b) isum[b] = 0.f;
+    const int steps = k1 > k0 ? (k1 - k0 + BK - 1) / BK : 0;
+    const int total = NP * steps;
+    const int64_t stepi = IT ? BK * I.ld : BK, stepj = JT ? BK * J.ld : BK;
+    int at = 0, prod = 0;  // next stage to issue: its step and product
+    auto issue = [&](int buf) {
+      // plane of each operand in product ``prod``; the last product is hi.hi
+      const bool lo_i = NP == 3 ? prod == 1 : NP == 2 ? prod == 0 : false;
+      const bool lo_j = NP == 3 && prod == 0;
+      uint8_t* lds = smem + buf * kStage;
+      const int left = k1 - k0 - at * BK;
+      si.issue(lds, at * stepi + (lo_i ? I.plane : 0), left, w.wave, w.lane);
+      sj.issue(lds + SI::kBytes, at * stepj + (lo_j ? J.plane : 0), left, w.wave, w.lane);
+      if (++at == steps) { at = 0; ++prod; }
+    };
+    int fill = 0;  // buffer of the next stage to issue
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s) {
+      if (s < total) issue(fill);
+      ++fill;
+    }
+    int buf = 0;
+    for (int st = 0; st < total; ++st) {
+      // stage st is whole once at most the later issued stages are outstanding; past the barrier
+      // every wave is done with the buffer that is refilled next
+      if (ST > 2 && st + ST - 2 < total) wait_vm_barrier<(ST - 2) * kPer>();
+      else if (ST > 3 && st + ST - 3 < total) wait_vm_barrier<(ST > 3 ? ST - 3 : 0) * kPer>();
+      else wait_vm_barrier<0>();
+      if (st + ST - 1 < total) issue(fill);
+      fill = fill + 1 == ST ? 0 : fill + 1;
+      if (NP > 1 && st == (NP - 1) * steps) {
+#pragma unroll
+        for (int a = 0; a < TJ; ++a)
+#pragma unroll
+          for (int b = 0; b < TI; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[a][b][r] *= kLoScale;
+      }
+      const uint8_t* li = smem + buf * kStage;
+      const uint8_t* lj = li + SI::kBytes;
+      uint4 fi[2][TI], fj[2][TJ];
+#pragma unroll
+      for (int b = 0; b < TI; ++b) fi[0][b] = si.frag(li, b, 0);
+#pragma unroll
+      for (int a = 0; a < TJ; ++a) fj[0][a] = sj.frag(lj, a, 0);
+#pragma unroll
+      for (int kk = 0; kk < BK / 16; ++kk) {
+        if (kk + 1 < BK / 16) {
+#pragma unroll
+          for (int b = 0; b < TI; ++b) fi[(kk + 1) & 1][b] = si.frag(li, b, kk + 1);
+#pragma unroll
+          for (int a = 0; a < TJ; ++a) fj[(kk + 1) & 1][a] = sj.frag(lj, a, kk + 1);
+        }
+#pragma unroll
+        for (int a = 0; a < TJ; ++a)
+#pragma unroll
+          for (int b = 0; b < TI; ++b) acc[a][b] = mfma<F16>(fj[kk & 1][a], fi[kk & 1][b], acc[a][b]);
+        if constexpr (SUM) {
+          // the reduction's sum of I: the hi plane in the last product, lo where it runs with J's hi
+          const bool lo = NP == 3 ? st >= steps && st < 2 * steps : NP == 2 ? st < steps : false;
+          if (want && (lo || st >= (NP - 1) * steps)) {
+#pragma unroll
+            for (int b = 0; b < TI; ++b) {
+              const uint32_t u[4] = {fi[kk & 1][b].x, fi[kk & 1][b].y, fi[kk & 1][b].z, fi[kk & 1][b].w};
+              float s = 0.f;
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                s += F16 ? h2f(u[e] & 0xffff) + h2f(u[e] >> 16) : bf2f(u[e] & 0xffff) + bf2f(u[e] >> 16);
+              isum[b] += lo ? s * kLoScale : s;
+            }
+          }
+        }
+      }
+      buf = buf + 1 == ST ? 0 : buf + 1;
+    }
+  }
+};
+
+// Tiles in the order that an XCD's L2 serves best: workgroups are dealt to the 8 XCDs in turn, so
+// each XCD gets one run of the order; inside it, groups of ``gi`` row tiles stay while the column
+// tiles go by.
+struct Order {
+  int ti, tj, gi, splits;
+  __device__ __forceinline__ void at(int bid, int grid, int& i, int& j, int& s) const {
+    const int x = bid & 7, q = grid >> 3, r = grid & 7;
+    const int t = x * q + min(x, r) + (bid >> 3);
+    const int tiles = ti * tj;
+    s = t / tiles;
+    const int u = t - s * tiles;
+    const int per = gi * tj, grp = u / per, v = u - grp * per;
+    const int rows = min(gi, ti - grp * gi);
+    j = v / rows;
+    i = grp * gi + (v - j * rows);
+  }
+};
+
+// fp32 -> its two planes, of x 2^a
+__device__ __forceinline__ void split2(float xs, uint16_t& hi, uint16_t& lo) {
+  const _Float16 h = static_cast<_Float16>(xs);
+  hi = __builtin_bit_cast(uint16_t, h);
+  lo = f2h((xs - static_cast<float>(h)) * 2048.f);
+}
+
+// 2^a for a tensor whose largest finite |element| is amax: amax 2^a in [2^14, 2^15)
+__device__ __forceinline__ float split_scale(float amax) {
+  if (!(amax > 0.f)) return 1.f;
+  const int e = int((__float_as_uint(amax) >> 23) & 255) - 127;  // floor(log2); subnormal: -127
+  return __uint_as_float(uint32_t(min(kSplitExp - 1 - e, 126) + 127) << 23);
+}
+
+// 1 / 2^a, exact (2^a is between 2^-113 and 2^126)
+__device__ __forceinline__ float pow2_inverse(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
+
+// ---- stores -----------------------------------------------------------------------------------
+
+// What becomes of a product: out = (sum of its splits) * factors [* gelu'(checkpoint)] [+ bias]
+// [+ out], in fp32 until the one rounding to out's type.
+struct Emit {
+  void* out;
+  int64_t ldo;
+  int bf16;                 // out's type: bf16 or fp32
+  int nj;                   // columns
+  int vec;                  // rows start 4-element aligned: quads go out as one store
+  int accumulate;           // add to what out holds
+  int zero_from;            // rows i >= zero_from are zero
+  const void* bias;         // [nj], or null
+  int bias_bf16;
+  const uint8_t* q;         // e4m3 checkpoint [i][ldq] whose gelu' multiplies, or null
+  const uint8_t* qs;        // its scales [i][ldq / 32]
+  int64_t ldq;
+  // factors: f times I's and J's inverse plane scales times *gl / max(*gn, 1), each pointer or null
+  float f;
+  const float* fi;
+  const float* fj;
+  const float* gl;
+  const int* gn;
+
+  // ``with_j`` false: of a sum over I alone
+  __device__ __forceinline__ float scaled(float v, bool with_j = true) const {
+    // one after the other: a product of two factors may leave fp32's range where the result does not
+    v *= f;
+    if (fi) v *= *fi;
+    if (fj && with_j) v *= *fj;
+    if (gl) v *= *gl / float(max(*gn, 1));
+    return v;
+  }
+  __device__ __forceinline__ void quad(int i, int j, float (&v)[4], bool keep = true) const;
+};
+
+// gelu_tanh'(c) to fp32 accuracy (common.h's form: 1 ulp exp2 and reciprocal)
+// ``keep`` false: the row is zero whatever the factors are.
+__device__ __forceinline__ void Emit::quad(int i, int j, float (&v)[4], bool keep) const {
+  if (j >= nj) return;
+  keep = keep && i < zero_from;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = keep ? scaled(v[e]) : 0.f;
+  if (q) {
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(q + int64_t(i) * ldq + j);  // ldq % 32 == 0, j % 4 == 0
+    const float s = __uint_as_float(uint32_t(qs[int64_t(i) * (ldq >> 5) + (j >> 5)]) << 23);
+    v[0] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u, 0) * s);
+    v[1] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u, 1) * s);
+    v[2] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u, 2) * s);
+    v[3] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u, 3) * s);
+  }
+  const int n = min(4, nj - j);
+  if (bias) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < n)
+        v[e] += bias_bf16 ? bf2f(static_cast<const uint16_t*>(bias)[j + e]) : static_cast<const float*>(bias)[j + e];
+  }
+  if (bf16) {
+    uint16_t* o = static_cast<uint16_t*>(out) + int64_t(i) * ldo + j;
+    if (vec && n == 4) {
+      if (accumulate) {
+        const uint2 u = *reinterpret_cast<const uint2*>(o);
+        v[0] += bf2f(u.x & 0xffff);
+        v[1] += bf2f(u.x >> 16);
+        v[2] += bf2f(u.y & 0xffff);
+        v[3] += bf2f(u.y >> 16);
+      }
+      *reinterpret_cast<uint2*>(o) = make_uint2(uint32_t(f2bf(v[0])) | (uint32_t(f2bf(v[1])) << 16),
+                                                uint32_t(f2bf(v[2])) | (uint32_t(f2bf(v[3])) << 16));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < n) o[e] = f2bf(v[e] + (accumulate ? bf2f(o[e]) : 0.f));
+    }
+  } else {
+    float* o = static_cast<float*>(out) + int64_t(i) * ldo + j;
+    if (vec && n == 4) {
+      if (accumulate) {
+        const float4 u = *reinterpret_cast<const float4*>(o);
+        v[0] += u.x;
+        v[1] += u.y;
+        v[2] += u.z;
+        v[3] += u.w;
+      }
+      *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < n) o[e] = v[e] + (accumulate ? o[e] : 0.f);
+    }
+  }
+}
+
+struct GemmArgs {
+  Operand I, J;
+  const int* ni_dev;     // rows in use (<= I.n), or null: all
+  const int* nk_dev;     // reduction length in use (<= nk), or null: all
+  int nk;
+  Order o;
+  // o.splits > 1 or slab given: fp32 partial results [split][I.n][lds] (``add``: onto what is there)
+  float* slab;
+  int64_t lds;
+  int add;
+  float* bslab;          // [split][I.n] partial sums of I over k (col I), or null
+  void* bout;            // their result when there is no slab, in out's type
+  Emit e;
+};
+
+// one split's reduction range: whole stages, as even as they go
+__device__ __forceinline__ void split_range(int nk, int splits, int s, int bk, int& k0, int& k1) {
+  const int steps = (nk + bk - 1) / bk, per = (steps + splits - 1) / splits;
+  k0 = min(nk, s * per * bk);
+  k1 = min(nk, k0 + per * bk);
+}
+
+__device__ __forceinline__ void emit_sum(const Emit& e, void* out, int i, float v) {
+  v = i < e.zero_from ? e.scaled(v, false) : 0.f;
+  if (e.bf16) {
+    uint16_t* o = static_cast<uint16_t*>(out) + i;
+    *o = f2bf(v + (e.accumulate ? bf2f(*o) : 0.f));
+  } else {
+    float* o = static_cast<float*>(out) + i;
+    *o = v + (e.accumulate ? *o : 0.f);
+  }
+}
+
+template <class T, bool SUM>
+__global__ __launch_bounds__(T::kThreads, 2) void gemm_kernel(GemmArgs p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[T::kLds];
+  int ti, tj, s;
+  p.o.at(blockIdx.x, gridDim.x, ti, tj, s);
+  const int i0 = ti * T::BI, j0 = tj * T::BJ;
+  Operand I = p.I;
+  if (p.ni_dev) I.n = min(I.n, *p.ni_dev);
+  if (i0 >= I.n) return;
+  const int nk = p.nk_dev ? min(p.nk, *p.nk_dev) : p.nk;
+  int k0, k1;
+  split_range(nk, p.o.splits, s, T::BK, k0, k1);
+  const typename T::Where w;
+  const bool want = SUM && (p.bslab || p.bout) && tj == 0 && w.wj == 0;
+  f32x16 acc[T::TJ][T::TI];
+  float isum[T::TI];
+  T::template run<SUM>(smem, I, p.J, i0, j0, k0, k1, acc, isum, want);
+#pragma unroll
+  for (int b = 0; b < T::TI; ++b) {
+    const int i = i0 + w.i(b);
+    if constexpr (SUM) {
+      if (want) {
+        const float tot = isum[b] + __shfl_xor(isum[b], 32, 64);
+        if (w.h == 0 && i < I.n) {
+          if (p.bslab) p.bslab[int64_t(s) * p.I.n + i] = tot;
+          else emit_sum(p.e, p.bout, i, tot);
+        }
+      }
+    }
+    if (i >= I.n) continue;
+#pragma unroll
+    for (int a = 0; a < T::TJ; ++a) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int j = j0 + w.j(a, g);
+        float v[4] = {acc[a][b][4 * g], acc[a][b][4 * g + 1], acc[a][b][4 * g + 2], acc[a][b][4 * g + 3]};
+        if (p.slab) {
+          if (j < p.lds) {
+            float4* o = reinterpret_cast<float4*>(p.slab + (int64_t(s) * p.I.n + i) * p.lds + j);
+            if (p.add) {
+              const float4 u = *o;
+              v[0] += u.x;
+              v[1] += u.y;
+              v[2] += u.z;
+              v[3] += u.w;
+            }
+            *o = make_float4(v[0], v[1], v[2], v[3]);
+          }
+        } else {
+          p.e.quad(i, j, v);
+        }
+      }
+    }
+  }
+}
+
+// Sums the splits of a slab and stores the result; ``inv`` (or null) maps an output row to its row of
+// the slab, -1 where the row is zero.  One thread a quad of columns, then one a partial sum.
+struct FinishArgs {
+  const float* slab;
+  int64_t lds;
+  int splits, slab_rows, rows;
+  const int* inv;
+  const float* bslab;
+  void* bout;
+  Emit e;
+};
+
+static __global__ __launch_bounds__(256) void finish_kernel(FinishArgs p) {
+  const int quads = (p.e.nj + 3) >> 2;
+  const int64_t n = int64_t(p.rows) * quads;
+  const int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (t < n) {
+    const int i = int(t / quads), j = 4 * int(t - int64_t(i) * quads);
+    const int src = p.inv ? p.inv[i] : i;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (src >= 0) {
+      const float* a = p.slab + int64_t(src) * p.lds + j;
+      for (int s = 0; s < p.splits; ++s) {
+        const float4 u = *reinterpret_cast<const float4*>(a + int64_t(s) * p.slab_rows * p.lds);
+        v[0] += u.x;
+        v[1] += u.y;
+        v[2] += u.z;
+        v[3] += u.w;
+      }
+    }
+    p.e.quad(i, j, v, src >= 0);
+  } else if (p.bslab && t - n < p.rows) {
+    const int i = int(t - n);
+    float v = 0.f;
+    for (int s = 0; s < p.splits; ++s) v += p.bslab[int64_t(s) * p.slab_rows + i];
+    emit_sum(p.e, p.bout, i, v);
+  }
+}
+
+inline void finish(const FinishArgs& p, hipStream_t st) {
+  const int64_t n = int64_t(p.rows) * ((p.e.nj + 3) / 4) + (p.bslab ? p.rows : 0);
+  hipLaunchKernelGGL(finish_kernel, dim3(unsigned((n + 255) / 256)), dim3(256), 0, st, p);
+  check_launch();
+}
+
+template <class T, bool SUM>
+inline void gemm(GemmArgs p, hipStream_t st) {
+  p.o.ti = (p.I.n + T::BI - 1) / T::BI;
+  p.o.tj = (p.e.nj + T::BJ - 1) / T::BJ;
+  hipLaunchKernelGGL((gemm_kernel<T, SUM>), dim3(unsigned(int64_t(p.o.ti) * p.o.tj * p.o.splits)), dim3(T::kThreads), 0,
+                     st, p);
+  check_launch();
+}
+
+// ---- fp32 -> planes ----------------------------------------------------------------------------
+
+constexpr int kAmaxBlocks = 256;  // partial maxima a tensor
+
+// the largest of a tensor's partial maxima, by every thread of a block of 256
+__device__ __forceinline__ float amax_of(const float* part, float* lds4) {
+  float m = wave_max(part[threadIdx.x]);
+  __syncthreads();  // lds4 may still be read from an earlier call
+  if ((threadIdx.x & 63) == 0) lds4[threadIdx.x >> 6] = m;
+  __syncthreads();
+  return fmaxf(fmaxf(lds4[0], lds4[1]), fmaxf(lds4[2], lds4[3]));
+}
+
+// an infinite or NaN element: hi carries it, lo is zero
+__device__ __forceinline__ void split_safe(float x, float scale, uint16_t& hi, uint16_t& lo) {
+  split2(x * scale, hi, lo);
+  if (!(fabsf(x) <= 3.4028235e38f)) lo = 0;
+}
+
+struct Rows {
+  const float* p;
+  int64_t ld;
+  int n, width;
+};
+
+// Partial maxima [2][kAmaxBlocks] of the finite |elements| of a and b (grid: 2 kAmaxBlocks, or half of
+// it for a alone).  With ``labels``, of the rows of a whose label is in [0, classes) and not ``ignore``.
+static __global__ __launch_bounds__(256) void amax_kernel(Rows a, Rows b, const int64_t* __restrict__ labels, int64_t ignore,
+                                                   int classes, float* __restrict__ part) {
+  const bool second = blockIdx.x >= kAmaxBlocks;
+  const Rows x = second ? b : a;
+  const int blk = second ? blockIdx.x - kAmaxBlocks : blockIdx.x;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  auto of = [](float v) { return fabsf(v) <= 3.4028235e38f ? fabsf(v) : 0.f; };
+  const bool vec = (x.ld & 3) == 0 && (x.width & 3) == 0 && (reinterpret_cast<uintptr_t>(x.p) & 15) == 0;
+  float m = 0.f;
+  for (int r = blk * 4 + wave; r < x.n; r += kAmaxBlocks * 4) {
+    if (!second && labels) {
+      const int64_t y = labels[r];
+      if (y == ignore || y < 0 || y >= classes) continue;
+    }
+    const float* row = x.p + int64_t(r) * x.ld;
+    if (vec) {
+      for (int c = 4 * lane; c < x.width; c += 256) {
+        const float4 u = *reinterpret_cast<const float4*>(row + c);
+        m = fmaxf(m, fmaxf(fmaxf(of(u.x), of(u.y)), fmaxf(of(u.z), of(u.w))));
+      }
+    } else {
+      for (int c = lane; c < x.width; c += 64) m = fmaxf(m, of(row[c]));
+    }
+  }
+  __shared__ float lds[4];
+  m = wave_max(m);
+  if (lane == 0) lds[wave] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
+}
+
+inline void amax(const Rows& a, const Rows* b, const int64_t* labels, int64_t ignore, int classes, float* part,
+                 hipStream_t st) {
+  hipLaunchKernelGGL(amax_kernel, dim3(b ? 2 * kAmaxBlocks : kAmaxBlocks), dim3(256), 0, st, a, b ? *b : a, labels, ignore,
+                     classes, part);
+  check_launch();
+}
+
+__device__ __forceinline__ uint2 pack4(const uint16_t (&v)[4]) {
+  return make_uint2(v[0] | (uint32_t(v[1]) << 16), v[2] | (uint32_t(v[3]) << 16));
+}
+
+// x's rows as two fp16 planes [n][kp] (zeros from width to kp), and 2^-a to *inv; one quad a thread
+static __global__ __launch_bounds__(256) void split_kernel(Rows x, uint16_t* __restrict__ out, int kp, int64_t plane,
+                                                    const float* __restrict__ part, float* __restrict__ inv) {
+  __shared__ float lds[4];
+  const float s = split_scale(amax_of(part, lds));
+  if (blockIdx.x == 0 && threadIdx.x == 0) *inv = pow2_inverse(s);
+  const int quads = kp >> 2;
+  const bool vec = (x.ld & 3) == 0 && (x.width & 3) == 0 && (reinterpret_cast<uintptr_t>(x.p) & 15) == 0;
+  const int64_t n = int64_t(x.n) * quads;
+  for (int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x; t < n; t += int64_t(gridDim.x) * 256) {
+    const int64_t r = t / quads;
+    const int c = 4 * int(t - r * quads);
+    const float* row = x.p + r * x.ld + c;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (vec) {
+      if (c < x.width) {
+        const float4 u = *reinterpret_cast<const float4*>(row);
+        v[0] = u.x;
+        v[1] = u.y;
+        v[2] = u.z;
+        v[3] = u.w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < x.width) v[e] = row[e];
+    }
+    uint16_t hi[4], lo[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split_safe(v[e], s, hi[e], lo[e]);
+    *reinterpret_cast<uint2*>(out + 4 * t) = pack4(hi);
+    *reinterpret_cast<uint2*>(out + plane + 4 * t) = pack4(lo);
+  }
+}
+
+inline void split(const Rows& x, uint16_t* out, int kp, int64_t plane, const float* part, float* inv, hipStream_t st) {
+  hipLaunchKernelGGL(split_kernel, dim3(stream_grid(int64_t(x.n) * (kp >> 2), 256, 8192)), dim3(256), 0, st, x, out, kp,
+                     plane, part, inv);
+  check_launch();
+}
+
+// ---- choices shared by the operators -------------------------------------------------------------
+
+inline int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+// Tiles: kBig (256 columns x 128 rows) for full batches; kFew (128 x 32) for a handful of rows, whose
+// products only stream the weights.
+template <bool F16, int NP, bool IT, bool JT> using Big = Tile<F16, NP, IT, JT, 2, 2, 4, 2, 32, 3>;
+template <bool F16, int NP, bool IT, bool JT> using Mid = Tile<F16, NP, IT, JT, 2, 2, 2, 1, 64, 3>;
+template <bool F16, int NP, bool IT, bool JT> using Few = Tile<F16, NP, IT, JT, 4, 1, 1, 1, 64, 3>;
+
+enum { kBig = 0, kMid = 1, kFew = 2 };
+inline int tile_bj(int t) { return t == kBig ? 256 : 128; }
+inline int tile_bi(int t) { return t == kBig ? 128 : t == kMid ? 64 : 32; }
+
+inline int64_t tiles_of(int tile, int64_t ni, int64_t nj) {
+  return ((ni + tile_bi(tile) - 1) / tile_bi(tile)) * ((nj + tile_bj(tile) - 1) / tile_bj(tile));
+}
+
+// splits of a reduction of ``nk`` so that tiles x splits comes near two workgroups a CU, each split
+// at least ``least`` long
+inline int splits_for(int64_t tiles, int64_t nk, int64_t least) {
+  int64_t s = (512 + tiles - 1) / tiles;
+  s = s < nk / least ? s : nk / least;
+  return int(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+}  // namespace gt
+}  // namespace voda

@@ -1,0 +1,676 @@
+// Softmax cross-entropy of a vocabulary head without its logits (CDNA4, gfx950).
+//
+//   z[r][v]  = sum_k x[r][k] w[v][k] + b[v]           v < C (classes), r over the labelled rows
+//   loss     = 1/n sum_r (lse_r - z[r][y_r])          lse_r = log sum_v exp z[r][v]
+//   G[r][v]  = exp(z[r][v] - lse_r) - [v == y_r]
+//   dx = g/n G w     dw = g/n G^T x     db = g/n sum_r G     (g: the loss's own gradient)
+//
+// The logits of a tile live in the accumulators only.  Forward: one product x w^T whose epilogue
+// leaves a (max, sum exp) pair a row for each 32 * TJ columns of the vocabulary, joined by
+// xent_join.  Backward: piece by piece of the vocabulary the product runs again and leaves G of the
+// piece in a workspace (16 bits; fp32 inputs: two fp16 planes), which the two gradient products read.
+// So 8 n C K operations instead of 6, and no memory that grows with n C.
+//
+// Rows whose label is ignored (or lies outside [0, C)) are left out at the start: xent_gather copies
+// the labelled rows together, all later kernels work on those n rows (n stays on the device, the
+// launches are sized for all rows and the workgroups behind n end at once).  An ignored row costs
+// nothing, its dx is exactly zero and nothing that it holds, NaN included, reaches any output.
+//
+// bf16 inputs: G is rounded once to bf16 (2^-9 of each element, random in sign, against the same
+// rounding of the sums to bf16 at the end); the one-hot part is subtracted before that rounding and
+// g/n multiplied after the sums.  fp32 inputs: two fp16 planes an operand (gemm_tile.h); G 2^15.
+// Sums over rows and splits have a fixed order: the same call gives the same bits.
+#include "gemm_tile.h"
+#include "ops.h"
+
+#include <algorithm>
+
+namespace voda {
+
+namespace {
+
+using namespace gt;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kGatherRows = 32;   // rows a gather workgroup
+constexpr float kGScale = 32768.f;  // G's planes hold G 2^15: |G| <= 1
+
+// device scalars of one call
+struct XentDev {
+  int n;           // labelled rows
+  int done;        // workgroups of xent_join that are through
+  float inv_x;     // 2^-a of x's planes (fp32 inputs)
+  float inv_w;     // 2^-a of w's planes
+};
+
+__device__ __forceinline__ bool labelled(int64_t y, int64_t ignore, int classes) {
+  return y != ignore && y >= 0 && y < classes;
+}
+
+struct GatherArgs {
+  const void* x;
+  int64_t ldx;
+  int rows, width, classes, vec;
+  const int64_t* labels;
+  int64_t ignore;
+  uint16_t* xc;      // [rows][kp] (fp32: two planes)
+  int kp;
+  int64_t plane;
+  int* inv;          // [rows]: place among the labelled rows, or -1
+  int* lab;          // [rows]: labels of the labelled rows
+  XentDev* dev;
+  int64_t* n_out;
+  const void* bias;  // [classes] or null
+  int bias_bf16;
+  float* bias32;     // [bias_n]: bias, 0 where there is none, -inf from classes on
+  int bias_n;
+  const float* amax; // fp32: partial maxima of x
+  int gather_blocks;
+};
+
+// Labelled rows of x together, and what goes with them; then the bias in fp32.
+template <bool F32>
+__global__ __launch_bounds__(256) void xent_gather_kernel(GatherArgs p) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  if (int(blockIdx.x) >= p.gather_blocks) {
+    const int v = (blockIdx.x - p.gather_blocks) * 256 + t;
+    if (v < p.bias_n)
+      p.bias32[v] = v >= p.classes ? -INFINITY
+                    : !p.bias      ? 0.f
+                    : p.bias_bf16  ? bf2f(static_cast<const uint16_t*>(p.bias)[v])
+                                   : static_cast<const float*>(p.bias)[v];
+    return;
+  }
+  __shared__ float lds[4];
+  __shared__ int cnt[4];
+  __shared__ int place[kGatherRows];
+  float scale = 1.f;
+  if constexpr (F32) {
+    scale = split_scale(amax_of(p.amax, lds));
+    if (blockIdx.x == 0 && t == 0) p.dev->inv_x = pow2_inverse(scale);
+  }
+  // labelled rows in front of this workgroup's: every workgroup counts them itself (8 bytes a row
+  // out of the L2), which is cheaper than a second launch
+  const int r0 = blockIdx.x * kGatherRows;
+  int c = 0;
+  for (int r = t; r < r0; r += 256) c += labelled(p.labels[r], p.ignore, p.classes);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
+  if (lane == 0) cnt[wave] = c;
+  __syncthreads();
+  if (wave == 0) {
+    const int base = cnt[0] + cnt[1] + cnt[2] + cnt[3];
+    const int r = r0 + lane;
+    const bool mine = lane < kGatherRows && r < p.rows;
+    const int64_t y = mine ? p.labels[r] : -1;
+    const bool ok = mine && labelled(y, p.ignore, p.classes);
+    const uint64_t all = __ballot(ok);
+    const int at = base + __popcll(all & ((uint64_t(1) << lane) - 1));
+    if (mine) {
+      p.inv[r] = ok ? at : -1;
+      place[lane] = ok ? at : -1;
+      if (ok) p.lab[at] = int(y);
+    }
+    if (lane == 0 && r0 + kGatherRows >= p.rows) {
+      p.dev->n = base + __popcll(all);
+      p.dev->done = 0;
+      *p.n_out = base + __popcll(all);
+    }
+  }
+  __syncthreads();
+  for (int u = wave; u < kGatherRows && r0 + u < p.rows; u += 4) {
+    const int at = place[u];
+    if (at < 0) continue;
+    uint16_t* o = p.xc + int64_t(at) * p.kp;
+    if constexpr (F32) {
+      const float* row = static_cast<const float*>(p.x) + int64_t(r0 + u) * p.ldx;
+      if (p.vec) {
+        for (int k = 4 * lane; k < p.kp; k += 256) {
+          uint16_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+          if (k < p.width) {
+            const float4 f = *reinterpret_cast<const float4*>(row + k);
+            const float v[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split_safe(v[e], scale, hi[e], lo[e]);
+          }
+          *reinterpret_cast<uint2*>(o + k) = make_uint2(hi[0] | (uint32_t(hi[1]) << 16), hi[2] | (uint32_t(hi[3]) << 16));
+          *reinterpret_cast<uint2*>(o + p.plane + k) =
+              make_uint2(lo[0] | (uint32_t(lo[1]) << 16), lo[2] | (uint32_t(lo[3]) << 16));
+        }
+      } else {
+        for (int k = lane; k < p.kp; k += 64) {
+          uint16_t hi = 0, lo = 0;
+          if (k < p.width) split_safe(row[k], scale, hi, lo);
+          o[k] = hi;
+          o[p.plane + k] = lo;
+        }
+      }
+    } else {
+      const uint16_t* row = static_cast<const uint16_t*>(p.x) + int64_t(r0 + u) * p.ldx;
+      if (p.vec) {
+        for (int k = 8 * lane; k < p.kp; k += 512)
+          *reinterpret_cast<uint4*>(o + k) = *reinterpret_cast<const uint4*>(row + k);
+      } else {
+        for (int k = lane; k < p.kp; k += 64) o[k] = k < p.width ? row[k] : uint16_t(0);
+      }
+    }
+  }
+}
+
+struct LogitArgs {
+  Operand X, W;
+  int width, classes;
+  Order o;
+  int v0, v1;           // vocabulary columns of this launch
+  const float* bias32;
+  const XentDev* dev;
+  const int* lab;
+  // forward: partial (max, sum exp) [slot][rows], a slot 32 TJ columns; the label's logit and whether
+  // an earlier column of its slot equals it
+  float2* part;
+  float* zlab;
+  int* tie;
+  // backward: (max, 1 / sum exp) of each row, G [rows][ldg] (fp32 inputs: two planes)
+  const float2* stat;
+  uint16_t* G;
+  int64_t ldg, gplane;
+};
+
+// Rows are the tile's i, vocabulary columns its j.  The epilogue is vector work that the matrix cores
+// wait for unless another workgroup of the CU is in its main loop: two workgroups a CU (72 KB of LDS each).
+template <class T, bool F16, bool BWD>
+__global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[T::kLds];
+  int ti, tj, s;
+  p.o.at(blockIdx.x, gridDim.x, ti, tj, s);
+  const int i0 = ti * T::BI, j0 = p.v0 + tj * T::BJ;
+  Operand X = p.X;
+  X.n = min(X.n, p.dev->n);
+  if (i0 >= X.n) return;
+  f32x16 acc[T::TJ][T::TI];
+  float unused[T::TI];
+  T::template run<false>(smem, X, p.W, i0, j0, 0, p.width, acc, unused);
+  const typename T::Where w;
+  float sx = 1.f, sw = 1.f;
+  if constexpr (F16) {
+    sx = p.dev->inv_x;
+    sw = p.dev->inv_w;
+  }
+  // z = products + bias; columns past the classes get the bias's -inf
+#pragma unroll
+  for (int a = 0; a < T::TJ; ++a) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 b4 = *reinterpret_cast<const float4*>(p.bias32 + j0 + w.j(a, g));
+      const float b[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int c = 0; c < T::TI; ++c) {
+          float v = acc[a][c][4 * g + e];
+          if constexpr (F16) v = v * sx * sw;
+          acc[a][c][4 * g + e] = v + b[e];
+        }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < T::TI; ++c) {
+    const int i = i0 + w.i(c);
+    const bool live = i < X.n;
+    const int y = live ? p.lab[i] : -1;
+    if constexpr (!BWD) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int a = 0; a < T::TJ; ++a)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[a][c][r]);
+      m = fmaxf(m, __shfl_xor(m, 32, 64));
+      const float ms = m == -INFINITY ? 0.f : m;  // all -inf: a sum of zeros
+      float sum = 0.f;
+#pragma unroll
+      for (int a = 0; a < T::TJ; ++a)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f((acc[a][c][r] - ms) * kLog2e);
+      sum += __shfl_xor(sum, 32, 64);
+      const int slot = tj * T::WJ + w.wj;
+      if (live && w.h == 0) p.part[int64_t(slot) * p.X.n + i] = make_float2(m, sum);
+      // the label's logit, from the one wave whose columns hold it
+      const int jw = j0 + w.wj * T::TJ * 32;
+      const bool here = y >= jw && y < jw + T::TJ * 32;
+      if (__ballot(here)) {
+        float z = -INFINITY;
+        bool has = false;
+#pragma unroll
+        for (int a = 0; a < T::TJ; ++a)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (j0 + w.j(a, r >> 2) + (r & 3) == y) {
+              z = acc[a][c][r];
+              has = true;
+            }
+        const float z2 = __shfl_xor(z, 32, 64);
+        if (!has) z = z2;
+        int t = 0;
+#pragma unroll
+        for (int a = 0; a < T::TJ; ++a)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) t |= int(j0 + w.j(a, r >> 2) + (r & 3) < y && acc[a][c][r] == z);
+        t |= __shfl_xor(t, 32, 64);
+        if (here && w.h == 0) {
+          p.zlab[i] = z;
+          p.tie[i] = t;
+        }
+      }
+    } else {
+      const float2 st = live ? p.stat[i] : make_float2(0.f, 0.f);
+      uint16_t* g0 = p.G + int64_t(i) * p.ldg + (j0 - p.v0);
+      if (!live) continue;
+#pragma unroll
+      for (int a = 0; a < T::TJ; ++a) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int j = w.j(a, g);
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] = __builtin_amdgcn_exp2f((acc[a][c][4 * g + e] - st.x) * kLog2e) * st.y;
+            if (j0 + j + e == y) v[e] -= 1.f;
+          }
+          if constexpr (F16) {
+            uint16_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split2(v[e] * kGScale, hi[e], lo[e]);
+            *reinterpret_cast<uint2*>(g0 + j) = make_uint2(hi[0] | (uint32_t(hi[1]) << 16), hi[2] | (uint32_t(hi[3]) << 16));
+            *reinterpret_cast<uint2*>(g0 + p.gplane + j) =
+                make_uint2(lo[0] | (uint32_t(lo[1]) << 16), lo[2] | (uint32_t(lo[3]) << 16));
+          } else {
+            *reinterpret_cast<uint2*>(g0 + j) = make_uint2(uint32_t(f2bf(v[0])) | (uint32_t(f2bf(v[1])) << 16),
+                                                           uint32_t(f2bf(v[2])) | (uint32_t(f2bf(v[3])) << 16));
+          }
+        }
+      }
+    }
+  }
+}
+
+// Joins the slots of 64 rows a workgroup: 16 waves each take every 16th slot.  The last workgroup to
+// finish adds the workgroups' sums up, in their order.
+constexpr int kJoinWaves = 16;
+__global__ __launch_bounds__(64 * kJoinWaves) void xent_join_kernel(const float2* __restrict__ part, int slots, int cap,
+                                                                    int slot_cols, const float* __restrict__ zlab,
+                                                                    const int* __restrict__ tie,
+                                                                    const int* __restrict__ lab, XentDev* dev,
+                                                                    float2* __restrict__ stat, double* __restrict__ lsum,
+                                                                    int* __restrict__ csum, float* __restrict__ loss,
+                                                                    int64_t* __restrict__ correct) {
+  __shared__ float sm[kJoinWaves][64], ss[kJoinWaves][64], sl[kJoinWaves][64];
+  __shared__ int last;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = dev->n;
+  const int i = blockIdx.x * 64 + lane;
+  const bool live = i < n;
+  const int yslot = live ? lab[i] / slot_cols : 0;
+  const float z = live ? zlab[i] : 0.f;
+  float m = -INFINITY, s = 0.f, before = -INFINITY;  // before: largest of the slots in front of the label's
+  if (live) {
+    for (int k = wave; k < slots; k += kJoinWaves) {
+      const float2 v = part[int64_t(k) * cap + i];
+      const float nm = fmaxf(m, v.x);
+      const float at = nm == -INFINITY ? 0.f : nm;
+      s = s * __builtin_amdgcn_exp2f((m - at) * kLog2e) + v.y * __builtin_amdgcn_exp2f((v.x - at) * kLog2e);
+      m = nm;
+      if (k < yslot) before = fmaxf(before, v.x);
+    }
+  }
+  sm[wave][lane] = m;
+  ss[wave][lane] = s;
+  sl[wave][lane] = before;
+  __syncthreads();
+  if (wave == 0) {
+    double l = 0.0;
+    int ok = 0;
+    if (live) {
+      for (int k = 0; k < kJoinWaves; ++k) {
+        m = fmaxf(m, sm[k][lane]);
+        before = fmaxf(before, sl[k][lane]);
+      }
+      const float at = m == -INFINITY ? 0.f : m;
+      s = 0.f;
+      for (int k = 0; k < kJoinWaves; ++k) s += ss[k][lane] * __builtin_amdgcn_exp2f((sm[k][lane] - at) * kLog2e);
+      stat[i] = make_float2(m, 1.f / s);
+      // (max - z) first: exact where the label's logit is the largest or near it
+      l = double(m - z) + double(logf(s));
+      ok = z == m && before < z && !tie[i] && s == s;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      l += __shfl_xor(l, o, 64);
+      ok += __shfl_xor(ok, o, 64);
+    }
+    if (lane == 0) {
+      __hip_atomic_store(lsum + blockIdx.x, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(csum + blockIdx.x, ok, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      last = __hip_atomic_fetch_add(&dev->done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == int(gridDim.x) - 1;
+    }
+  }
+  __syncthreads();
+  if (!last || wave != 0) return;
+  double l = 0.0;
+  int64_t ok = 0;
+  for (unsigned b = lane; b < gridDim.x; b += 64) {
+    l += __hip_atomic_load(lsum + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    ok += __hip_atomic_load(csum + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    l += __shfl_xor(l, o, 64);
+    ok += __shfl_xor(ok, o, 64);
+  }
+  if (lane == 0) {
+    *loss = n > 0 ? float(l / n) : 0.f;
+    *correct = ok;
+  }
+}
+
+// The product's tile: kBig where it gives every CU one, kMid below, kFew for a handful of rows.
+int logits_tile(int rows, int cols) {
+  if (rows <= 32) return kFew;
+  return tiles_of(kBig, rows, cols) >= 256 ? kBig : kMid;
+}
+int tile_slot(int t) { return t == kBig ? 128 : t == kMid ? 64 : 32; }
+
+template <bool F16, bool BWD>
+void launch_logits(LogitArgs& p, int tile, hipStream_t st) {
+  p.o.gi = 8;
+  p.o.splits = 1;
+  p.o.ti = (p.X.n + tile_bi(tile) - 1) / tile_bi(tile);
+  p.o.tj = (p.v1 - p.v0 + tile_bj(tile) - 1) / tile_bj(tile);
+  const dim3 grid(unsigned(int64_t(p.o.ti) * p.o.tj)), block(256);
+  constexpr int NP = F16 ? 3 : 1;
+  if (tile == kBig)
+    hipLaunchKernelGGL((xent_logits_kernel<Big<F16, NP, false, false>, F16, BWD>), grid, block, 0, st, p);
+  else if (tile == kMid)
+    hipLaunchKernelGGL((xent_logits_kernel<Mid<F16, NP, false, false>, F16, BWD>), grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL((xent_logits_kernel<Few<F16, NP, false, false>, F16, BWD>), grid, block, 0, st, p);
+  check_launch();
+}
+
+}  // namespace
+
+// ---- host --------------------------------------------------------------------------------------
+
+namespace {
+
+struct XentPlan {
+  int kp, vpad, piece, tile, slots, gtile, dx_tile, dx_splits, dw_splits, planes;
+  int64_t fwd_bytes, bwd_bytes;
+  // offsets into the forward's workspace
+  int64_t o_amax, o_wp, o_part, o_zlab, o_tie, o_lsum, o_csum;
+  // offsets into the backward's
+  int64_t b_amax, b_wp, b_g, b_dx, b_dw, b_db;
+};
+
+constexpr int64_t kGBytes = int64_t(256) << 20;  // G of one piece of the vocabulary
+
+XentPlan xent_plan(int rows, int width, int classes, bool f32) {
+  XentPlan q{};
+  q.planes = f32 ? 2 : 1;
+  q.kp = int(up(width, 8));
+  q.vpad = int(up(classes, 256));
+  q.tile = logits_tile(rows, classes);
+  q.slots = int(up(classes, tile_bj(q.tile)) / tile_slot(q.tile));
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at = up(at + bytes, 256);
+    return o;
+  };
+  q.o_amax = take(f32 ? 2 * kAmaxBlocks * 4 : 0);
+  q.o_wp = take(f32 ? int64_t(classes) * q.kp * 4 : 0);
+  q.o_part = take(int64_t(q.slots) * rows * 8);
+  q.o_zlab = take(int64_t(rows) * 4);
+  q.o_tie = take(int64_t(rows) * 4);
+  const int64_t jb = (rows + 63) / 64;
+  q.o_lsum = take(jb * 8);
+  q.o_csum = take(jb * 4);
+  q.fwd_bytes = at;
+  at = 0;
+  q.b_wp = take(f32 ? int64_t(classes) * q.kp * 4 : 0);
+  const int64_t row_bytes = int64_t(rows) * q.planes * 2;
+  q.piece = int(std::max<int64_t>(256, std::min<int64_t>(q.vpad, kGBytes / row_bytes / 256 * 256)));
+  q.gtile = logits_tile(rows, q.piece);
+  q.b_g = take(row_bytes * q.piece);
+  q.dx_tile = rows <= 32 ? kFew : kBig;
+  q.dx_splits = splits_for(tiles_of(q.dx_tile, rows, width), q.piece, 256);
+  q.b_dx = take(int64_t(q.dx_splits) * rows * q.kp * 4);
+  const int64_t wt = tiles_of(kBig, std::min(q.piece, classes), width);
+  q.dw_splits = wt >= 256 ? 1 : splits_for(wt, rows, 512);
+  q.b_dw = take(q.dw_splits > 1 ? int64_t(q.dw_splits) * q.piece * q.kp * 4 : 0);
+  q.b_db = take(q.dw_splits > 1 ? int64_t(q.dw_splits) * q.piece * 4 : 0);
+  q.bwd_bytes = at;
+  return q;
+}
+
+void check_xent(int64_t rows, int64_t width, int64_t classes, int64_t vocab) {
+  VODA_CHECK(rows > 0 && rows <= (1 << 24), "linear_xent: 1 to 2^24 rows");
+  VODA_CHECK(width > 0 && width <= (1 << 20), "linear_xent: width 1 to 2^20");
+  VODA_CHECK(classes > 0 && classes <= vocab && vocab <= (1 << 24), "linear_xent: 1 <= classes <= vocabulary <= 2^24");
+  VODA_CHECK(up(rows, 32) / 32 * (up(classes, 128) / 128) < (int64_t(1) << 31), "linear_xent: rows x vocabulary too large");
+}
+
+}  // namespace
+
+// bytes of (forward workspace, backward workspace), and the widths of x's compact rows and of the
+// padded fp32 bias
+std::vector<int64_t> linear_xent_sizes(int64_t rows, int64_t width, int64_t classes, int64_t vocab, bool f32) {
+  check_xent(rows, width, classes, vocab);
+  const XentPlan q = xent_plan(int(rows), int(width), int(classes), f32);
+  return {q.fwd_bytes, q.bwd_bytes, q.kp, q.vpad, int64_t(sizeof(XentDev))};
+}
+
+// ``keep``: what the backward needs (x's compact rows, bias32, inv, lab, stat, dev and, for fp32, w's
+// partial maxima), each its own allocation of the caller.
+void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr_t bias, int bias_dt, uintptr_t labels,
+                     int64_t ignore, int64_t rows, int64_t width, int64_t classes, int64_t vocab, int dt, uintptr_t ws,
+                     uintptr_t xc, uintptr_t bias32, uintptr_t inv, uintptr_t lab, uintptr_t stat, uintptr_t dev,
+                     uintptr_t amax, uintptr_t loss, uintptr_t correct, uintptr_t n_out, uintptr_t stream) {
+  check_xent(rows, width, classes, vocab);
+  VODA_CHECK(dt == kF32 || dt == kBF16, "linear_xent: x must be fp32 or bf16");
+  const bool f32 = dt == kF32;
+  VODA_CHECK(f32 || (w % 16 == 0 && ldw % 8 == 0 && ldw >= up(width, 8)),
+             "linear_xent: bf16 weight rows must be 16-byte aligned and whole 16-byte vectors");
+  VODA_CHECK(xc % 16 == 0 && ws % 256 == 0, "linear_xent: workspaces must be aligned");
+  const XentPlan q = xent_plan(int(rows), int(width), int(classes), f32);
+  hipStream_t st = as_stream(stream);
+  uint8_t* base = reinterpret_cast<uint8_t*>(ws);
+  XentDev* d = reinterpret_cast<XentDev*>(dev);
+  float* am = reinterpret_cast<float*>(amax);
+  if (f32) {
+    const Rows rw = {reinterpret_cast<const float*>(w), ldw, int(classes), int(width)};
+    gt::amax({reinterpret_cast<const float*>(x), ldx, int(rows), int(width)}, &rw, reinterpret_cast<const int64_t*>(labels),
+             ignore, int(classes), am, st);
+  }
+  GatherArgs g{};
+  g.x = reinterpret_cast<const void*>(x);
+  g.ldx = ldx;
+  g.rows = int(rows);
+  g.width = int(width);
+  g.classes = int(classes);
+  g.vec = f32 ? x % 16 == 0 && ldx % 4 == 0 && width % 4 == 0 : x % 16 == 0 && ldx % 8 == 0 && width % 8 == 0;
+  g.labels = reinterpret_cast<const int64_t*>(labels);
+  g.ignore = ignore;
+  g.xc = reinterpret_cast<uint16_t*>(xc);
+  g.kp = q.kp;
+  g.plane = rows * q.kp;
+  g.inv = reinterpret_cast<int*>(inv);
+  g.lab = reinterpret_cast<int*>(lab);
+  g.dev = d;
+  g.n_out = reinterpret_cast<int64_t*>(n_out);
+  g.bias = reinterpret_cast<const void*>(bias);
+  g.bias_bf16 = bias_dt == kBF16;
+  g.bias32 = reinterpret_cast<float*>(bias32);
+  g.bias_n = q.vpad;
+  g.amax = am;
+  g.gather_blocks = int((rows + kGatherRows - 1) / kGatherRows);
+  const dim3 gg(unsigned(g.gather_blocks + (q.vpad + 255) / 256));
+  if (f32) hipLaunchKernelGGL((xent_gather_kernel<true>), gg, dim3(256), 0, st, g);
+  else hipLaunchKernelGGL((xent_gather_kernel<false>), gg, dim3(256), 0, st, g);
+  check_launch();
+  LogitArgs p{};
+  p.X = {g.xc, q.kp, g.plane, int(rows)};
+  p.W = {reinterpret_cast<const uint16_t*>(w), ldw, 0, int(classes)};
+  if (f32) {
+    uint16_t* wp = reinterpret_cast<uint16_t*>(base + q.o_wp);
+    split({reinterpret_cast<const float*>(w), ldw, int(classes), int(width)}, wp, q.kp, classes * q.kp, am + kAmaxBlocks,
+          &d->inv_w, st);
+    p.W = {wp, q.kp, classes * q.kp, int(classes)};
+  }
+  p.width = q.kp;
+  p.classes = int(classes);
+  p.v0 = 0;
+  p.v1 = int(classes);
+  p.bias32 = g.bias32;
+  p.dev = d;
+  p.lab = g.lab;
+  p.part = reinterpret_cast<float2*>(base + q.o_part);
+  p.zlab = reinterpret_cast<float*>(base + q.o_zlab);
+  p.tie = reinterpret_cast<int*>(base + q.o_tie);
+  if (f32) launch_logits<true, false>(p, q.tile, st);
+  else launch_logits<false, false>(p, q.tile, st);
+  hipLaunchKernelGGL(xent_join_kernel, dim3(unsigned((rows + 63) / 64)), dim3(64 * kJoinWaves), 0, st, p.part, q.slots,
+                     int(rows), tile_slot(q.tile), p.zlab, p.tie, g.lab, d, reinterpret_cast<float2*>(stat),
+                     reinterpret_cast<double*>(base + q.o_lsum), reinterpret_cast<int*>(base + q.o_csum),
+                     reinterpret_cast<float*>(loss), reinterpret_cast<int64_t*>(correct));
+  check_launch();
+}
+
+// dx [rows][width] contiguous in x's type; rows [0, classes) of dw [..][ldd] and of db in ``grad_dt``
+// (added to when ``accumulate``); dx, db, or dw and db may be null.
+void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int64_t classes, int64_t vocab, int dt,
+                     uintptr_t ws, uintptr_t xc, uintptr_t bias32, uintptr_t inv, uintptr_t lab, uintptr_t stat,
+                     uintptr_t dev, uintptr_t amax, uintptr_t gloss, uintptr_t dx, uintptr_t dw, int64_t ldd,
+                     uintptr_t db, int grad_dt, bool accumulate, uintptr_t stream) {
+  check_xent(rows, width, classes, vocab);
+  VODA_CHECK(dt == kF32 || dt == kBF16, "linear_xent: x must be fp32 or bf16");
+  VODA_CHECK(grad_dt == kF32 || grad_dt == kBF16, "linear_xent: weight gradients must be fp32 or bf16");
+  const bool f32 = dt == kF32;
+  VODA_CHECK(f32 || (w % 16 == 0 && ldw % 8 == 0 && ldw >= up(width, 8)),
+             "linear_xent: bf16 weight rows must be 16-byte aligned and whole 16-byte vectors");
+  VODA_CHECK(xc % 16 == 0 && ws % 256 == 0, "linear_xent: workspaces must be aligned");
+  const XentPlan q = xent_plan(int(rows), int(width), int(classes), f32);
+  hipStream_t st = as_stream(stream);
+  uint8_t* base = reinterpret_cast<uint8_t*>(ws);
+  XentDev* d = reinterpret_cast<XentDev*>(dev);
+  LogitArgs p{};
+  p.X = {reinterpret_cast<const uint16_t*>(xc), q.kp, rows * q.kp, int(rows)};
+  p.W = {reinterpret_cast<const uint16_t*>(w), ldw, 0, int(classes)};
+  if (f32) {
+    uint16_t* wp = reinterpret_cast<uint16_t*>(base + q.b_wp);
+    split({reinterpret_cast<const float*>(w), ldw, int(classes), int(width)}, wp, q.kp, classes * q.kp,
+          reinterpret_cast<const float*>(amax) + kAmaxBlocks, &d->inv_w, st);
+    p.W = {wp, q.kp, classes * q.kp, int(classes)};
+  }
+  p.width = q.kp;
+  p.classes = int(classes);
+  p.bias32 = reinterpret_cast<const float*>(bias32);
+  p.dev = d;
+  p.lab = reinterpret_cast<const int*>(lab);
+  p.stat = reinterpret_cast<const float2*>(stat);
+  p.G = reinterpret_cast<uint16_t*>(base + q.b_g);
+  p.ldg = q.piece;
+  p.gplane = rows * q.piece;
+  const float* gl = reinterpret_cast<const float*>(gloss);
+  Emit e{};
+  e.f = f32 ? 1.f / kGScale : 1.f;
+  e.gl = gl;
+  e.gn = &d->n;
+  e.zero_from = 0x7fffffff;
+  const int gsz = grad_dt == kF32 ? 4 : 2;
+  for (int v0 = 0; v0 < q.vpad; v0 += q.piece) {
+    const int v1 = int(std::min<int64_t>(classes, v0 + q.piece));
+    if (v1 <= v0) break;
+    p.v0 = v0;
+    p.v1 = v1;
+    if (f32) launch_logits<true, true>(p, q.gtile, st);
+    else launch_logits<false, true>(p, q.gtile, st);
+    if (dx) {
+      GemmArgs a{};
+      a.I = {p.G, q.piece, p.gplane, int(rows)};
+      a.J = {p.W.p + int64_t(v0) * p.W.ld, p.W.ld, p.W.plane, int(up(width, 8))};
+      a.ni_dev = &d->n;
+      a.nk = v1 - v0;
+      a.o.gi = 8;
+      a.o.splits = q.dx_splits;
+      a.slab = reinterpret_cast<float*>(base + q.b_dx);
+      a.lds = q.kp;
+      a.add = v0 > 0;
+      a.e.nj = int(width);
+      if (q.dx_tile == kFew) {
+        if (f32) gemm<Few<true, 3, false, true>, false>(a, st);
+        else gemm<Few<false, 1, false, true>, false>(a, st);
+      } else {
+        if (f32) gemm<Big<true, 3, false, true>, false>(a, st);
+        else gemm<Big<false, 1, false, true>, false>(a, st);
+      }
+    }
+    if (dw) {
+      GemmArgs a{};
+      a.I = {p.G, q.piece, p.gplane, v1 - v0};
+      a.J = {p.X.p, p.X.ld, p.X.plane, int(up(width, 8))};
+      a.nk_dev = &d->n;
+      a.nk = int(rows);
+      a.o.gi = 8;
+      a.o.splits = q.dw_splits;
+      a.e = e;
+      a.e.fj = f32 ? &d->inv_x : nullptr;
+      a.e.out = reinterpret_cast<void*>(dw + uintptr_t(int64_t(v0) * ldd * gsz));
+      a.e.ldo = ldd;
+      a.e.bf16 = grad_dt == kBF16;
+      a.e.nj = int(width);
+      a.e.vec = ldd % 4 == 0 && dw % (4 * gsz) == 0;
+      a.e.accumulate = accumulate;
+      void* dbp = db ? reinterpret_cast<void*>(db + uintptr_t(v0) * gsz) : nullptr;
+      if (q.dw_splits > 1) {
+        a.slab = reinterpret_cast<float*>(base + q.b_dw);
+        a.lds = q.kp;
+        a.bslab = db ? reinterpret_cast<float*>(base + q.b_db) : nullptr;
+      } else {
+        a.bout = dbp;
+      }
+      if (f32) gemm<Big<true, 3, true, true>, true>(a, st);
+      else gemm<Big<false, 1, true, true>, true>(a, st);
+      if (q.dw_splits > 1) {
+        FinishArgs f{};
+        f.slab = a.slab;
+        f.lds = a.lds;
+        f.splits = q.dw_splits;
+        f.slab_rows = a.I.n;
+        f.rows = a.I.n;
+        f.bslab = a.bslab;
+        f.bout = dbp;
+        f.e = a.e;
+        finish(f, st);
+      }
+    }
+  }
+  if (dx) {
+    FinishArgs f{};
+    f.slab = reinterpret_cast<const float*>(base + q.b_dx);
+    f.lds = q.kp;
+    f.splits = q.dx_splits;
+    f.slab_rows = int(rows);
+    f.rows = int(rows);
+    f.inv = reinterpret_cast<const int*>(inv);
+    f.e = e;
+    f.e.fj = f32 ? &d->inv_w : nullptr;
+    f.e.out = reinterpret_cast<void*>(dx);
+    f.e.ldo = width;
+    f.e.bf16 = !f32;
+    f.e.nj = int(width);
+    f.e.vec = width % 4 == 0 && dx % 16 == 0;
+    finish(f, st);
+  }
+}
+
+}  // namespace voda
