@@ -204,7 +204,9 @@ unsigned blocks(int64_t threads) { return unsigned((threads + 255) / 256); }
 
 struct Act8Plan {
   int kq, np8, kp;               // features up to 32, outputs up to 8, features up to 8
-  int y_tile, dx_tile, y_s, dx_s, dw_s;
+  int y_tile, dx_tile, dw_tile;
+  Split y_split, dx_split, dw_split;
+  int y_s, dx_s, dw_s;
   bool copy;                     // the forward's product reads a copy that act8_pack writes
   // forward workspace: planes' inverse scales, x's operand, w's planes, slab
   int64_t f_inv, f_x, f_w, f_slab, fwd;
@@ -218,14 +220,16 @@ Act8Plan act8_plan(int64_t rows, int64_t width, int64_t out, bool f32, bool copy
   q.kp = int(up(width, 8));
   q.np8 = int(up(out, 8));
   q.copy = copy;
-  // a product's tile and the splits of its reduction: whole reductions where the tiles alone give
-  // every other CU one
-  auto tile = [&](int64_t ni) { return ni <= 32 ? kFew : kBig; };
-  auto splits = [&](int64_t tiles, int64_t nk, int64_t least) { return tiles >= 192 ? 1 : splits_for(tiles, nk, least); };
-  q.y_tile = q.dx_tile = tile(rows);
-  q.y_s = splits(tiles_of(q.y_tile, rows, out), width, 256);
-  q.dx_s = splits(tiles_of(q.dx_tile, rows, width), out, 256);
-  q.dw_s = splits(tiles_of(kBig, out, width), rows, 256);
+  const int np = f32 ? 3 : 1;
+  q.y_tile = choose_tile(rows, out, width * np, false);
+  q.dx_tile = choose_tile(rows, width, out * np, false);
+  q.dw_tile = choose_tile(out, width, rows * np, true);
+  q.y_split = {tile_slots(q.y_tile), 256};
+  q.dx_split = {tile_slots(q.dx_tile), 256};
+  q.dw_split = {tile_slots(q.dw_tile), 256};
+  q.y_s = q.y_split.of(tiles_of(q.y_tile, rows, out), q.kp);
+  q.dx_s = q.dx_split.of(tiles_of(q.dx_tile, rows, width), out);
+  q.dw_s = q.dw_split.of(tiles_of(q.dw_tile, out, width), rows);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
@@ -235,7 +239,7 @@ Act8Plan act8_plan(int64_t rows, int64_t width, int64_t out, bool f32, bool copy
   q.f_inv = take(f32 ? 16 : 0);
   q.f_x = take(copy ? rows * q.kq * (f32 ? 4 : 2) : 0);
   q.f_w = take(f32 ? out * q.kp * 4 : 0);
-  q.f_slab = take(q.y_s > 1 ? q.y_s * rows * up(out, 4) * 4 : 0);
+  q.f_slab = take(q.y_s > 1 ? q.y_s * rows * up(out, 8) * 4 : 0);
   q.fwd = at;
   at = 0;
   q.b_amax = take(f32 ? kAmaxBlocks * 4 : 0);
@@ -257,17 +261,6 @@ void check_act8(int64_t rows, int64_t width, int64_t out, int dt) {
                  up(rows * up(width, 32), 256) / 256 < (int64_t(1) << 31),
              "linear_act8: rows x features too large");
   VODA_CHECK(dt == kF32 || dt == kBF16, "linear_act8: fp32 or bf16");
-}
-
-FinishArgs finish_args(const GemmArgs& a, int splits) {
-  FinishArgs f{};
-  f.slab = a.slab;
-  f.lds = a.lds;
-  f.splits = splits;
-  f.slab_rows = f.rows = a.I.n;
-  f.bslab = a.bslab;
-  f.e = a.e;
-  return f;
 }
 
 }  // namespace
@@ -364,29 +357,24 @@ void linear_act8_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
     a.e.fj = inv + 1;
   }
   a.nk = q.kp;
-  a.o.gi = 8;
-  a.o.splits = q.y_s;
+  a.split = q.y_split;
+  a.nk_split = a.nk;
   a.e.f = 1.f;
   a.e.out = reinterpret_cast<void*>(y);
   a.e.ldo = out;
   a.e.bf16 = !f32;
   a.e.nj = int(out);
-  a.e.vec = out % 4 == 0 && y % 16 == 0;
-  a.e.zero_from = 0x7fffffff;
+  a.e.vec = whole_rows(y, out, !f32);
   a.e.bias = reinterpret_cast<const void*>(bias);
   a.e.bias_bf16 = bias_dt == kBF16;
   if (q.y_s > 1) {
     a.slab = reinterpret_cast<float*>(base + q.f_slab);
-    a.lds = up(out, 4);
+    a.lds = up(out, 8);
   }
-  if (q.y_tile == kFew) {
-    if (f32) gemm<Few<true, 3, false, false>, false>(a, st);
-    else gemm<Few<false, 1, false, false>, false>(a, st);
-  } else {
-    if (f32) gemm<Big<true, 3, false, false>, false>(a, st);
-    else gemm<Big<false, 1, false, false>, false>(a, st);
-  }
-  if (q.y_s > 1) finish(finish_args(a, q.y_s), st);
+  const int64_t grid_y = tiles_of(q.y_tile, rows, out) * q.y_s;
+  if (f32) gemm<true, 3, false, false, false>(q.y_tile, a, grid_y, st);
+  else gemm<false, 1, false, false, false>(q.y_tile, a, grid_y, st);
+  if (a.slab) finish(q.y_tile, a, int(rows), nullptr, st);
 }
 
 // dx [rows][ldo] in x's type (added to when ``dx_add``); dw [out][ldd] and db [out] in ``grad_dt``
@@ -431,8 +419,8 @@ void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintpt
     a.J = W;
     a.J.n = q.kp;  // columns: W is read down its rows
     a.nk = int(out);
-    a.o.gi = 8;
-    a.o.splits = q.dx_s;
+    a.split = q.dx_split;
+    a.nk_split = a.nk;
     a.e.f = 1.f;
     a.e.fi = f32 ? inv : nullptr;
     a.e.fj = f32 ? inv + 1 : nullptr;
@@ -440,10 +428,9 @@ void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintpt
     a.e.ldo = width;
     a.e.bf16 = !f32;
     a.e.nj = int(width);
-    a.e.vec = width % 4 == 0 && dx % 16 == 0;
+    a.e.vec = whole_rows(dx, width, !f32);
     a.e.accumulate = dx_add;
-    a.e.zero_from = 0x7fffffff;
-    if (gelu) {
+      if (gelu) {
       a.e.q = q8;
       a.e.qs = s8;
       a.e.ldq = q.kq;
@@ -452,14 +439,10 @@ void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintpt
       a.slab = reinterpret_cast<float*>(base + q.b_dx);
       a.lds = q.kp;
     }
-    if (q.dx_tile == kFew) {
-      if (f32) gemm<Few<true, 3, false, true>, false>(a, st);
-      else gemm<Few<false, 1, false, true>, false>(a, st);
-    } else {
-      if (f32) gemm<Big<true, 3, false, true>, false>(a, st);
-      else gemm<Big<false, 1, false, true>, false>(a, st);
-    }
-    if (q.dx_s > 1) finish(finish_args(a, q.dx_s), st);
+    const int64_t grid_x = tiles_of(q.dx_tile, rows, width) * q.dx_s;
+    if (f32) gemm<true, 3, false, true, false>(q.dx_tile, a, grid_x, st);
+    else gemm<false, 1, false, true, false>(q.dx_tile, a, grid_x, st);
+    if (a.slab) finish(q.dx_tile, a, int(rows), nullptr, st);
   }
   if (!dw) return;
   UnpackArgs u{};
@@ -480,8 +463,8 @@ void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintpt
   a.I.n = int(out);
   a.J = {u.o, q.kq, u.plane, q.kq};
   a.nk = int(rows);
-  a.o.gi = 8;
-  a.o.splits = q.dw_s;
+  a.split = q.dw_split;
+  a.nk_split = a.nk;
   a.e.f = 1.f;
   a.e.fi = f32 ? inv : nullptr;
   a.e.fj = f32 ? inv + 2 : nullptr;
@@ -489,25 +472,19 @@ void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintpt
   a.e.ldo = ldd;
   a.e.bf16 = grad_dt == kBF16;
   a.e.nj = int(width);
-  a.e.vec = ldd % 4 == 0 && dw % 16 == 0;
+  a.e.vec = whole_rows(dw, ldd, a.e.bf16);
   a.e.accumulate = accumulate;
-  a.e.zero_from = 0x7fffffff;
-  void* dbp = reinterpret_cast<void*>(db);
+  a.bout = reinterpret_cast<void*>(db);
   if (q.dw_s > 1) {
     a.slab = reinterpret_cast<float*>(base + q.b_dw);
     a.lds = q.kp;
     a.bslab = db ? reinterpret_cast<float*>(base + q.b_db) : nullptr;
-  } else {
-    a.bout = dbp;
   }
-  if (f32 && gelu) gemm<Big<true, 3, true, true>, true>(a, st);
-  else if (f32) gemm<Big<true, 2, true, true>, true>(a, st);
-  else gemm<Big<false, 1, true, true>, true>(a, st);
-  if (q.dw_s > 1) {
-    FinishArgs f = finish_args(a, q.dw_s);
-    f.bout = dbp;
-    finish(f, st);
-  }
+  const int64_t grid_w = tiles_of(q.dw_tile, out, width) * q.dw_s;
+  if (f32 && gelu) gemm<true, 3, true, true, true>(q.dw_tile, a, grid_w, st);
+  else if (f32) gemm<true, 2, true, true, true>(q.dw_tile, a, grid_w, st);
+  else gemm<false, 1, true, true, true>(q.dw_tile, a, grid_w, st);
+  if (a.slab) finish(q.dw_tile, a, int(out), nullptr, st);
 }
 
 }  // namespace voda

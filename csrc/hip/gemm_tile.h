@@ -13,8 +13,10 @@
 //    four consecutive columns j in each register quad, so a softmax over j is nearly all in-lane and
 //    a store moves 8 or 16 bytes.
 //  * Stages of BK reduction steps arrive in a ring of ST LDS buffers by 16-byte LDS-DMA (no staging
-//    registers); ST - 1 stages are in flight, one barrier a stage.  Chunks past the reduction's end
-//    read a zero buffer; rows past an operand's end read its last row (never stored).
+//    registers), one barrier a stage.  The barrier stands in front of a stage's last products: their
+//    fragments are in registers, so the buffer is refilled (one DMA instruction between two products)
+//    and the next stage's first fragments are read while they run.  Chunks past the reduction's end
+//    read a zero chunk; rows past an operand's end read its last row (never stored).
 //  * fp32 operands run as two fp16 planes, x 2^a = hi + 2^-11 lo: hi is x's first 11 bits, lo the
 //    next 11, so an element is held to 2^-24 of its size, or 2^-50 of the largest element where that
 //    is more (a: the power of two that brings the tensor's largest element to [2^14, 2^15)).
@@ -24,17 +26,21 @@
 
 #include "common.h"
 
+#include <algorithm>
+
 namespace voda {
 namespace gt {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x4_v __attribute__((__vector_size__(4 * sizeof(__bf16))));
 typedef __attribute__((address_space(3))) bf16x4_v lds_bf16x4;
 typedef __attribute__((address_space(3))) void lds_void;
 
-constexpr float kLoScale = 1.f / 2048.f;  // weight of a lo plane
+constexpr float kLoScale = 1.f / 2048.f;  // weight of an fp16 lo plane
 constexpr int kSplitExp = 15;             // hi planes: the largest element lies below 2^15
 
 // what chunks past a reduction's end read
@@ -72,6 +78,21 @@ __device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// sum of a fragment's eight elements, in fp32
+template <bool F16>
+__device__ __forceinline__ float sum8(uint4 f) {
+  const uint32_t u[4] = {f.x, f.y, f.z, f.w};
+  float s = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (F16)
+      s = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, u[e]), f16x2{1, 1}, s, false);
+    else
+      s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, u[e]), bf16x2{1, 1}, s, false);
+  }
+  return s;
 }
 
 // One operand's stage in LDS: EXT rows i x BK reduction steps, filled by NW waves, read by waves
@@ -132,16 +153,15 @@ struct Stage {
     }
   }
 
-  // fill: ``shift`` elements from the stage-0 addresses, ``left`` reduction steps remain
-  __device__ __forceinline__ void issue(uint8_t* lds, int64_t shift, int left, int wave, int lane) const {
-#pragma unroll
-    for (int u = 0; u < kPer; ++u) {
-      const int q = wave * kPer + u;
-      int r, k;
-      place(q, lane, r, k);
-      const bool ok = k < left && (!COL || src[u] != nullptr);
-      dma16(ok ? static_cast<const void*>(src[u] + shift) : zero_chunk, __builtin_amdgcn_readfirstlane(uint32_t(size_t((lds_void*)(lds + 1024 * q)))));
-    }
+  // this wave's instruction u: ``shift`` elements from the first stage's addresses, ``left`` reduction
+  // steps remain
+  __device__ __forceinline__ void issue(int u, uint8_t* lds, int64_t shift, int left, int wave, int lane) const {
+    const int q = wave * kPer + u;
+    int r, k;
+    place(q, lane, r, k);
+    const bool ok = k < left && (!COL || src[u] != nullptr);
+    dma16(ok ? static_cast<const void*>(src[u] + shift) : zero_chunk,
+          __builtin_amdgcn_readfirstlane(uint32_t(size_t((lds_void*)(lds + 1024 * q)))));
   }
 
   __device__ __forceinline__ uint4 frag(const uint8_t* lds, int t, int kk) const {
@@ -155,7 +175,8 @@ struct Stage {
 };
 
 // Tile of WJ x WI waves, each TJ x TI 32 x 32 blocks: BJ = 32 WJ TJ columns, BI = 32 WI TI rows.
-// NP products: 1 (plain 16-bit operands), 2 (I in two planes, J in one), 3 (both in two planes).
+// NP products: 1 (plain 16-bit operands), 2 (I in two planes, J in one), 3 (both in two planes).  A lo
+// plane weighs 2^-11 in fp16 and 1 in bf16, whose exponent needs no help.
 template <bool F16, int NP, bool IT, bool JT, int WJ_, int WI_, int TJ_, int TI_, int BK_, int ST_>
 struct Tile {
   static constexpr int WJ = WJ_, WI = WI_, TJ = TJ_, TI = TI_, BK = BK_, ST = ST_;
@@ -166,7 +187,8 @@ struct Tile {
   static constexpr int kStage = SI::kBytes + SJ::kBytes;
   static constexpr int kLds = ST * kStage;
   static constexpr int kPer = SI::kPer + SJ::kPer;
-  static_assert(ST >= 2 && (ST - 2) * kPer < 64, "ring depth");
+  static constexpr float kLo = F16 ? kLoScale : 1.f;  // weight of a lo plane
+  static_assert(ST >= 2 && (ST - 1) * kPer < 64 && BK % 32 == 0, "ring depth");
 
   struct Where {
     int lane, wave, h, il, wi, wj;
@@ -205,94 +227,115 @@ struct Tile {
     const int total = NP * steps;
     const int64_t stepi = IT ? BK * I.ld : BK, stepj = JT ? BK * J.ld : BK;
     int at = 0, prod = 0;  // next stage to issue: its step and product
-    auto issue = [&](int buf) {
-      // plane of each operand in product ``prod``; the last product is hi.hi
+    // instruction u of the next stage into ``lds``; stages past the last one read zeros
+    int64_t shi = 0, shj = 0;
+    int left = 0;
+    auto aim = [&] {
       const bool lo_i = NP == 3 ? prod == 1 : NP == 2 ? prod == 0 : false;
       const bool lo_j = NP == 3 && prod == 0;
-      uint8_t* lds = smem + buf * kStage;
-      const int left = k1 - k0 - at * BK;
-      si.issue(lds, at * stepi + (lo_i ? I.plane : 0), left, w.wave, w.lane);
-      sj.issue(lds + SI::kBytes, at * stepj + (lo_j ? J.plane : 0), left, w.wave, w.lane);
-      if (++at == steps) { at = 0; ++prod; }
+      left = prod < NP ? k1 - k0 - at * BK : 0;
+      shi = at * stepi + (lo_i ? I.plane : 0);
+      shj = at * stepj + (lo_j ? J.plane : 0);
+      if (++at >= steps) { at = 0; ++prod; }
     };
-    int fill = 0;  // buffer of the next stage to issue
+    auto issue = [&](int u, uint8_t* lds) {
+      if (u < SI::kPer) si.issue(u, lds, shi, left, w.wave, w.lane);
+      else sj.issue(u - SI::kPer, lds + SI::kBytes, shj, left, w.wave, w.lane);
+    };
 #pragma unroll
-    for (int s = 0; s < ST - 1; ++s) {
-      if (s < total) issue(fill);
-      ++fill;
+    for (int s = 0; s < ST; ++s) {
+      aim();
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) issue(u, smem + s * kStage);
     }
+    uint4 fi[2][TI], fj[2][TJ];
+    auto fetch = [&](int buf, int kk, int set) {
+      const uint8_t* li = smem + buf * kStage;
+#pragma unroll
+      for (int b = 0; b < TI; ++b) fi[set][b] = si.frag(li, b, kk);
+#pragma unroll
+      for (int a = 0; a < TJ; ++a) fj[set][a] = sj.frag(li + SI::kBytes, a, kk);
+    };
+    wait_vm_barrier<(ST - 1) * kPer>();
+    fetch(0, 0, 0);
     int buf = 0;
+    constexpr int mf = TI * TJ;
     for (int st = 0; st < total; ++st) {
-      // stage st is whole once at most the later issued stages are outstanding; past the barrier
-      // every wave is done with the buffer that is refilled next
-      if (ST > 2 && st + ST - 2 < total) wait_vm_barrier<(ST - 2) * kPer>();
-      else if (ST > 3 && st + ST - 3 < total) wait_vm_barrier<(ST > 3 ? ST - 3 : 0) * kPer>();
-      else wait_vm_barrier<0>();
-      if (st + ST - 1 < total) issue(fill);
-      fill = fill + 1 == ST ? 0 : fill + 1;
-      if (NP > 1 && st == (NP - 1) * steps) {
+      if (NP > 1 && F16 && st == (NP - 1) * steps) {
 #pragma unroll
         for (int a = 0; a < TJ; ++a)
 #pragma unroll
           for (int b = 0; b < TI; ++b)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[a][b][r] *= kLoScale;
+            for (int r = 0; r < 16; ++r) acc[a][b][r] *= kLo;
       }
-      const uint8_t* li = smem + buf * kStage;
-      const uint8_t* lj = li + SI::kBytes;
-      uint4 fi[2][TI], fj[2][TJ];
-#pragma unroll
-      for (int b = 0; b < TI; ++b) fi[0][b] = si.frag(li, b, 0);
-#pragma unroll
-      for (int a = 0; a < TJ; ++a) fj[0][a] = sj.frag(lj, a, 0);
+      const int next = buf + 1 == ST ? 0 : buf + 1;
 #pragma unroll
       for (int kk = 0; kk < BK / 16; ++kk) {
-        if (kk + 1 < BK / 16) {
-#pragma unroll
-          for (int b = 0; b < TI; ++b) fi[(kk + 1) & 1][b] = si.frag(li, b, kk + 1);
-#pragma unroll
-          for (int a = 0; a < TJ; ++a) fj[(kk + 1) & 1][a] = sj.frag(lj, a, kk + 1);
+        const bool tail = kk + 1 == BK / 16;
+        if (tail) {
+          wait_vm_barrier<(ST - 2) * kPer>();
+          aim();
+          fetch(next, 0, 0);
+        } else {
+          fetch(buf, kk + 1, (kk + 1) & 1);
         }
-#pragma unroll
-        for (int a = 0; a < TJ; ++a)
-#pragma unroll
-          for (int b = 0; b < TI; ++b) acc[a][b] = mfma<F16>(fj[kk & 1][a], fi[kk & 1][b], acc[a][b]);
         if constexpr (SUM) {
           // the reduction's sum of I: the hi plane in the last product, lo where it runs with J's hi
           const bool lo = NP == 3 ? st >= steps && st < 2 * steps : NP == 2 ? st < steps : false;
           if (want && (lo || st >= (NP - 1) * steps)) {
 #pragma unroll
             for (int b = 0; b < TI; ++b) {
-              const uint32_t u[4] = {fi[kk & 1][b].x, fi[kk & 1][b].y, fi[kk & 1][b].z, fi[kk & 1][b].w};
-              float s = 0.f;
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                s += F16 ? h2f(u[e] & 0xffff) + h2f(u[e] >> 16) : bf2f(u[e] & 0xffff) + bf2f(u[e] >> 16);
-              isum[b] += lo ? s * kLoScale : s;
+              const float s = sum8<F16>(fi[kk & 1][b]);
+              isum[b] += lo ? s * kLo : s;
             }
           }
         }
+#pragma unroll
+        for (int x = 0; x < mf; ++x) {
+          acc[x / TI][x % TI] = mfma<F16>(fj[kk & 1][x / TI], fi[kk & 1][x % TI], acc[x / TI][x % TI]);
+          if (tail) {
+            constexpr int per = (kPer + mf - 1) / mf;
+#pragma unroll
+            for (int y = x * per; y < (x + 1) * per && y < kPer; ++y) issue(y, smem + buf * kStage);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      buf = buf + 1 == ST ? 0 : buf + 1;
+      buf = next;
     }
+    wait_vm_barrier<0>();
   }
 };
 
 // Tiles in the order that an XCD's L2 serves best: workgroups are dealt to the 8 XCDs in turn, so
 // each XCD gets one run of the order; inside it, groups of ``gi`` row tiles stay while the column
-// tiles go by.
-struct Order {
-  int ti, tj, gi, splits;
-  __device__ __forceinline__ void at(int bid, int grid, int& i, int& j, int& s) const {
-    const int x = bid & 7, q = grid >> 3, r = grid & 7;
-    const int t = x * q + min(x, r) + (bid >> 3);
-    const int tiles = ti * tj;
-    s = t / tiles;
-    const int u = t - s * tiles;
-    const int per = gi * tj, grp = u / per, v = u - grp * per;
-    const int rows = min(gi, ti - grp * gi);
-    j = v / rows;
-    i = grp * gi + (v - j * rows);
+// tiles go by.  The order covers the live tiles only (a device count decides how many there are), so
+// that the work is spread over the XCDs whatever their number.
+__device__ __forceinline__ void tile_at(int bid, int live, int ti, int tj, int gi, int& i, int& j, int& s) {
+  const int x = bid & 7, q = live >> 3, r = live & 7;
+  const int t = x * q + min(x, r) + (bid >> 3);
+  const int tiles = ti * tj;
+  s = t / tiles;
+  const int u = t - s * tiles;
+  const int per = gi * tj, grp = u / per, v = u - grp * per;
+  const int rows = min(gi, ti - grp * gi);
+  j = v / rows;
+  i = grp * gi + (v - j * rows);
+}
+
+constexpr int kGroup = 8;  // row tiles a group
+
+// Splits of a reduction: as many as fill the chip's ``slots`` workgroups once, each at least ``least``
+// steps long, ``most`` at most.  The same on the host and on the device, where the sizes may be known
+// only there.
+struct Split {
+  int slots, least, most = 64;
+  __host__ __device__ int of(int64_t tiles, int64_t nk) const {
+    int64_t s = slots / (tiles < 1 ? 1 : tiles);
+    s = s < nk / least ? s : nk / least;
+    return int(s < 1 ? 1 : s > most ? most : s);
   }
 };
 
@@ -322,9 +365,8 @@ struct Emit {
   int64_t ldo;
   int bf16;                 // out's type: bf16 or fp32
   int nj;                   // columns
-  int vec;                  // rows start 4-element aligned: quads go out as one store
+  int vec;                  // rows start 16-byte aligned: eights go out in whole vectors
   int accumulate;           // add to what out holds
-  int zero_from;            // rows i >= zero_from are zero
   const void* bias;         // [nj], or null
   int bias_bf16;
   const uint8_t* q;         // e4m3 checkpoint [i][ldq] whose gelu' multiplies, or null
@@ -346,65 +388,99 @@ struct Emit {
     if (gl) v *= *gl / float(max(*gn, 1));
     return v;
   }
-  __device__ __forceinline__ void quad(int i, int j, float (&v)[4], bool keep = true) const;
+  // columns j .. j+7 of row i (j % 8 == 0); ``keep`` false: the row is zero whatever the factors are
+  __device__ __forceinline__ void eight(int i, int j, float (&v)[8], bool keep = true) const {
+    if (j >= nj) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = keep ? scaled(v[e]) : 0.f;
+    if (q) {  // ldq % 32 == 0
+      const uint2 u = *reinterpret_cast<const uint2*>(q + int64_t(i) * ldq + j);
+      const float s = __uint_as_float(uint32_t(qs[int64_t(i) * (ldq >> 5) + (j >> 5)]) << 23);
+      v[0] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u.x, 0) * s);
+      v[1] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u.x, 1) * s);
+      v[2] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u.x, 2) * s);
+      v[3] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u.x, 3) * s);
+      v[4] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u.y, 0) * s);
+      v[5] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u.y, 1) * s);
+      v[6] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u.y, 2) * s);
+      v[7] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u.y, 3) * s);
+    }
+    if (bias) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (j + e < nj)
+          v[e] += bias_bf16 ? bf2f(static_cast<const uint16_t*>(bias)[j + e]) : static_cast<const float*>(bias)[j + e];
+    }
+    put(i, j, v);
+  }
+  __device__ __forceinline__ void put(int i, int j, const float (&v)[8]) const {
+    const bool whole = vec && j + 8 <= nj;
+    if (bf16) {
+      uint16_t* o = static_cast<uint16_t*>(out) + int64_t(i) * ldo + j;
+      if (whole) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (accumulate) u = *reinterpret_cast<const uint4*>(o);
+        auto two = [&](uint32_t old, float x, float y) {
+          return uint32_t(f2bf(x + bf2f(old & 0xffff))) | (uint32_t(f2bf(y + bf2f(old >> 16))) << 16);
+        };
+        *reinterpret_cast<uint4*>(o) =
+            make_uint4(two(u.x, v[0], v[1]), two(u.y, v[2], v[3]), two(u.z, v[4], v[5]), two(u.w, v[6], v[7]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (j + e < nj) o[e] = f2bf(v[e] + (accumulate ? bf2f(o[e]) : 0.f));
+      }
+    } else {
+      float* o = static_cast<float*>(out) + int64_t(i) * ldo + j;
+      if (whole) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+        if (accumulate) {
+          a = *reinterpret_cast<const float4*>(o);
+          b = *reinterpret_cast<const float4*>(o + 4);
+        }
+        *reinterpret_cast<float4*>(o) = make_float4(v[0] + a.x, v[1] + a.y, v[2] + a.z, v[3] + a.w);
+        *reinterpret_cast<float4*>(o + 4) = make_float4(v[4] + b.x, v[5] + b.y, v[6] + b.z, v[7] + b.w);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (j + e < nj) o[e] = v[e] + (accumulate ? o[e] : 0.f);
+      }
+    }
+  }
 };
 
-// gelu_tanh'(c) to fp32 accuracy (common.h's form: 1 ulp exp2 and reciprocal)
-// ``keep`` false: the row is zero whatever the factors are.
-__device__ __forceinline__ void Emit::quad(int i, int j, float (&v)[4], bool keep) const {
-  if (j >= nj) return;
-  keep = keep && i < zero_from;
+// A wave's block of 32 rows x 32 TJ columns goes through its own part of the LDS, fp32, so that the
+// stores move whole lines: straight from the accumulators a store would scatter 32 rows' worth of 16
+// or 32 bytes.  Chunks of 16 bytes are XOR-swizzled by the row: no bank conflicts either way.
+// ``g(i, j, v)`` gets eight columns of a row at a time, a lane the same columns each time.
+template <class T, class G>
+__device__ __forceinline__ void through_lds(uint8_t* smem, const typename T::Where& w, const f32x16 (&acc)[T::TJ][T::TI],
+                                            int b, G&& g) {
+  constexpr int CH = 8 * T::TJ;  // chunks a row
+  static_assert(T::kLds / T::NW >= 32 * CH * 16, "a wave's block fits its part of the LDS");
+  uint8_t* mine = smem + w.wave * (T::kLds / T::NW / 16 * 16);
+  uint8_t* row = mine + w.il * (CH * 16);
+  const int sw = 16 * (w.il & (CH - 1)) ^ (16 * w.h);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = keep ? scaled(v[e]) : 0.f;
-  if (q) {
-    const uint32_t u = *reinterpret_cast<const uint32_t*>(q + int64_t(i) * ldq + j);  // ldq % 32 == 0, j % 4 == 0
-    const float s = __uint_as_float(uint32_t(qs[int64_t(i) * (ldq >> 5) + (j >> 5)]) << 23);
-    v[0] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u, 0) * s);
-    v[1] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u, 1) * s);
-    v[2] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u, 2) * s);
-    v[3] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u, 3) * s);
-  }
-  const int n = min(4, nj - j);
-  if (bias) {
+  for (int a = 0; a < T::TJ; ++a)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < n)
-        v[e] += bias_bf16 ? bf2f(static_cast<const uint16_t*>(bias)[j + e]) : static_cast<const float*>(bias)[j + e];
-  }
-  if (bf16) {
-    uint16_t* o = static_cast<uint16_t*>(out) + int64_t(i) * ldo + j;
-    if (vec && n == 4) {
-      if (accumulate) {
-        const uint2 u = *reinterpret_cast<const uint2*>(o);
-        v[0] += bf2f(u.x & 0xffff);
-        v[1] += bf2f(u.x >> 16);
-        v[2] += bf2f(u.y & 0xffff);
-        v[3] += bf2f(u.y >> 16);
-      }
-      *reinterpret_cast<uint2*>(o) = make_uint2(uint32_t(f2bf(v[0])) | (uint32_t(f2bf(v[1])) << 16),
-                                                uint32_t(f2bf(v[2])) | (uint32_t(f2bf(v[3])) << 16));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < n) o[e] = f2bf(v[e] + (accumulate ? bf2f(o[e]) : 0.f));
+    for (int q = 0; q < 4; ++q) {
+      *reinterpret_cast<float4*>(row + ((16 * (8 * a + 2 * q)) ^ sw)) =
+          make_float4(acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
     }
-  } else {
-    float* o = static_cast<float*>(out) + int64_t(i) * ldo + j;
-    if (vec && n == 4) {
-      if (accumulate) {
-        const float4 u = *reinterpret_cast<const float4*>(o);
-        v[0] += u.x;
-        v[1] += u.y;
-        v[2] += u.z;
-        v[3] += u.w;
-      }
-      *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < n) o[e] = v[e] + (accumulate ? o[e] : 0.f);
-    }
+  __builtin_amdgcn_wave_barrier();
+  constexpr int EI = CH / 2;     // eights a row
+  constexpr int RP = 64 / EI;    // rows a pass
+  const int e = w.lane % EI;
+#pragma unroll 2
+  for (int r = w.lane / EI; r < 32; r += RP) {
+    const uint8_t* from = mine + r * (CH * 16);
+    const int x = 16 * ((2 * e) ^ (r & (CH - 1)));
+    const float4 lo = *reinterpret_cast<const float4*>(from + x), hi = *reinterpret_cast<const float4*>(from + (x ^ 16));
+    float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    g((w.wi * T::TI + b) * 32 + r, w.wj * T::TJ * 32 + 8 * e, v);
   }
+  __builtin_amdgcn_wave_barrier();
 }
 
 struct GemmArgs {
@@ -412,14 +488,21 @@ struct GemmArgs {
   const int* ni_dev;     // rows in use (<= I.n), or null: all
   const int* nk_dev;     // reduction length in use (<= nk), or null: all
   int nk;
-  Order o;
-  // o.splits > 1 or slab given: fp32 partial results [split][I.n][lds] (``add``: onto what is there)
+  Split split;
+  int nk_split;          // length that the number of splits goes by
+  // fp32 partial results [split][rows in use][lds] (``add``: onto what is there), or null: one split
   float* slab;
   int64_t lds;
   int add;
   float* bslab;          // [split][I.n] partial sums of I over k (col I), or null
   void* bout;            // their result when there is no slab, in out's type
   Emit e;
+
+  __device__ __forceinline__ int rows() const { return ni_dev ? min(I.n, *ni_dev) : I.n; }
+  __device__ __forceinline__ int length() const { return nk_dev ? min(nk, *nk_dev) : nk; }
+  __device__ __forceinline__ int splits(int64_t tiles) const {
+    return slab ? split.of(tiles, nk_dev ? length() : nk_split) : 1;
+  }
 };
 
 // one split's reduction range: whole stages, as even as they go
@@ -430,7 +513,7 @@ __device__ __forceinline__ void split_range(int nk, int splits, int s, int bk, i
 }
 
 __device__ __forceinline__ void emit_sum(const Emit& e, void* out, int i, float v) {
-  v = i < e.zero_from ? e.scaled(v, false) : 0.f;
+  v = e.scaled(v, false);
   if (e.bf16) {
     uint16_t* o = static_cast<uint16_t*>(out) + i;
     *o = f2bf(v + (e.accumulate ? bf2f(*o) : 0.f));
@@ -443,20 +526,28 @@ __device__ __forceinline__ void emit_sum(const Emit& e, void* out, int i, float 
 template <class T, bool SUM>
 __global__ __launch_bounds__(T::kThreads, 2) void gemm_kernel(GemmArgs p) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[T::kLds];
-  int ti, tj, s;
-  p.o.at(blockIdx.x, gridDim.x, ti, tj, s);
-  const int i0 = ti * T::BI, j0 = tj * T::BJ;
   Operand I = p.I;
-  if (p.ni_dev) I.n = min(I.n, *p.ni_dev);
-  if (i0 >= I.n) return;
-  const int nk = p.nk_dev ? min(p.nk, *p.nk_dev) : p.nk;
-  int k0, k1;
-  split_range(nk, p.o.splits, s, T::BK, k0, k1);
+  I.n = p.rows();
+  const int ni = (I.n + T::BI - 1) / T::BI, nj = (p.e.nj + T::BJ - 1) / T::BJ;
+  const int splits = p.splits(int64_t(ni) * nj), live = ni * nj * splits;
+  if (int(blockIdx.x) >= live) return;
+  int ti, tj, s, k0, k1;
+  tile_at(blockIdx.x, live, ni, nj, kGroup, ti, tj, s);
+  const int i0 = ti * T::BI, j0 = tj * T::BJ;
+  split_range(p.length(), splits, s, T::BK, k0, k1);
   const typename T::Where w;
   const bool want = SUM && (p.bslab || p.bout) && tj == 0 && w.wj == 0;
   f32x16 acc[T::TJ][T::TI];
   float isum[T::TI];
   T::template run<SUM>(smem, I, p.J, i0, j0, k0, k1, acc, isum, want);
+  Emit o = p.e;
+  if (p.slab) {
+    o.out = p.slab + int64_t(s) * I.n * p.lds;
+    o.ldo = o.nj = int(p.lds);
+    o.bf16 = 0;
+    o.vec = 1;
+    o.accumulate = p.add;
+  }
 #pragma unroll
   for (int b = 0; b < T::TI; ++b) {
     const int i = i0 + w.i(b);
@@ -469,94 +560,69 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm_kernel(GemmArgs p) {
         }
       }
     }
-    if (i >= I.n) continue;
-#pragma unroll
-    for (int a = 0; a < T::TJ; ++a) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int j = j0 + w.j(a, g);
-        float v[4] = {acc[a][b][4 * g], acc[a][b][4 * g + 1], acc[a][b][4 * g + 2], acc[a][b][4 * g + 3]};
-        if (p.slab) {
-          if (j < p.lds) {
-            float4* o = reinterpret_cast<float4*>(p.slab + (int64_t(s) * p.I.n + i) * p.lds + j);
-            if (p.add) {
-              const float4 u = *o;
-              v[0] += u.x;
-              v[1] += u.y;
-              v[2] += u.z;
-              v[3] += u.w;
-            }
-            *o = make_float4(v[0], v[1], v[2], v[3]);
-          }
-        } else {
-          p.e.quad(i, j, v);
-        }
-      }
-    }
+    through_lds<T>(smem, w, acc, b, [&](int r, int c, float(&v)[8]) {
+      if (i0 + r >= I.n) return;
+      if (p.slab) o.put(i0 + r, j0 + c, v);
+      else o.eight(i0 + r, j0 + c, v);
+    });
   }
 }
 
-// Sums the splits of a slab and stores the result; ``inv`` (or null) maps an output row to its row of
-// the slab, -1 where the row is zero.  One thread a quad of columns, then one a partial sum.
+// Sums the splits of a product's slab and stores the result; ``inv`` (or null) maps an output row to its
+// row of the slab, -1 where the row is zero.  LANES threads take eight columns together, each every
+// LANES-th split; behind them one thread a partial sum.
 struct FinishArgs {
-  const float* slab;
-  int64_t lds;
-  int splits, slab_rows, rows;
+  GemmArgs g;
+  int bi, bj;   // the product's tile
+  int rows;
   const int* inv;
-  const float* bslab;
-  void* bout;
-  Emit e;
 };
 
+template <int LANES>
 static __global__ __launch_bounds__(256) void finish_kernel(FinishArgs p) {
-  const int quads = (p.e.nj + 3) >> 2;
-  const int64_t n = int64_t(p.rows) * quads;
-  const int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int eights = (p.g.e.nj + 7) >> 3;
+  const int64_t n = int64_t(p.rows) * eights;
+  const int64_t t = (int64_t(blockIdx.x) * 256 + threadIdx.x) / LANES;
+  const int part = threadIdx.x % LANES;
+  const int used = p.g.rows();
+  const int splits = p.g.splits(int64_t((used + p.bi - 1) / p.bi) * ((p.g.e.nj + p.bj - 1) / p.bj));
   if (t < n) {
-    const int i = int(t / quads), j = 4 * int(t - int64_t(i) * quads);
+    const int i = int(t / eights), j = 8 * int(t - int64_t(i) * eights);
     const int src = p.inv ? p.inv[i] : i;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (src >= 0) {
-      const float* a = p.slab + int64_t(src) * p.lds + j;
-      for (int s = 0; s < p.splits; ++s) {
-        const float4 u = *reinterpret_cast<const float4*>(a + int64_t(s) * p.slab_rows * p.lds);
-        v[0] += u.x;
-        v[1] += u.y;
-        v[2] += u.z;
-        v[3] += u.w;
+      const float* a = p.g.slab + int64_t(src) * p.g.lds + j;
+#pragma unroll 4
+      for (int s = part; s < splits; s += LANES) {
+        const float* b = a + int64_t(s) * used * p.g.lds;
+        const float4 x = *reinterpret_cast<const float4*>(b), y = *reinterpret_cast<const float4*>(b + 4);
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+        v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
       }
     }
-    p.e.quad(i, j, v, src >= 0);
-  } else if (p.bslab && t - n < p.rows) {
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += __shfl_xor(v[e], o, 64);
+    if (part == 0) p.g.e.eight(i, j, v, src >= 0);
+  } else if (p.g.bslab && t - n < p.rows && part == 0) {
     const int i = int(t - n);
     float v = 0.f;
-    for (int s = 0; s < p.splits; ++s) v += p.bslab[int64_t(s) * p.slab_rows + i];
-    emit_sum(p.e, p.bout, i, v);
+    for (int s = 0; s < splits; ++s) v += p.g.bslab[int64_t(s) * p.g.I.n + i];
+    emit_sum(p.g.e, p.g.bout, i, v);
   }
-}
-
-inline void finish(const FinishArgs& p, hipStream_t st) {
-  const int64_t n = int64_t(p.rows) * ((p.e.nj + 3) / 4) + (p.bslab ? p.rows : 0);
-  hipLaunchKernelGGL(finish_kernel, dim3(unsigned((n + 255) / 256)), dim3(256), 0, st, p);
-  check_launch();
-}
-
-template <class T, bool SUM>
-inline void gemm(GemmArgs p, hipStream_t st) {
-  p.o.ti = (p.I.n + T::BI - 1) / T::BI;
-  p.o.tj = (p.e.nj + T::BJ - 1) / T::BJ;
-  hipLaunchKernelGGL((gemm_kernel<T, SUM>), dim3(unsigned(int64_t(p.o.ti) * p.o.tj * p.o.splits)), dim3(T::kThreads), 0,
-                     st, p);
-  check_launch();
 }
 
 // ---- fp32 -> planes ----------------------------------------------------------------------------
 
-constexpr int kAmaxBlocks = 256;  // partial maxima a tensor
+constexpr int kAmaxBlocks = 1024;  // partial maxima a tensor
 
 // the largest of a tensor's partial maxima, by every thread of a block of 256
 __device__ __forceinline__ float amax_of(const float* part, float* lds4) {
-  float m = wave_max(part[threadIdx.x]);
+  float m = 0.f;
+#pragma unroll
+  for (int k = 0; k < kAmaxBlocks / 256; ++k) m = fmaxf(m, part[threadIdx.x + 256 * k]);
+  m = wave_max(m);
   __syncthreads();  // lds4 may still be read from an earlier call
   if ((threadIdx.x & 63) == 0) lds4[threadIdx.x >> 6] = m;
   __syncthreads();
@@ -593,6 +659,7 @@ static __global__ __launch_bounds__(256) void amax_kernel(Rows a, Rows b, const 
     }
     const float* row = x.p + int64_t(r) * x.ld;
     if (vec) {
+#pragma unroll 4
       for (int c = 4 * lane; c < x.width; c += 256) {
         const float4 u = *reinterpret_cast<const float4*>(row + c);
         m = fmaxf(m, fmaxf(fmaxf(of(u.x), of(u.y)), fmaxf(of(u.z), of(u.w))));
@@ -664,26 +731,74 @@ inline void split(const Rows& x, uint16_t* out, int kp, int64_t plane, const flo
 
 inline int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
-// Tiles: kBig (256 columns x 128 rows) for full batches; kFew (128 x 32) for a handful of rows, whose
-// products only stream the weights.
+inline int whole_rows(uintptr_t p, int64_t ld, bool bf16) { return p % 16 == 0 && ld % (bf16 ? 8 : 4) == 0; }
+
+// Tiles (columns x rows).  A CU is bound by the rate at which lines reach its LDS, so the tile should be
+// as large as the product fills the chip with:
+//   kWide 256 x 256, one workgroup of 8 waves a CU;
+//   kBig  256 x 128, two workgroups a CU: one's epilogue runs beside the other's products;
+//   kSq   128 x 128, two a CU;
+//   kFew  128 x 32 (row operands), for a handful of rows, whose products only stream the weights.
+template <bool F16, int NP, bool IT, bool JT> using Wide = Tile<F16, NP, IT, JT, 2, 4, 4, 2, 64, 2>;
 template <bool F16, int NP, bool IT, bool JT> using Big = Tile<F16, NP, IT, JT, 2, 2, 4, 2, 32, 3>;
-template <bool F16, int NP, bool IT, bool JT> using Mid = Tile<F16, NP, IT, JT, 2, 2, 2, 1, 64, 3>;
+template <bool F16, int NP, bool IT, bool JT> using Sq = Tile<F16, NP, IT, JT, 2, 2, 2, 2, 64, 2>;
 template <bool F16, int NP, bool IT, bool JT> using Few = Tile<F16, NP, IT, JT, 4, 1, 1, 1, 64, 3>;
 
-enum { kBig = 0, kMid = 1, kFew = 2 };
-inline int tile_bj(int t) { return t == kBig ? 256 : 128; }
-inline int tile_bi(int t) { return t == kBig ? 128 : t == kMid ? 64 : 32; }
+enum { kWide = 0, kBig = 1, kSq = 2, kFew = 3 };
+inline int tile_bj(int t) { return t <= kBig ? 256 : 128; }
+inline int tile_bi(int t) { return t == kWide ? 256 : t == kFew ? 32 : 128; }
+inline int tile_slots(int t) { return t == kWide ? 256 : 512; }  // workgroups that the chip holds
 
 inline int64_t tiles_of(int tile, int64_t ni, int64_t nj) {
   return ((ni + tile_bi(tile) - 1) / tile_bi(tile)) * ((nj + tile_bj(tile) - 1) / tile_bj(tile));
 }
 
-// splits of a reduction of ``nk`` so that tiles x splits comes near two workgroups a CU, each split
-// at least ``least`` long
-inline int splits_for(int64_t tiles, int64_t nk, int64_t least) {
-  int64_t s = (512 + tiles - 1) / tiles;
-  s = s < nk / least ? s : nk / least;
-  return int(s < 1 ? 1 : s > 64 ? 64 : s);
+// ``steps``: reduction length times products.
+inline int choose_tile(int64_t ni, int64_t nj, int64_t steps, bool col_i) {
+  if (ni <= 32 && !col_i) return kFew;
+  const int64_t w = tiles_of(kWide, ni, nj), b = tiles_of(kBig, ni, nj);
+  // the busiest CU's work: a kBig tile is half a kWide one at 0.84 of its rate (850 against 1000 TFLOP/s
+  // over a long reduction); over a short one kWide's epilogue, which nothing hides, costs more than that
+  if (w >= 192 && steps >= 1536 && (w + 255) / 256 * 10 <= (b + 255) / 256 * 6) return kWide;
+  return b >= 256 ? kBig : kSq;
+}
+
+// Largest grid and slab (in rows) of a product whose rows in use are known on the device only: any
+// number up to ni.
+struct Extent {
+  int64_t grid, slab_rows;
+};
+inline Extent extent_of(int tile, int64_t ni, int64_t nj, const Split& split, int64_t nk) {
+  Extent x{1, 1};
+  for (int64_t t = 1, n = tiles_of(tile, ni, 1); t <= n; ++t) {
+    const int64_t tiles = t * tiles_of(tile, 1, nj), s = split.of(tiles, nk), rows = s * std::min(ni, t * tile_bi(tile));
+    x.grid = std::max(x.grid, tiles * s);
+    x.slab_rows = std::max(x.slab_rows, rows);
+  }
+  return x;
+}
+
+template <class T, bool SUM>
+inline void launch_gemm(const GemmArgs& p, int64_t grid, hipStream_t st) {
+  hipLaunchKernelGGL((gemm_kernel<T, SUM>), dim3(unsigned(grid)), dim3(T::kThreads), 0, st, p);
+  check_launch();
+}
+
+template <bool F16, int NP, bool IT, bool JT, bool SUM>
+inline void gemm(int tile, const GemmArgs& p, int64_t grid, hipStream_t st) {
+  if (tile == kWide) launch_gemm<Wide<F16, NP, IT, JT>, SUM>(p, grid, st);
+  else if (tile == kBig) launch_gemm<Big<F16, NP, IT, JT>, SUM>(p, grid, st);
+  else if (tile == kSq) launch_gemm<Sq<F16, NP, IT, JT>, SUM>(p, grid, st);
+  else if constexpr (!IT) launch_gemm<Few<F16, NP, IT, JT>, SUM>(p, grid, st);
+}
+
+inline void finish(int tile, const GemmArgs& g, int rows, const int* inv, hipStream_t st) {
+  const FinishArgs p = {g, tile_bi(tile), tile_bj(tile), rows, inv};
+  const int64_t n = int64_t(rows) * ((g.e.nj + 7) / 8) + (g.bslab ? rows : 0);
+  // few outputs: eight lanes on each keep the loads of many splits in flight
+  if (n <= 16384) hipLaunchKernelGGL((finish_kernel<8>), dim3(unsigned((n * 8 + 255) / 256)), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((finish_kernel<1>), dim3(unsigned((n + 255) / 256)), dim3(256), 0, st, p);
+  check_launch();
 }
 
 }  // namespace gt

@@ -24,6 +24,7 @@
 #include "ops.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace voda {
 
@@ -93,6 +94,7 @@ __global__ __launch_bounds__(256) void xent_gather_kernel(GatherArgs p) {
   // out of the L2), which is cheaper than a second launch
   const int r0 = blockIdx.x * kGatherRows;
   int c = 0;
+#pragma unroll 8
   for (int r = t; r < r0; r += 256) c += labelled(p.labels[r], p.ignore, p.classes);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
@@ -159,8 +161,7 @@ __global__ __launch_bounds__(256) void xent_gather_kernel(GatherArgs p) {
 
 struct LogitArgs {
   Operand X, W;
-  int width, classes;
-  Order o;
+  int width, classes, tj;
   int v0, v1;           // vocabulary columns of this launch
   const float* bias32;
   const XentDev* dev;
@@ -178,15 +179,16 @@ struct LogitArgs {
 
 // Rows are the tile's i, vocabulary columns its j.  The epilogue is vector work that the matrix cores
 // wait for unless another workgroup of the CU is in its main loop: two workgroups a CU (72 KB of LDS each).
-template <class T, bool F16, bool BWD>
+template <class T, bool F16, bool BWD, bool TWO>
 __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[T::kLds];
-  int ti, tj, s;
-  p.o.at(blockIdx.x, gridDim.x, ti, tj, s);
-  const int i0 = ti * T::BI, j0 = p.v0 + tj * T::BJ;
   Operand X = p.X;
   X.n = min(X.n, p.dev->n);
-  if (i0 >= X.n) return;
+  const int ni = (X.n + T::BI - 1) / T::BI, live = ni * p.tj;
+  if (int(blockIdx.x) >= live) return;
+  int ti, tj, s;
+  tile_at(blockIdx.x, live, ni, p.tj, kGroup, ti, tj, s);
+  const int i0 = ti * T::BI, j0 = p.v0 + tj * T::BJ;
   f32x16 acc[T::TJ][T::TI];
   float unused[T::TI];
   T::template run<false>(smem, X, p.W, i0, j0, 0, p.width, acc, unused);
@@ -198,7 +200,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
   }
   // z = products + bias; columns past the classes get the bias's -inf
 #pragma unroll
-  for (int a = 0; a < T::TJ; ++a) {
+  for (int a = 0; a < (BWD ? 0 : T::TJ); ++a) {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const float4 b4 = *reinterpret_cast<const float4*>(p.bias32 + j0 + w.j(a, g));
@@ -215,10 +217,10 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
   }
 #pragma unroll
   for (int c = 0; c < T::TI; ++c) {
-    const int i = i0 + w.i(c);
-    const bool live = i < X.n;
-    const int y = live ? p.lab[i] : -1;
     if constexpr (!BWD) {
+      const int i = i0 + w.i(c);
+      const bool live = i < X.n;
+      const int y = live ? p.lab[i] : -1;
       float m = -INFINITY;
 #pragma unroll
       for (int a = 0; a < T::TJ; ++a)
@@ -262,40 +264,48 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
         }
       }
     } else {
-      const float2 st = live ? p.stat[i] : make_float2(0.f, 0.f);
-      uint16_t* g0 = p.G + int64_t(i) * p.ldg + (j0 - p.v0);
-      if (!live) continue;
-#pragma unroll
-      for (int a = 0; a < T::TJ; ++a) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int j = w.j(a, g);
-          float v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[e] = __builtin_amdgcn_exp2f((acc[a][c][4 * g + e] - st.x) * kLog2e) * st.y;
-            if (j0 + j + e == y) v[e] -= 1.f;
-          }
-          if constexpr (F16) {
-            uint16_t hi[4], lo[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) split2(v[e] * kGScale, hi[e], lo[e]);
-            *reinterpret_cast<uint2*>(g0 + j) = make_uint2(hi[0] | (uint32_t(hi[1]) << 16), hi[2] | (uint32_t(hi[3]) << 16));
-            *reinterpret_cast<uint2*>(g0 + p.gplane + j) =
-                make_uint2(lo[0] | (uint32_t(lo[1]) << 16), lo[2] | (uint32_t(lo[3]) << 16));
-          } else {
-            *reinterpret_cast<uint2*>(g0 + j) = make_uint2(uint32_t(f2bf(v[0])) | (uint32_t(f2bf(v[1])) << 16),
-                                                           uint32_t(f2bf(v[2])) | (uint32_t(f2bf(v[3])) << 16));
-          }
+      float bias[8];
+      bool have = false;
+      through_lds<T>(smem, w, acc, c, [&](int r, int j, float(&v)[8]) {
+        if (i0 + r >= X.n) return;
+        if (!have) {  // a lane's columns stay the same
+          const float* b = p.bias32 + j0 + j;
+          const float4 x = *reinterpret_cast<const float4*>(b), y = *reinterpret_cast<const float4*>(b + 4);
+          bias[0] = x.x; bias[1] = x.y; bias[2] = x.z; bias[3] = x.w;
+          bias[4] = y.x; bias[5] = y.y; bias[6] = y.z; bias[7] = y.w;
+          have = true;
         }
-      }
+        const float2 st = p.stat[i0 + r];
+        const int y = p.lab[i0 + r] - (j0 + j);
+        uint16_t* g = p.G + int64_t(i0 + r) * p.ldg + (j0 - p.v0) + j;
+        uint16_t hi[8], lo[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float z = v[e];
+          if constexpr (F16) z = z * sx * sw;
+          float d = __builtin_amdgcn_exp2f((z + bias[e] - st.x) * kLog2e) * st.y;
+          if (e == y) d -= 1.f;
+          if constexpr (F16) split2(d * kGScale, hi[e], lo[e]);
+          else hi[e] = f2bf(d);
+          if constexpr (TWO && !F16) lo[e] = f2bf(d - bf2f(hi[e]));
+        }
+        auto eight = [](const uint16_t(&a)[8]) {
+          return make_uint4(a[0] | (uint32_t(a[1]) << 16), a[2] | (uint32_t(a[3]) << 16), a[4] | (uint32_t(a[5]) << 16),
+                            a[6] | (uint32_t(a[7]) << 16));
+        };
+        *reinterpret_cast<uint4*>(g) = eight(hi);
+        if constexpr (TWO) *reinterpret_cast<uint4*>(g + p.gplane) = eight(lo);
+      });
     }
   }
 }
 
-// Joins the slots of 64 rows a workgroup: 16 waves each take every 16th slot.  The last workgroup to
-// finish adds the workgroups' sums up, in their order.
+// Joins the slots of ROWS rows a workgroup: 1024 / ROWS groups of ROWS threads each take every so-manieth
+// slot.  The last workgroup to finish adds the workgroups' sums up, in their order.  16 rows where
+// there are few (their slots are read by 64 groups at once), 64 otherwise (a fourth of the workgroups
+// for the count that finds the last one).
 constexpr int kJoinWaves = 16;
+template <int kJoinRows>
 __global__ __launch_bounds__(64 * kJoinWaves) void xent_join_kernel(const float2* __restrict__ part, int slots, int cap,
                                                                     int slot_cols, const float* __restrict__ zlab,
                                                                     const int* __restrict__ tie,
@@ -303,17 +313,19 @@ __global__ __launch_bounds__(64 * kJoinWaves) void xent_join_kernel(const float2
                                                                     float2* __restrict__ stat, double* __restrict__ lsum,
                                                                     int* __restrict__ csum, float* __restrict__ loss,
                                                                     int64_t* __restrict__ correct) {
-  __shared__ float sm[kJoinWaves][64], ss[kJoinWaves][64], sl[kJoinWaves][64];
+  constexpr int kJoinGroups = 64 * kJoinWaves / kJoinRows, kQ = 64 / kJoinRows;
+  __shared__ float sm[kJoinGroups][kJoinRows], ss[kJoinGroups][kJoinRows], sl[kJoinGroups][kJoinRows];
   __shared__ int last;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row = threadIdx.x % kJoinRows, grp = threadIdx.x / kJoinRows;
   const int n = dev->n;
-  const int i = blockIdx.x * 64 + lane;
+  const int i = blockIdx.x * kJoinRows + row;
   const bool live = i < n;
   const int yslot = live ? lab[i] / slot_cols : 0;
-  const float z = live ? zlab[i] : 0.f;
   float m = -INFINITY, s = 0.f, before = -INFINITY;  // before: largest of the slots in front of the label's
   if (live) {
-    for (int k = wave; k < slots; k += kJoinWaves) {
+#pragma unroll 4
+    for (int k = grp; k < slots; k += kJoinGroups) {
       const float2 v = part[int64_t(k) * cap + i];
       const float nm = fmaxf(m, v.x);
       const float at = nm == -INFINITY ? 0.f : nm;
@@ -322,21 +334,36 @@ __global__ __launch_bounds__(64 * kJoinWaves) void xent_join_kernel(const float2
       if (k < yslot) before = fmaxf(before, v.x);
     }
   }
-  sm[wave][lane] = m;
-  ss[wave][lane] = s;
-  sl[wave][lane] = before;
+  sm[grp][row] = m;
+  ss[grp][row] = s;
+  sl[grp][row] = before;
   __syncthreads();
   if (wave == 0) {
+    // kQ lanes a row, each a share of the groups
+    const int q = lane / kJoinRows;
+    m = -INFINITY;
+    before = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kJoinGroups / kQ; ++k) {
+      m = fmaxf(m, sm[kQ * k + q][row]);
+      before = fmaxf(before, sl[kQ * k + q][row]);
+    }
+#pragma unroll
+    for (int o = kJoinRows; o < 64; o <<= 1) {
+      m = fmaxf(m, __shfl_xor(m, o, 64));
+      before = fmaxf(before, __shfl_xor(before, o, 64));
+    }
+    const float at = m == -INFINITY ? 0.f : m;
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < kJoinGroups / kQ; ++k)
+      s += ss[kQ * k + q][row] * __builtin_amdgcn_exp2f((sm[kQ * k + q][row] - at) * kLog2e);
+#pragma unroll
+    for (int o = kJoinRows; o < 64; o <<= 1) s += __shfl_xor(s, o, 64);
     double l = 0.0;
     int ok = 0;
-    if (live) {
-      for (int k = 0; k < kJoinWaves; ++k) {
-        m = fmaxf(m, sm[k][lane]);
-        before = fmaxf(before, sl[k][lane]);
-      }
-      const float at = m == -INFINITY ? 0.f : m;
-      s = 0.f;
-      for (int k = 0; k < kJoinWaves; ++k) s += ss[k][lane] * __builtin_amdgcn_exp2f((sm[k][lane] - at) * kLog2e);
+    if (live && q == 0) {
+      const float z = zlab[i];
       stat[i] = make_float2(m, 1.f / s);
       // (max - z) first: exact where the label's logit is the largest or near it
       l = double(m - z) + double(logf(s));
@@ -372,27 +399,26 @@ __global__ __launch_bounds__(64 * kJoinWaves) void xent_join_kernel(const float2
   }
 }
 
-// The product's tile: kBig where it gives every CU one, kMid below, kFew for a handful of rows.
-int logits_tile(int rows, int cols) {
-  if (rows <= 32) return kFew;
-  return tiles_of(kBig, rows, cols) >= 256 ? kBig : kMid;
-}
-int tile_slot(int t) { return t == kBig ? 128 : t == kMid ? 64 : 32; }
+// columns of one (max, sum) slot: a wave's part of the tile
+int tile_slot(int t) { return t <= kBig ? 128 : t == kSq ? 64 : 32; }
 
-template <bool F16, bool BWD>
+template <bool F16, bool BWD, bool TWO>
 void launch_logits(LogitArgs& p, int tile, hipStream_t st) {
-  p.o.gi = 8;
-  p.o.splits = 1;
-  p.o.ti = (p.X.n + tile_bi(tile) - 1) / tile_bi(tile);
-  p.o.tj = (p.v1 - p.v0 + tile_bj(tile) - 1) / tile_bj(tile);
-  const dim3 grid(unsigned(int64_t(p.o.ti) * p.o.tj)), block(256);
   constexpr int NP = F16 ? 3 : 1;
-  if (tile == kBig)
-    hipLaunchKernelGGL((xent_logits_kernel<Big<F16, NP, false, false>, F16, BWD>), grid, block, 0, st, p);
-  else if (tile == kMid)
-    hipLaunchKernelGGL((xent_logits_kernel<Mid<F16, NP, false, false>, F16, BWD>), grid, block, 0, st, p);
-  else
-    hipLaunchKernelGGL((xent_logits_kernel<Few<F16, NP, false, false>, F16, BWD>), grid, block, 0, st, p);
+  p.tj = (p.v1 - p.v0 + tile_bj(tile) - 1) / tile_bj(tile);
+  const dim3 grid(unsigned(tiles_of(tile, p.X.n, p.v1 - p.v0)));
+  auto go = [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    hipLaunchKernelGGL((xent_logits_kernel<T, F16, BWD, TWO>), grid, dim3(T::kThreads), 0, st, p);
+  };
+  // bf16 G in two planes comes with few rows only
+  constexpr bool large = F16 || !TWO;
+  if (tile == kFew) go(static_cast<Few<F16, NP, false, false>*>(nullptr));
+  else if (!large || tile == kSq) go(static_cast<Sq<F16, NP, false, false>*>(nullptr));
+  else if constexpr (large) {
+    if (tile == kBig) go(static_cast<Big<F16, NP, false, false>*>(nullptr));
+    else go(static_cast<Wide<F16, NP, false, false>*>(nullptr));
+  }
   check_launch();
 }
 
@@ -403,22 +429,32 @@ void launch_logits(LogitArgs& p, int tile, hipStream_t st) {
 namespace {
 
 struct XentPlan {
-  int kp, vpad, piece, tile, slots, gtile, dx_tile, dx_splits, dw_splits, planes;
+  int kp, vpad, piece, tile, slots, gtile, dx_tile, dw_tile, dw_splits;
+  bool two;               // G in two planes
+  Split dx_split, dw_split;
+  Extent dx;
   int64_t fwd_bytes, bwd_bytes;
   // offsets into the forward's workspace
-  int64_t o_amax, o_wp, o_part, o_zlab, o_tie, o_lsum, o_csum;
+  int64_t o_wp, o_part, o_zlab, o_tie, o_lsum, o_csum;
   // offsets into the backward's
-  int64_t b_amax, b_wp, b_g, b_dx, b_dw, b_db;
+  int64_t b_wp, b_g, b_dx, b_dw, b_db;
 };
 
-constexpr int64_t kGBytes = int64_t(256) << 20;  // G of one piece of the vocabulary
+constexpr int64_t kGBytes = int64_t(512) << 20;  // G of one piece of the vocabulary
+constexpr int kTwoRows = 128;
 
 XentPlan xent_plan(int rows, int width, int classes, bool f32) {
   XentPlan q{};
-  q.planes = f32 ? 2 : 1;
+  const int np = f32 ? 3 : 1;
+  // bf16: one rounding of G to bf16 is one more of the same size as the gradients' own, and over many
+  // rows their errors add up to 1.2 times that one's; with a few rows one element can make up a
+  // gradient, and the sum reaches twice.  There the products only stream the weights, and a second plane
+  // costs nothing.
+  q.two = f32 || rows <= kTwoRows;
   q.kp = int(up(width, 8));
   q.vpad = int(up(classes, 256));
-  q.tile = logits_tile(rows, classes);
+  auto tile = [&](int cols) { return rows > 32 && rows <= kTwoRows ? kSq : choose_tile(rows, cols, int64_t(width) * np, false); };
+  q.tile = tile(classes);
   q.slots = int(up(classes, tile_bj(q.tile)) / tile_slot(q.tile));
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -426,26 +462,34 @@ XentPlan xent_plan(int rows, int width, int classes, bool f32) {
     at = up(at + bytes, 256);
     return o;
   };
-  q.o_amax = take(f32 ? 2 * kAmaxBlocks * 4 : 0);
   q.o_wp = take(f32 ? int64_t(classes) * q.kp * 4 : 0);
   q.o_part = take(int64_t(q.slots) * rows * 8);
   q.o_zlab = take(int64_t(rows) * 4);
   q.o_tie = take(int64_t(rows) * 4);
-  const int64_t jb = (rows + 63) / 64;
+  const int64_t jb = (rows + 15) / 16;
   q.o_lsum = take(jb * 8);
   q.o_csum = take(jb * 4);
   q.fwd_bytes = at;
   at = 0;
   q.b_wp = take(f32 ? int64_t(classes) * q.kp * 4 : 0);
-  const int64_t row_bytes = int64_t(rows) * q.planes * 2;
-  q.piece = int(std::max<int64_t>(256, std::min<int64_t>(q.vpad, kGBytes / row_bytes / 256 * 256)));
-  q.gtile = logits_tile(rows, q.piece);
+  // pieces of equal width, so that none of them is a remainder that fills a few CUs
+  const int64_t row_bytes = int64_t(rows) * (q.two ? 4 : 2);
+  const int64_t most = std::max<int64_t>(256, kGBytes / row_bytes / 256 * 256);
+  const int64_t pieces = (q.vpad + most - 1) / most;
+  q.piece = int(up((q.vpad + pieces - 1) / pieces, 256));
+  q.gtile = tile(q.piece);
   q.b_g = take(row_bytes * q.piece);
-  q.dx_tile = rows <= 32 ? kFew : kBig;
-  q.dx_splits = splits_for(tiles_of(q.dx_tile, rows, width), q.piece, 256);
-  q.b_dx = take(int64_t(q.dx_splits) * rows * q.kp * 4);
-  const int64_t wt = tiles_of(kBig, std::min(q.piece, classes), width);
-  q.dw_splits = wt >= 256 ? 1 : splits_for(wt, rows, 512);
+  // dx: few tiles and a long reduction (the piece), so as large a tile as the rows fill: its slabs'
+  // traffic grows with the splits
+  q.dx_tile = rows <= 32 ? kFew : rows < 1024 ? kSq : kWide;
+  q.dx_split = {tile_slots(q.dx_tile), 256};
+  q.dx = extent_of(q.dx_tile, rows, width, q.dx_split, q.piece);
+  q.b_dx = take(q.dx.slab_rows * q.kp * 4);
+  const int64_t wi = std::min(q.piece, classes);
+  q.dw_tile = rows <= kTwoRows ? kSq : choose_tile(wi, width, int64_t(rows) * np, true);
+  q.dw_split = {tile_slots(q.dw_tile), 512};
+  q.dw_splits = q.dw_split.of(tiles_of(q.dw_tile, wi, width), rows);
+  q.dw_split.most = q.dw_splits;  // a narrower last piece has no room for more
   q.b_dw = take(q.dw_splits > 1 ? int64_t(q.dw_splits) * q.piece * q.kp * 4 : 0);
   q.b_db = take(q.dw_splits > 1 ? int64_t(q.dw_splits) * q.piece * 4 : 0);
   q.bwd_bytes = at;
@@ -536,12 +580,16 @@ void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
   p.part = reinterpret_cast<float2*>(base + q.o_part);
   p.zlab = reinterpret_cast<float*>(base + q.o_zlab);
   p.tie = reinterpret_cast<int*>(base + q.o_tie);
-  if (f32) launch_logits<true, false>(p, q.tile, st);
-  else launch_logits<false, false>(p, q.tile, st);
-  hipLaunchKernelGGL(xent_join_kernel, dim3(unsigned((rows + 63) / 64)), dim3(64 * kJoinWaves), 0, st, p.part, q.slots,
-                     int(rows), tile_slot(q.tile), p.zlab, p.tie, g.lab, d, reinterpret_cast<float2*>(stat),
-                     reinterpret_cast<double*>(base + q.o_lsum), reinterpret_cast<int*>(base + q.o_csum),
-                     reinterpret_cast<float*>(loss), reinterpret_cast<int64_t*>(correct));
+  if (f32) launch_logits<true, false, true>(p, q.tile, st);
+  else launch_logits<false, false, false>(p, q.tile, st);
+  auto join = [&](auto kernel, int per) {
+    hipLaunchKernelGGL(kernel, dim3(unsigned((rows + per - 1) / per)), dim3(64 * kJoinWaves), 0, st, p.part, q.slots, int(rows),
+                       tile_slot(q.tile), p.zlab, p.tie, g.lab, d, reinterpret_cast<float2*>(stat),
+                       reinterpret_cast<double*>(base + q.o_lsum), reinterpret_cast<int*>(base + q.o_csum),
+                       reinterpret_cast<float*>(loss), reinterpret_cast<int64_t*>(correct));
+  };
+  if (rows <= 1024) join(xent_join_kernel<16>, 16);
+  else join(xent_join_kernel<64>, 64);
   check_launch();
 }
 
@@ -585,34 +633,37 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
   e.f = f32 ? 1.f / kGScale : 1.f;
   e.gl = gl;
   e.gn = &d->n;
-  e.zero_from = 0x7fffffff;
   const int gsz = grad_dt == kF32 ? 4 : 2;
+  GemmArgs x{};
+  x.I = {p.G, q.piece, p.gplane, int(rows)};
+  x.ni_dev = &d->n;
+  x.split = q.dx_split;
+  x.nk_split = q.piece;
+  x.slab = reinterpret_cast<float*>(base + q.b_dx);
+  x.lds = q.kp;
+  x.e = e;
+  x.e.fj = f32 ? &d->inv_w : nullptr;
+  x.e.out = reinterpret_cast<void*>(dx);
+  x.e.ldo = width;
+  x.e.bf16 = !f32;
+  x.e.nj = int(width);
+  x.e.vec = whole_rows(dx, width, !f32);
   for (int v0 = 0; v0 < q.vpad; v0 += q.piece) {
     const int v1 = int(std::min<int64_t>(classes, v0 + q.piece));
     if (v1 <= v0) break;
     p.v0 = v0;
     p.v1 = v1;
-    if (f32) launch_logits<true, true>(p, q.gtile, st);
-    else launch_logits<false, true>(p, q.gtile, st);
+    if (f32) launch_logits<true, true, true>(p, q.gtile, st);
+    else if (q.two) launch_logits<false, true, true>(p, q.gtile, st);
+    else launch_logits<false, true, false>(p, q.gtile, st);
     if (dx) {
-      GemmArgs a{};
-      a.I = {p.G, q.piece, p.gplane, int(rows)};
-      a.J = {p.W.p + int64_t(v0) * p.W.ld, p.W.ld, p.W.plane, int(up(width, 8))};
-      a.ni_dev = &d->n;
-      a.nk = v1 - v0;
-      a.o.gi = 8;
-      a.o.splits = q.dx_splits;
-      a.slab = reinterpret_cast<float*>(base + q.b_dx);
-      a.lds = q.kp;
-      a.add = v0 > 0;
-      a.e.nj = int(width);
-      if (q.dx_tile == kFew) {
-        if (f32) gemm<Few<true, 3, false, true>, false>(a, st);
-        else gemm<Few<false, 1, false, true>, false>(a, st);
-      } else {
-        if (f32) gemm<Big<true, 3, false, true>, false>(a, st);
-        else gemm<Big<false, 1, false, true>, false>(a, st);
-      }
+      x.J = {p.W.p + int64_t(v0) * p.W.ld, p.W.ld, p.W.plane, int(up(width, 8))};
+      x.nk = v1 - v0;
+      x.add = v0 > 0;
+      if (f32) gemm<true, 3, false, true, false>(q.dx_tile, x, q.dx.grid, st);
+      else if (!q.two) gemm<false, 1, false, true, false>(q.dx_tile, x, q.dx.grid, st);
+      else if (q.dx_tile == kFew) launch_gemm<Few<false, 2, false, true>, false>(x, q.dx.grid, st);
+      else launch_gemm<Sq<false, 2, false, true>, false>(x, q.dx.grid, st);
     }
     if (dw) {
       GemmArgs a{};
@@ -620,57 +671,29 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
       a.J = {p.X.p, p.X.ld, p.X.plane, int(up(width, 8))};
       a.nk_dev = &d->n;
       a.nk = int(rows);
-      a.o.gi = 8;
-      a.o.splits = q.dw_splits;
+      a.split = q.dw_split;
       a.e = e;
       a.e.fj = f32 ? &d->inv_x : nullptr;
       a.e.out = reinterpret_cast<void*>(dw + uintptr_t(int64_t(v0) * ldd * gsz));
       a.e.ldo = ldd;
       a.e.bf16 = grad_dt == kBF16;
       a.e.nj = int(width);
-      a.e.vec = ldd % 4 == 0 && dw % (4 * gsz) == 0;
+      a.e.vec = whole_rows(dw, ldd, a.e.bf16);
       a.e.accumulate = accumulate;
-      void* dbp = db ? reinterpret_cast<void*>(db + uintptr_t(v0) * gsz) : nullptr;
+      a.bout = db ? reinterpret_cast<void*>(db + uintptr_t(v0) * gsz) : nullptr;
       if (q.dw_splits > 1) {
         a.slab = reinterpret_cast<float*>(base + q.b_dw);
         a.lds = q.kp;
         a.bslab = db ? reinterpret_cast<float*>(base + q.b_db) : nullptr;
-      } else {
-        a.bout = dbp;
       }
-      if (f32) gemm<Big<true, 3, true, true>, true>(a, st);
-      else gemm<Big<false, 1, true, true>, true>(a, st);
-      if (q.dw_splits > 1) {
-        FinishArgs f{};
-        f.slab = a.slab;
-        f.lds = a.lds;
-        f.splits = q.dw_splits;
-        f.slab_rows = a.I.n;
-        f.rows = a.I.n;
-        f.bslab = a.bslab;
-        f.bout = dbp;
-        f.e = a.e;
-        finish(f, st);
-      }
+      const int64_t grid = tiles_of(q.dw_tile, v1 - v0, width) * q.dw_splits;
+      if (f32) gemm<true, 3, true, true, true>(q.dw_tile, a, grid, st);
+      else if (q.two) launch_gemm<Sq<false, 2, true, true>, true>(a, grid, st);
+      else gemm<false, 1, true, true, true>(q.dw_tile, a, grid, st);
+      if (a.slab) finish(q.dw_tile, a, a.I.n, nullptr, st);
     }
   }
-  if (dx) {
-    FinishArgs f{};
-    f.slab = reinterpret_cast<const float*>(base + q.b_dx);
-    f.lds = q.kp;
-    f.splits = q.dx_splits;
-    f.slab_rows = int(rows);
-    f.rows = int(rows);
-    f.inv = reinterpret_cast<const int*>(inv);
-    f.e = e;
-    f.e.fj = f32 ? &d->inv_w : nullptr;
-    f.e.out = reinterpret_cast<void*>(dx);
-    f.e.ldo = width;
-    f.e.bf16 = !f32;
-    f.e.nj = int(width);
-    f.e.vec = width % 4 == 0 && dx % 16 == 0;
-    finish(f, st);
-  }
+  if (dx) finish(q.dx_tile, x, int(rows), reinterpret_cast<const int*>(inv), st);
 }
 
 }  // namespace voda

@@ -128,7 +128,7 @@ class _LinearAct8Fn(torch.autograd.Function):
             y = torch.empty(rows, out, dtype=x.dtype, device=dev)
             q = torch.empty(rows, kq, dtype=_F8, device=dev) if keep else None
             s = torch.empty(rows, kq // BLOCK, dtype=_E8, device=dev) if keep else None
-            amax = torch.empty(512, dtype=torch.float32, device=dev) if f32 else None
+            amax = torch.empty(2048, dtype=torch.float32, device=dev) if f32 else None
             h.linear_act8_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), N.ptr(bias),
                               N.DT_F32 if bias is None else N.dtype_code(bias.dtype), y.data_ptr(), N.ptr(q),
                               N.ptr(s), rows, K, out, dt, gelu, copy, N.ptr(amax), ws.data_ptr(), N.stream_of(x))

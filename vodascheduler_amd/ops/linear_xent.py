@@ -81,7 +81,7 @@ class _LinearXentFn(torch.autograd.Function):
             ws = torch.empty(max(nf, 256), dtype=torch.uint8, device=dev)
             xc = torch.empty((2 if f32 else 1) * rows * kp, dtype=torch.int16, device=dev)
             # what the backward needs besides: each part 256-byte aligned
-            parts = [4 * vpad, 4 * rows, 4 * rows, 8 * rows, nd, 4 * 512 if f32 else 0]
+            parts = [4 * vpad, 4 * rows, 4 * rows, 8 * rows, nd, 4 * 2048 if f32 else 0]
             at = [0]
             for n in parts:
                 at.append(at[-1] + _up(n))
@@ -99,11 +99,14 @@ class _LinearXentFn(torch.autograd.Function):
         ctx.params = (weight, bias)
         ctx.x_dtype = x.dtype
         ctx.mark_non_differentiable(correct, n)
+        ctx.set_materialize_grads(False)  # no zero gradients for the two counts
         return loss, correct, n
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gloss, _gc, _gn):
+        if gloss is None:
+            return None, None, None, None, None, None
         weight, xc, keep = ctx.saved_tensors
         rows, K, C, V = ctx.dims
         wp, bp = ctx.params
