@@ -379,20 +379,29 @@ struct Emit {
   const float* gl;
   const int* gn;
 
-  // ``with_j`` false: of a sum over I alone
-  __device__ __forceinline__ float scaled(float v, bool with_j = true) const {
-    // one after the other: a product of two factors may leave fp32's range where the result does not
-    v *= f;
-    if (fi) v *= *fi;
-    if (fj && with_j) v *= *fj;
-    if (gl) v *= *gl / float(max(*gn, 1));
-    return v;
+  // what a kernel reads once: the factors (one after the other: a product of two may leave fp32's range
+  // where the result does not) and the bias of a lane's eight columns
+  struct Once {
+    float a, b, c;
+    float bias[8];
+  };
+  __device__ __forceinline__ Once once(int j) const {
+    Once o;
+    o.a = gl ? f * (*gl / float(max(*gn, 1))) : f;
+    o.b = fi ? *fi : 1.f;
+    o.c = fj ? *fj : 1.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      o.bias[e] = !bias || j + e >= nj ? 0.f
+                  : bias_bf16          ? bf2f(static_cast<const uint16_t*>(bias)[j + e])
+                                       : static_cast<const float*>(bias)[j + e];
+    return o;
   }
   // columns j .. j+7 of row i (j % 8 == 0); ``keep`` false: the row is zero whatever the factors are
-  __device__ __forceinline__ void eight(int i, int j, float (&v)[8], bool keep = true) const {
+  __device__ __forceinline__ void eight(const Once& o, int i, int j, float (&v)[8], bool keep = true) const {
     if (j >= nj) return;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = keep ? scaled(v[e]) : 0.f;
+    for (int e = 0; e < 8; ++e) v[e] = keep ? v[e] * o.a * o.b * o.c : 0.f;
     if (q) {  // ldq % 32 == 0
       const uint2 u = *reinterpret_cast<const uint2*>(q + int64_t(i) * ldq + j);
       const float s = __uint_as_float(uint32_t(qs[int64_t(i) * (ldq >> 5) + (j >> 5)]) << 23);
@@ -407,9 +416,7 @@ struct Emit {
     }
     if (bias) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (j + e < nj)
-          v[e] += bias_bf16 ? bf2f(static_cast<const uint16_t*>(bias)[j + e]) : static_cast<const float*>(bias)[j + e];
+      for (int e = 0; e < 8; ++e) v[e] += o.bias[e];
     }
     put(i, j, v);
   }
@@ -512,8 +519,9 @@ __device__ __forceinline__ void split_range(int nk, int splits, int s, int bk, i
   k1 = min(nk, k0 + per * bk);
 }
 
-__device__ __forceinline__ void emit_sum(const Emit& e, void* out, int i, float v) {
-  v = e.scaled(v, false);
+// a sum over I alone: without J's factor
+__device__ __forceinline__ void emit_sum(const Emit& e, const Emit::Once& o, void* out, int i, float v) {
+  v = v * o.a * o.b;
   if (e.bf16) {
     uint16_t* o = static_cast<uint16_t*>(out) + i;
     *o = f2bf(v + (e.accumulate ? bf2f(*o) : 0.f));
@@ -540,6 +548,8 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm_kernel(GemmArgs p) {
   f32x16 acc[T::TJ][T::TI];
   float isum[T::TI];
   T::template run<SUM>(smem, I, p.J, i0, j0, k0, k1, acc, isum, want);
+  // through_lds gives a lane the same columns each time
+  const Emit::Once once = p.e.once(j0 + w.wj * T::TJ * 32 + 8 * (w.lane % (4 * T::TJ)));
   Emit o = p.e;
   if (p.slab) {
     o.out = p.slab + int64_t(s) * I.n * p.lds;
@@ -556,14 +566,14 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm_kernel(GemmArgs p) {
         const float tot = isum[b] + __shfl_xor(isum[b], 32, 64);
         if (w.h == 0 && i < I.n) {
           if (p.bslab) p.bslab[int64_t(s) * p.I.n + i] = tot;
-          else emit_sum(p.e, p.bout, i, tot);
+          else emit_sum(p.e, once, p.bout, i, tot);
         }
       }
     }
     through_lds<T>(smem, w, acc, b, [&](int r, int c, float(&v)[8]) {
       if (i0 + r >= I.n) return;
       if (p.slab) o.put(i0 + r, j0 + c, v);
-      else o.eight(i0 + r, j0 + c, v);
+      else o.eight(once, i0 + r, j0 + c, v);
     });
   }
 }
@@ -604,12 +614,12 @@ static __global__ __launch_bounds__(256) void finish_kernel(FinishArgs p) {
     for (int o = 1; o < LANES; o <<= 1)
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += __shfl_xor(v[e], o, 64);
-    if (part == 0) p.g.e.eight(i, j, v, src >= 0);
+    if (part == 0) p.g.e.eight(p.g.e.once(j), i, j, v, src >= 0);
   } else if (p.g.bslab && t - n < p.rows && part == 0) {
     const int i = int(t - n);
     float v = 0.f;
     for (int s = 0; s < splits; ++s) v += p.g.bslab[int64_t(s) * p.g.I.n + i];
-    emit_sum(p.g.e, p.g.bout, i, v);
+    emit_sum(p.g.e, p.g.e.once(p.g.e.nj), p.g.bout, i, v);
   }
 }
 
