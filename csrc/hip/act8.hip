@@ -6,8 +6,8 @@
 //
 // Checkpoint: blocks of 32 features of one row, each e4m3 times the smallest power of two 2^e,
 // e >= -126, with the block's largest finite |x| <= 448 2^e.  The scaling is exact, so the one rounding
-// is e4m3's (at most 2^-4 of the value, or 2^(e-10) for the smallest), and nothing saturates.  Infinite
-// and NaN elements are held as NaN.  33 bytes for 32 features against 64 (bf16) or 128 (fp32).
+// is e4m3's (at most 2^-4 of the value, or 2^(e-10) for the smallest); only what would round past fp32's
+// own range stays at 240 2^120, within 2^-4 too.  Infinite and NaN elements are held as NaN.  33 bytes for 32 features against 64 (bf16) or 128 (fp32).
 //
 //  * act8_pack reads x once and writes the checkpoint and, where the product cannot take x as it is,
 //    act(x) as the product's operand (bf16, or the two fp16 planes of fp32).  It moves 8 features a
@@ -116,9 +116,10 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(PackArgs p) {
   const uint32_t bits = __float_as_uint(m);
   const int ex = max(int(bits >> 23) - 127 - 8 + int((bits & 0x7fffff) > 0x600000), -126);
   const float inv = __uint_as_float(uint32_t(127 - ex) << 23);
+  const float most = ex == 120 ? 240.f : 448.f;  // 256 2^120 is past fp32
   float w[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = finite(v[e]) ? v[e] * inv : NAN;
+  for (int e = 0; e < 8; ++e) w[e] = finite(v[e]) ? fminf(fmaxf(v[e] * inv, -most), most) : NAN;
   uint32_t q0 = 0, q1 = 0;
   q0 = __builtin_amdgcn_cvt_pk_fp8_f32(w[0], w[1], q0, false);
   q0 = __builtin_amdgcn_cvt_pk_fp8_f32(w[2], w[3], q0, true);

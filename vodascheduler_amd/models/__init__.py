@@ -105,6 +105,15 @@ def _nmt_loss(model, batch):
     return _nmt_metrics(model, batch)[0]
 
 
+def _nmt_lean_metrics(model, batch):
+    src, tin, tout = batch
+    return model.head_metrics(src, tin, tout, ignore_index=0)
+
+
+def _bert_lean_metrics(model, batch):
+    return model.head_metrics(*batch)
+
+
 def _bert_batch(b, dev, g=None, vocab=30522, T=128, P=20):
     """BERT pretraining batch in the reference input format: input ids, attention mask,
     ``masked_lm_positions`` [B, P] and ``masked_lm_ids`` [B, P] (P = max_predictions_per_seq
@@ -149,6 +158,15 @@ WORKLOADS: dict[str, Workload] = {
                           # column-sum / index_add path (check 31: frozen grads bitwise, 5-step
                           # trajectory equal); 11.0-11.28 -> 10.75 ms per step as a graph
                           graph_safe=True),
+    # the same two steps with less kept for the backward: the head's loss without its logits, and in
+    # BERT's layers 8-bit checkpoints of the projections' inputs
+    "transformer-lean": Workload("transformer-lean", TransformerNMT, _nmt_batch,
+                                 lambda m, b: _nmt_lean_metrics(m, b)[0], 512, "rmsprop", dict(lr=1e-3),
+                                 samples_unit="tok", tokens_per_sample=20, metrics=_nmt_lean_metrics),
+    "bert-base-lean": Workload("bert-base-lean", lambda: BertBase(act8=True), _bert_batch,
+                               lambda m, b: _bert_lean_metrics(m, b)[0], 64, "adamw",
+                               dict(lr=1e-4, weight_decay=0.01), samples_unit="tok", tokens_per_sample=128,
+                               metrics=_bert_lean_metrics),
 }
 
 

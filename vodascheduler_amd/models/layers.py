@@ -17,6 +17,7 @@ import torch
 from torch import nn
 
 from ..ops import ffn as _ffn
+from ..ops.act8 import Act8Linear
 from ..ops.activation import GeluTanh
 from ..ops.attention import attention_q_kvpacked, attention_qkvpacked
 from ..ops.conv1x1 import USE_GRAD_SINK, GradSink
@@ -35,7 +36,7 @@ BIAS_HANDOFF = True
 
 class MultiHeadAttention(nn.Module):
     def __init__(self, d_model: int, num_heads: int, key_dim: int | None = None, dropout: float = 0.0,
-                 bias: bool = True, cross: bool = False):
+                 bias: bool = True, cross: bool = False, act8: bool = False):
         super().__init__()
         self.h = num_heads
         self.dk = key_dim or d_model // num_heads
@@ -53,7 +54,9 @@ class MultiHeadAttention(nn.Module):
             self.q = FusedLinear(d_model, inner, bias=bias)
             self.kv = FusedLinear(d_model, 2 * inner, bias=bias)
         else:
-            self.qkv = FusedLinear(d_model, 3 * inner, bias=bias)
+            # act8: the projection keeps its input in 8 bits.  The output projection does not: its input
+            # is the attention's output, which the attention's backward keeps anyway
+            self.qkv = (Act8Linear if act8 else FusedLinear)(d_model, 3 * inner, bias=bias)
         self.o = FusedLinear(inner, d_model, bias=bias)
         self.inner = inner
         self.dropout = dropout
@@ -81,8 +84,17 @@ class MultiHeadAttention(nn.Module):
 
 
 class FeedForward(nn.Module):
-    def __init__(self, d_model: int, d_ff: int, act: str = "relu"):
+    def __init__(self, d_model: int, d_ff: int, act: str = "relu", act8: bool = False):
+        """``act8`` (GELU only): both layers keep their inputs in 8 bits, the second the GELU's input
+        (ops/act8.py); same parameters."""
         super().__init__()
+        self.act8 = act8
+        if act8:
+            if act != "gelu":
+                raise ValueError(f"FeedForward(act8=True) needs act='gelu', got {act!r}")
+            self.fc1 = Act8Linear(d_model, d_ff)
+            self.fc2 = Act8Linear(d_ff, d_model, act="gelu")
+            return
         self.fc1 = FusedLinear(d_model, d_ff)
         self.fc2 = FusedLinear(d_ff, d_model)
         if act == "gelu":
@@ -91,6 +103,8 @@ class FeedForward(nn.Module):
             self.act = nn.ReLU()
 
     def forward(self, x, sink_in=None, bias_handoff=None):
+        if self.act8:
+            return self.fc2(self.fc1(x, sink_in), bias_handoff=bias_handoff)
         if isinstance(self.act, GeluTanh) and x.is_cuda:
             if x.dtype != self.fc1.weight.dtype and torch.is_autocast_enabled("cuda"):
                 x = x.to(self.fc1.weight.dtype)
@@ -118,11 +132,11 @@ def _sink(module: nn.Module, x: torch.Tensor) -> GradSink | None:
 class EncoderLayer(nn.Module):
     """Post-LN encoder block (Keras TransformerEncoder / BERT layout)."""
 
-    def __init__(self, d_model, heads, d_ff, key_dim=None, act="relu", dropout=0.0, eps=1e-5):
+    def __init__(self, d_model, heads, d_ff, key_dim=None, act="relu", dropout=0.0, eps=1e-5, act8=False):
         super().__init__()
-        self.attn = MultiHeadAttention(d_model, heads, key_dim, dropout)
+        self.attn = MultiHeadAttention(d_model, heads, key_dim, dropout, act8=act8)
         self.ln1 = FusedLayerNorm(d_model, eps=eps)
-        self.ff = FeedForward(d_model, d_ff, act)
+        self.ff = FeedForward(d_model, d_ff, act, act8=act8)
         self.ln2 = FusedLayerNorm(d_model, eps=eps)
         self.drop = nn.Dropout(dropout)
 

@@ -37,12 +37,15 @@ _F8, _E8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 def _pack_ref(x2: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     rows, width = x2.shape
-    v = F.pad(x2.float(), (0, -width % BLOCK)).view(rows, -1, BLOCK)
+    kq = -(-width // BLOCK) * BLOCK
+    v = F.pad(x2.float(), (0, kq - width)).view(rows, kq // BLOCK, BLOCK)
     fin = torch.isfinite(v)
     mant, exp = torch.frexp(torch.where(fin, v, 0).abs().amax(2, keepdim=True))  # [0.5, 1) 2^exp
     exp = torch.where(mant > 0, exp - 9 + (mant > E4M3_MAX / 512), -126).clamp(min=-126)
-    q = torch.where(fin, torch.ldexp(v, -exp), torch.nan).to(_F8).view(rows, -1)
-    return q, (exp.view(rows, -1) + 127).to(torch.uint8).view(_E8)
+    most = torch.where(exp == 120, 240.0, E4M3_MAX)  # 256 2^120 is past fp32
+    v = torch.minimum(torch.maximum(torch.ldexp(v, -exp), -most), most)
+    q = torch.where(fin, v, torch.nan).to(_F8).view(rows, kq)
+    return q, (exp.view(rows, kq // BLOCK) + 127).to(torch.uint8).view(_E8)
 
 
 def _unpack_ref(q: torch.Tensor, scale: torch.Tensor, width: int, dtype: torch.dtype) -> torch.Tensor:
