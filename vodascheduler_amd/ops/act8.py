@@ -28,7 +28,7 @@ from ..utils.flat import flat_grad
 from . import _native as N
 from .dense import FusedLinear, _direct, _ready
 from .ffn import gelu_tanh_grad_ref
-from .linear_xent import _rows16
+from .linear_xent import _on, _rows16
 
 BLOCK = 32
 E4M3_MAX = 448.0
@@ -68,7 +68,7 @@ def act8_pack(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     else:
         if x2.stride(1) != 1:
             x2 = x2.contiguous()
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             q = torch.empty(rows, kq, dtype=_F8, device=x.device)
             s = torch.empty(rows, kq // BLOCK, dtype=_E8, device=x.device)
             N.hip().act8_pack(x2.data_ptr(), x2.stride(0), rows, width, N.dtype_code(x.dtype), q.data_ptr(),
@@ -90,7 +90,7 @@ def act8_unpack(q: torch.Tensor, scale: torch.Tensor, width: int, dtype: torch.d
     q, scale = q.contiguous(), scale.contiguous()
     if q.data_ptr() % 16:
         q = q.clone()
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         out = torch.empty(*q.shape[:-1], width, dtype=dtype, device=q.device)
         N.hip().act8_values(q.data_ptr(), scale.data_ptr(), rows, width, N.dtype_code(dtype), out.data_ptr(),
                             N.stream_of(q))
@@ -121,7 +121,7 @@ class _LinearAct8Fn(torch.autograd.Function):
             ctx.save_for_backward(weight, q, s, None)
             return y
         h = N.hip()
-        with torch.cuda.device(dev):
+        with _on(dev):
             dt = N.dtype_code(x.dtype)
             # bf16 rows of whole aligned vectors go into the product as they are
             copy = bool(f32 or gelu or x.data_ptr() % 16 or x.stride(0) % 8 or K % 8)
@@ -176,7 +176,7 @@ class _LinearAct8Fn(torch.autograd.Function):
         dev = dy.device
         f32 = dt == torch.float32
         h = N.hip()
-        with torch.cuda.device(dev):
+        with _on(dev):
             if not f32:
                 dy = _rows16(dy)
             _, nb, _, _ = h.linear_act8_sizes(rows, K, out, N.dtype_code(dt), True)
@@ -220,18 +220,19 @@ def linear_act8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
         raise ValueError(f"linear_act8: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not multiply")
     if bias is not None and tuple(bias.shape) != (weight.shape[0],):
         raise ValueError(f"linear_act8: bias {tuple(bias.shape)} for weight {tuple(weight.shape)}")
-    if torch.is_autocast_enabled(x.device.type) and x.dtype != weight.dtype:
+    if x.dtype != weight.dtype and torch.is_autocast_enabled(x.device.type):
         x = x.to(weight.dtype)
     _check_float("linear_act8", x)
     if weight.dtype != x.dtype:
         raise TypeError(f"linear_act8: x and weight must both be fp32 or bf16, got {x.dtype}, {weight.dtype}")
     if bias is not None and bias.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"linear_act8: bias must be fp32 or bf16, got {bias.dtype}")
+    dev = x.device
     for t, nm in ((weight, "weight"), (bias, "bias")):
-        if t is not None and t.device != x.device:
+        if t is not None and t.device != dev:
             raise ValueError(f"linear_act8: {nm} on {t.device}, x on {x.device}")
-    lead = x.shape[:-1]
-    x2 = x.reshape(-1, x.shape[-1])
+    # (a reshape that changes nothing would still be a node of the backward)
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if x2.shape[0] == 0:
         return F.linear(F.gelu(x, approximate="tanh") if act else x, weight, None if bias is None else bias.to(x.dtype))
     if x2.stride(1) != 1:
@@ -241,7 +242,7 @@ def linear_act8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
     y = _LinearAct8Fn.apply(x2, weight, bias, act == "gelu", sink_in, bias_handoff)
-    return y.view(*lead, weight.shape[0])
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])
 
 
 class Act8Linear(FusedLinear):

@@ -28,6 +28,8 @@ The reference's head is a Dense layer with a softmax over the vocabulary and a s
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
+
 import torch
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
@@ -63,8 +65,9 @@ def _rows16(w: torch.Tensor) -> torch.Tensor:
     return F.pad(w, (0, -w.shape[1] % 8)).contiguous()
 
 
-def _up(v: int, m: int = 256) -> int:
-    return -(-v // m) * m
+def _on(device: torch.device):
+    """Context with ``device`` current (nothing to do where it is already)."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 class _LinearXentFn(torch.autograd.Function):
@@ -75,26 +78,26 @@ class _LinearXentFn(torch.autograd.Function):
         V = weight.shape[0]
         f32 = x.dtype == torch.float32
         dev = x.device
-        with torch.cuda.device(dev):
+        with _on(dev):
             nf, nb, kp, vpad, nd = h.linear_xent_sizes(rows, K, C, V, f32)
             w = weight if f32 else _rows16(weight)
             ws = torch.empty(max(nf, 256), dtype=torch.uint8, device=dev)
-            xc = torch.empty((2 if f32 else 1) * rows * kp, dtype=torch.int16, device=dev)
-            # what the backward needs besides: each part 256-byte aligned
-            parts = [4 * vpad, 4 * rows, 4 * rows, 8 * rows, nd, 4 * 2048 if f32 else 0]
+            # what the backward needs, in one buffer, each part 256-byte aligned: x's compact rows, the
+            # padded bias, each row's place, the labels, (max, 1 / sum), the device scalars, w's maxima
             at = [0]
-            for n in parts:
-                at.append(at[-1] + _up(n))
+            for n in ((4 if f32 else 2) * rows * kp, 4 * vpad, 4 * rows, 4 * rows, 8 * rows, nd, 8192 if f32 else 0):
+                at.append(at[-1] + -(-n // 256) * 256)
             keep = torch.empty(at[-1], dtype=torch.uint8, device=dev)
-            p = [keep.data_ptr() + a for a in at]
+            p = keep.data_ptr()
+            p = [p + a for a in at]
             loss = torch.empty((), dtype=torch.float32, device=dev)
             correct = torch.empty((), dtype=torch.int64, device=dev)
             n = torch.empty((), dtype=torch.int64, device=dev)
             h.linear_xent_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), N.ptr(bias),
                               N.DT_F32 if bias is None else N.dtype_code(bias.dtype), labels.data_ptr(), ignore, rows,
-                              K, C, V, N.dtype_code(x.dtype), ws.data_ptr(), xc.data_ptr(), p[0], p[1], p[2], p[3],
-                              p[4], p[5], loss.data_ptr(), correct.data_ptr(), n.data_ptr(), N.stream_of(x))
-        ctx.save_for_backward(weight, xc, keep)
+                              K, C, V, N.dtype_code(x.dtype), ws.data_ptr(), p[0], p[1], p[2], p[3], p[4], p[5],
+                              p[6], loss.data_ptr(), correct.data_ptr(), n.data_ptr(), N.stream_of(x))
+        ctx.save_for_backward(weight, keep)
         ctx.at, ctx.dims, ctx.nb = at, (rows, K, C, V), nb
         ctx.params = (weight, bias)
         ctx.x_dtype = x.dtype
@@ -107,16 +110,17 @@ class _LinearXentFn(torch.autograd.Function):
     def backward(ctx, gloss, _gc, _gn):
         if gloss is None:
             return None, None, None, None, None, None
-        weight, xc, keep = ctx.saved_tensors
+        weight, keep = ctx.saved_tensors
         rows, K, C, V = ctx.dims
         wp, bp = ctx.params
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dev = weight.device
         f32 = ctx.x_dtype == torch.float32
         dx = dw = db = None
-        with torch.cuda.device(dev):
-            p = [keep.data_ptr() + a for a in ctx.at]
-            g = gloss.detach().to(torch.float32)
+        with _on(dev):
+            p = keep.data_ptr()
+            p = [p + a for a in ctx.at]
+            g = gloss  # fp32, as the loss is
             w = weight if f32 else _rows16(weight)
             if need_x:
                 dx = torch.empty(rows, K, dtype=ctx.x_dtype, device=dev)
@@ -143,7 +147,7 @@ class _LinearXentFn(torch.autograd.Function):
             if direct and not need_w:
                 dw.zero_()
             N.hip().linear_xent_bwd(w.data_ptr(), w.stride(0), rows, K, C, V, N.dtype_code(ctx.x_dtype), ws.data_ptr(),
-                                    xc.data_ptr(), p[0], p[1], p[2], p[3], p[4], p[5], g.data_ptr(), N.ptr(dx),
+                                    p[0], p[1], p[2], p[3], p[4], p[5], p[6], g.data_ptr(), N.ptr(dx),
                                     N.ptr(dw), dw.stride(0) if dw is not None else K, N.ptr(db), N.dtype_code(gdt),
                                     bool(direct), N.stream_of(weight))
         if direct:
@@ -170,8 +174,9 @@ def _check(x, weight, labels, bias, C) -> None:
         raise ValueError(f"linear_cross_entropy: bias {tuple(bias.shape)} for weight {tuple(weight.shape)}")
     if x.shape[-1] < 1 or not 1 <= C <= weight.shape[0]:
         raise ValueError(f"linear_cross_entropy: {C} classes of weight {tuple(weight.shape)}")
+    dev = x.device
     for t, nm in ((weight, "weight"), (labels, "labels"), (bias, "bias")):
-        if t is not None and t.device != x.device:
+        if t is not None and t.device != dev:
             raise ValueError(f"linear_cross_entropy: {nm} on {t.device}, x on {x.device}")
 
 
@@ -182,9 +187,12 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     ``num_classes`` classes against integer ``labels`` (one a row of x); see the module docstring."""
     C = weight.shape[0] if num_classes is None else int(num_classes)
     _check(x, weight, labels, bias, C)
-    if torch.is_autocast_enabled(x.device.type) and x.dtype != weight.dtype:
+    if x.dtype != weight.dtype and torch.is_autocast_enabled(x.device.type):
         x = x.to(weight.dtype)
-    x2, labels = x.reshape(-1, x.shape[-1]), labels.reshape(-1)
+    # (a reshape that changes nothing would still be a node of the backward)
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if labels.dim() != 1:
+        labels = labels.reshape(-1)
     if not x.is_cuda:
         return linear_cross_entropy_ref(x2, weight, labels, bias, C, ignore_index)
     if x.dtype not in (torch.float32, torch.bfloat16) or weight.dtype != x.dtype:
@@ -200,5 +208,6 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Te
         weight = weight.contiguous()
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    labels = labels.to(torch.int64).contiguous()
+    if labels.dtype != torch.int64 or not labels.is_contiguous():
+        labels = labels.to(torch.int64).contiguous()
     return _LinearXentFn.apply(x2, weight, bias, labels, C, int(ignore_index))
