@@ -222,12 +222,12 @@ Act8Plan act8_plan(int64_t rows, int64_t width, int64_t out, bool f32, bool copy
   q.np8 = int(up(out, 8));
   q.copy = copy;
   const int np = f32 ? 3 : 1;
-  q.y_tile = choose_tile(rows, out, width * np, false);
-  q.dx_tile = choose_tile(rows, width, out * np, false);
-  q.dw_tile = choose_tile(out, width, rows * np, true);
-  q.y_split = {tile_slots(q.y_tile), 256};
-  q.dx_split = {tile_slots(q.dx_tile), 256};
-  q.dw_split = {tile_slots(q.dw_tile), 256};
+  q.y_tile = choose_tile(rows, out, width, np, false, true);
+  q.dx_tile = choose_tile(rows, width, out, np, false, true);
+  q.dw_tile = choose_tile(out, width, rows, np, true, true);
+  q.y_split = split_of(q.y_tile);
+  q.dx_split = split_of(q.dx_tile);
+  q.dw_split = split_of(q.dw_tile);
   q.y_s = q.y_split.of(tiles_of(q.y_tile, rows, out), q.kp);
   q.dx_s = q.dx_split.of(tiles_of(q.dx_tile, rows, width), out);
   q.dw_s = q.dw_split.of(tiles_of(q.dw_tile, out, width), rows);

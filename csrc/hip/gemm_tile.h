@@ -748,29 +748,39 @@ inline int whole_rows(uintptr_t p, int64_t ld, bool bf16) { return p % 16 == 0 &
 //   kWide 256 x 256, one workgroup of 8 waves a CU;
 //   kBig  256 x 128, two workgroups a CU: one's epilogue runs beside the other's products;
 //   kSq   128 x 128, two a CU;
+//   kDeep 128 x 128, one a CU on a ring twice as deep, where there are not two: nothing else hides the
+//         loads' latency (2 us a stage) then.  [1001 x 331] . [331 x 1348] in fp32 36 -> 20 us, but
+//         [8192 x 2304]^T . [8192 x 768] in bf16, which splits into two a CU, 50 -> 64;
 //   kFew  128 x 32 (row operands), for a handful of rows, whose products only stream the weights.
 template <bool F16, int NP, bool IT, bool JT> using Wide = Tile<F16, NP, IT, JT, 2, 4, 4, 2, 64, 2>;
 template <bool F16, int NP, bool IT, bool JT> using Big = Tile<F16, NP, IT, JT, 2, 2, 4, 2, 32, 3>;
 template <bool F16, int NP, bool IT, bool JT> using Sq = Tile<F16, NP, IT, JT, 2, 2, 2, 2, 64, 2>;
+template <bool F16, int NP, bool IT, bool JT> using Deep = Tile<F16, NP, IT, JT, 2, 2, 2, 2, 64, 4>;
 template <bool F16, int NP, bool IT, bool JT> using Few = Tile<F16, NP, IT, JT, 4, 1, 1, 1, 64, 3>;
 
-enum { kWide = 0, kBig = 1, kSq = 2, kFew = 3 };
+enum { kWide = 0, kBig = 1, kSq = 2, kDeep = 3, kFew = 4 };
 inline int tile_bj(int t) { return t <= kBig ? 256 : 128; }
 inline int tile_bi(int t) { return t == kWide ? 256 : t == kFew ? 32 : 128; }
-inline int tile_slots(int t) { return t == kWide ? 256 : 512; }  // workgroups that the chip holds
+inline int tile_slots(int t) { return t == kWide || t == kDeep ? 256 : 512; }  // workgroups that the chip holds
 
 inline int64_t tiles_of(int tile, int64_t ni, int64_t nj) {
   return ((ni + tile_bi(tile) - 1) / tile_bi(tile)) * ((nj + tile_bj(tile) - 1) / tile_bj(tile));
 }
 
-// ``steps``: reduction length times products.
-inline int choose_tile(int64_t ni, int64_t nj, int64_t steps, bool col_i) {
+// least reduction steps a split; short ones where there are few workgroups
+inline int tile_least(int t) { return t >= kDeep ? 128 : 256; }
+
+inline Split split_of(int tile) { return {tile_slots(tile), tile_least(tile)}; }
+
+// Tile of a product of reduction length nk in np passes, which ``split``s over its reduction or not.
+inline int choose_tile(int64_t ni, int64_t nj, int64_t nk, int np, bool col_i, bool split) {
   if (ni <= 32 && !col_i) return kFew;
-  const int64_t w = tiles_of(kWide, ni, nj), b = tiles_of(kBig, ni, nj);
+  const int64_t w = tiles_of(kWide, ni, nj), b = tiles_of(kBig, ni, nj), q = tiles_of(kSq, ni, nj);
   // the busiest CU's work: a kBig tile is half a kWide one at 0.84 of its rate (850 against 1000 TFLOP/s
   // over a long reduction); over a short one kWide's epilogue, which nothing hides, costs more than that
-  if (w >= 192 && steps >= 1536 && (w + 255) / 256 * 10 <= (b + 255) / 256 * 6) return kWide;
-  return b >= 256 ? kBig : kSq;
+  if (w >= 192 && nk * np >= 1536 && (w + 255) / 256 * 10 <= (b + 255) / 256 * 6) return kWide;
+  if (b >= 256) return kBig;
+  return q * (split ? split_of(kSq).of(q, nk) : 1) > 256 ? kSq : kDeep;
 }
 
 // Largest grid and slab (in rows) of a product whose rows in use are known on the device only: any
@@ -799,6 +809,7 @@ inline void gemm(int tile, const GemmArgs& p, int64_t grid, hipStream_t st) {
   if (tile == kWide) launch_gemm<Wide<F16, NP, IT, JT>, SUM>(p, grid, st);
   else if (tile == kBig) launch_gemm<Big<F16, NP, IT, JT>, SUM>(p, grid, st);
   else if (tile == kSq) launch_gemm<Sq<F16, NP, IT, JT>, SUM>(p, grid, st);
+  else if (tile == kDeep) launch_gemm<Deep<F16, NP, IT, JT>, SUM>(p, grid, st);
   else if constexpr (!IT) launch_gemm<Few<F16, NP, IT, JT>, SUM>(p, grid, st);
 }
 

@@ -400,7 +400,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void xent_join_kernel(const float2
 }
 
 // columns of one (max, sum) slot: a wave's part of the tile
-int tile_slot(int t) { return t <= kBig ? 128 : t == kSq ? 64 : 32; }
+int tile_slot(int t) { return t <= kBig ? 128 : t == kFew ? 32 : 64; }
 
 template <bool F16, bool BWD, bool TWO>
 void launch_logits(LogitArgs& p, int tile, hipStream_t st) {
@@ -417,6 +417,7 @@ void launch_logits(LogitArgs& p, int tile, hipStream_t st) {
   else if (!large || tile == kSq) go(static_cast<Sq<F16, NP, false, false>*>(nullptr));
   else if constexpr (large) {
     if (tile == kBig) go(static_cast<Big<F16, NP, false, false>*>(nullptr));
+    else if (tile == kDeep) go(static_cast<Deep<F16, NP, false, false>*>(nullptr));
     else go(static_cast<Wide<F16, NP, false, false>*>(nullptr));
   }
   check_launch();
@@ -453,7 +454,7 @@ XentPlan xent_plan(int rows, int width, int classes, bool f32) {
   q.two = f32 || rows <= kTwoRows;
   q.kp = int(up(width, 8));
   q.vpad = int(up(classes, 256));
-  auto tile = [&](int cols) { return rows > 32 && rows <= kTwoRows ? kSq : choose_tile(rows, cols, int64_t(width) * np, false); };
+  auto tile = [&](int cols) { return rows > 32 && rows <= kTwoRows ? kSq : choose_tile(rows, cols, width, np, false, false); };
   q.tile = tile(classes);
   q.slots = int(up(classes, tile_bj(q.tile)) / tile_slot(q.tile));
   int64_t at = 0;
@@ -482,12 +483,12 @@ XentPlan xent_plan(int rows, int width, int classes, bool f32) {
   // dx: few tiles and a long reduction (the piece), so as large a tile as the rows fill: its slabs'
   // traffic grows with the splits
   q.dx_tile = rows <= 32 ? kFew : rows < 1024 ? kSq : kWide;
-  q.dx_split = {tile_slots(q.dx_tile), 256};
+  q.dx_split = split_of(q.dx_tile);
   q.dx = extent_of(q.dx_tile, rows, width, q.dx_split, q.piece);
   q.b_dx = take(q.dx.slab_rows * q.kp * 4);
   const int64_t wi = std::min(q.piece, classes);
-  q.dw_tile = rows <= kTwoRows ? kSq : choose_tile(wi, width, int64_t(rows) * np, true);
-  q.dw_split = {tile_slots(q.dw_tile), 512};
+  q.dw_tile = rows <= kTwoRows ? kSq : choose_tile(wi, width, rows, np, true, true);
+  q.dw_split = split_of(q.dw_tile);
   q.dw_splits = q.dw_split.of(tiles_of(q.dw_tile, wi, width), rows);
   q.dw_split.most = q.dw_splits;  // a narrower last piece has no room for more
   q.b_dw = take(q.dw_splits > 1 ? int64_t(q.dw_splits) * q.piece * q.kp * 4 : 0);
