@@ -277,8 +277,6 @@ struct Tile {
           wait_vm_barrier<(ST - 2) * kPer>();
           aim();
           fetch(next, 0, 0);
-        } else {
-          fetch(buf, kk + 1, (kk + 1) & 1);
         }
         if constexpr (SUM) {
           // the reduction's sum of I: the hi plane in the last product, lo where it runs with J's hi
@@ -294,14 +292,23 @@ struct Tile {
 #pragma unroll
         for (int x = 0; x < mf; ++x) {
           acc[x / TI][x % TI] = mfma<F16>(fj[kk & 1][x / TI], fi[kk & 1][x % TI], acc[x / TI][x % TI]);
+          // between two products: a DMA instruction or two of the refill, or a fragment of the next step
           if (tail) {
             constexpr int per = (kPer + mf - 1) / mf;
 #pragma unroll
             for (int y = x * per; y < (x + 1) * per && y < kPer; ++y) issue(y, smem + buf * kStage);
-            __builtin_amdgcn_sched_barrier(0);
+          } else {
+            constexpr int nf = TI + TJ;
+            const uint8_t* li = smem + buf * kStage;
+#pragma unroll
+            for (int y = 0; y < nf; ++y)
+              if (y * mf / nf == x) {
+                if (y < TI) fi[(kk + 1) & 1][y] = si.frag(li, y, kk + 1);
+                else fj[(kk + 1) & 1][y - TI] = sj.frag(li + SI::kBytes, y - TI, kk + 1);
+              }
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_barrier(0);
       }
       buf = next;
     }
@@ -745,7 +752,9 @@ inline int whole_rows(uintptr_t p, int64_t ld, bool bf16) { return p % 16 == 0 &
 
 // Tiles (columns x rows).  A CU is bound by the rate at which lines reach its LDS, so the tile should be
 // as large as the product fills the chip with:
-//   kWide 256 x 256, one workgroup of 8 waves a CU;
+//   kWide 256 x 256, one workgroup of 8 waves a CU (four waves of 128 x 128 read a third less from the
+//         LDS and ran 8192 x 2048 x 32768 at 1170 TFLOP/s against 1100, but one wave a SIMD lost as
+//         much again in every epilogue that computes);
 //   kBig  256 x 128, two workgroups a CU: one's epilogue runs beside the other's products;
 //   kSq   128 x 128, two a CU;
 //   kDeep 128 x 128, one a CU on a ring twice as deep, where there are not two: nothing else hides the
