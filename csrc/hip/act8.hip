@@ -375,7 +375,7 @@ void linear_act8_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
   const int64_t grid_y = tiles_of(q.y_tile, rows, out) * q.y_s;
   if (f32) gemm<true, 3, false, false, false>(q.y_tile, a, grid_y, st);
   else gemm<false, 1, false, false, false>(q.y_tile, a, grid_y, st);
-  if (a.slab) finish(q.y_tile, a, int(rows), nullptr, st);
+  if (a.slab) finish(q.y_tile, a, int(rows), nullptr, {}, st);
 }
 
 // dx [rows][ldo] in x's type (added to when ``dx_add``); dw [out][ldd] and db [out] in ``grad_dt``
@@ -443,7 +443,7 @@ void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintpt
     const int64_t grid_x = tiles_of(q.dx_tile, rows, width) * q.dx_s;
     if (f32) gemm<true, 3, false, true, false>(q.dx_tile, a, grid_x, st);
     else gemm<false, 1, false, true, false>(q.dx_tile, a, grid_x, st);
-    if (a.slab) finish(q.dx_tile, a, int(rows), nullptr, st);
+    if (a.slab) finish(q.dx_tile, a, int(rows), nullptr, {}, st);
   }
   if (!dw) return;
   UnpackArgs u{};
@@ -485,7 +485,15 @@ void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintpt
   if (f32 && gelu) gemm<true, 3, true, true, true>(q.dw_tile, a, grid_w, st);
   else if (f32) gemm<true, 2, true, true, true>(q.dw_tile, a, grid_w, st);
   else gemm<false, 1, true, true, true>(q.dw_tile, a, grid_w, st);
-  if (a.slab) finish(q.dw_tile, a, int(out), nullptr, st);
+  if (a.slab) {
+    ColumnSums c{};
+    c.part = a.bslab;
+    c.ld = c.n = int(out);
+    c.parts = q.dw_s;
+    c.out = a.bout;
+    c.e = a.e;
+    finish(q.dw_tile, a, int(out), nullptr, c, st);
+  }
 }
 
 }  // namespace voda

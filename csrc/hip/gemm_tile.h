@@ -585,14 +585,26 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm_kernel(GemmArgs p) {
   }
 }
 
+// Sums of ``parts`` partial sums a column (rows_dev: of ``per`` for each ``bi`` rows in use instead).
+struct ColumnSums {
+  const float* part;  // [parts][ld], or null: none
+  int64_t ld;
+  int n, parts;
+  const int* rows_dev;
+  int bi, per;
+  void* out;
+  Emit e;             // factors (without J's), type and whether to add
+};
+
 // Sums the splits of a product's slab and stores the result; ``inv`` (or null) maps an output row to its
 // row of the slab, -1 where the row is zero.  LANES threads take eight columns together, each every
-// LANES-th split; behind them one thread a partial sum.
+// LANES-th split; behind them one thread a column sum.
 struct FinishArgs {
   GemmArgs g;
   int bi, bj;   // the product's tile
-  int rows;
+  int rows;     // 0: column sums alone
   const int* inv;
+  ColumnSums c;
 };
 
 template <int LANES>
@@ -601,9 +613,9 @@ static __global__ __launch_bounds__(256) void finish_kernel(FinishArgs p) {
   const int64_t n = int64_t(p.rows) * eights;
   const int64_t t = (int64_t(blockIdx.x) * 256 + threadIdx.x) / LANES;
   const int part = threadIdx.x % LANES;
-  const int used = p.g.rows();
-  const int splits = p.g.splits(int64_t((used + p.bi - 1) / p.bi) * ((p.g.e.nj + p.bj - 1) / p.bj));
   if (t < n) {
+    const int used = p.g.rows();
+    const int splits = p.g.splits(int64_t((used + p.bi - 1) / p.bi) * ((p.g.e.nj + p.bj - 1) / p.bj));
     const int i = int(t / eights), j = 8 * int(t - int64_t(i) * eights);
     const int src = p.inv ? p.inv[i] : i;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -622,11 +634,13 @@ static __global__ __launch_bounds__(256) void finish_kernel(FinishArgs p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += __shfl_xor(v[e], o, 64);
     if (part == 0) p.g.e.eight(p.g.e.once(j), i, j, v, src >= 0);
-  } else if (p.g.bslab && t - n < p.rows && part == 0) {
+  } else if (p.c.part && t - n < p.c.n && part == 0) {
     const int i = int(t - n);
+    const int parts = p.c.rows_dev ? (*p.c.rows_dev + p.c.bi - 1) / p.c.bi * p.c.per : p.c.parts;
     float v = 0.f;
-    for (int s = 0; s < splits; ++s) v += p.g.bslab[int64_t(s) * p.g.I.n + i];
-    emit_sum(p.g.e, p.g.e.once(p.g.e.nj), p.g.bout, i, v);
+#pragma unroll 8
+    for (int s = 0; s < parts; ++s) v += p.c.part[int64_t(s) * p.c.ld + i];
+    emit_sum(p.c.e, p.c.e.once(p.c.e.nj), p.c.out, i, v);
   }
 }
 
@@ -822,9 +836,10 @@ inline void gemm(int tile, const GemmArgs& p, int64_t grid, hipStream_t st) {
   else if constexpr (!IT) launch_gemm<Few<F16, NP, IT, JT>, SUM>(p, grid, st);
 }
 
-inline void finish(int tile, const GemmArgs& g, int rows, const int* inv, hipStream_t st) {
-  const FinishArgs p = {g, tile_bi(tile), tile_bj(tile), rows, inv};
-  const int64_t n = int64_t(rows) * ((g.e.nj + 7) / 8) + (g.bslab ? rows : 0);
+inline void finish(int tile, const GemmArgs& g, int rows, const int* inv, const ColumnSums& c, hipStream_t st) {
+  const FinishArgs p = {g, tile_bi(tile), tile_bj(tile), rows, inv, c};
+  const int64_t n = int64_t(rows) * ((g.e.nj + 7) / 8) + (c.part ? c.n : 0);
+  if (n == 0) return;
   // few outputs: eight lanes on each keep the loads of many splits in flight
   if (n <= 16384) hipLaunchKernelGGL((finish_kernel<8>), dim3(unsigned((n * 8 + 255) / 256)), dim3(256), 0, st, p);
   else hipLaunchKernelGGL((finish_kernel<1>), dim3(unsigned((n + 255) / 256)), dim3(256), 0, st, p);

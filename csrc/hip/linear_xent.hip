@@ -175,6 +175,8 @@ struct LogitArgs {
   const float2* stat;
   uint16_t* G;
   int64_t ldg, gplane;
+  float* sums;          // sums of G over a wave's rows [tile, wave][sums_ld], or null
+  int64_t sums_ld;
 };
 
 // Rows are the tile's i, vocabulary columns its j.  The epilogue is vector work that the matrix cores
@@ -215,6 +217,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
         }
     }
   }
+  float sums[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // BWD: of this lane's columns
 #pragma unroll
   for (int c = 0; c < T::TI; ++c) {
     if constexpr (!BWD) {
@@ -285,6 +288,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
           if constexpr (F16) z = z * sx * sw;
           float d = __builtin_amdgcn_exp2f((z + bias[e] - st.x) * kLog2e) * st.y;
           if (e == y) d -= 1.f;
+          sums[e] += d;
           if constexpr (F16) split2(d * kGScale, hi[e], lo[e]);
           else hi[e] = f2bf(d);
           if constexpr (TWO && !F16) lo[e] = f2bf(d - bf2f(hi[e]));
@@ -296,6 +300,21 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
         *reinterpret_cast<uint4*>(g) = eight(hi);
         if constexpr (TWO) *reinterpret_cast<uint4*>(g + p.gplane) = eight(lo);
       });
+    }
+  }
+  if constexpr (BWD) {
+    if (p.sums) {
+      // db from G as it is, not as it was rounded for the products: its terms cancel
+      constexpr int EI = 4 * T::TJ;  // lanes with columns of their own
+#pragma unroll
+      for (int o = EI; o < 64; o <<= 1)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sums[e] += __shfl_xor(sums[e], o, 64);
+      if (w.lane < EI) {
+        float* o = p.sums + int64_t(ti * T::WI + w.wi) * p.sums_ld + j0 + w.wj * T::TJ * 32 + 8 * w.lane;
+        *reinterpret_cast<float4*>(o) = make_float4(sums[0], sums[1], sums[2], sums[3]);
+        *reinterpret_cast<float4*>(o + 4) = make_float4(sums[4], sums[5], sums[6], sums[7]);
+      }
     }
   }
 }
@@ -399,6 +418,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void xent_join_kernel(const float2
   }
 }
 
+// waves down a tile's rows
+int tile_wi(int t) { return t == kWide ? 4 : t == kFew ? 1 : 2; }
 // columns of one (max, sum) slot: a wave's part of the tile
 int tile_slot(int t) { return t <= kBig ? 128 : t == kFew ? 32 : 64; }
 
@@ -492,7 +513,7 @@ XentPlan xent_plan(int rows, int width, int classes, bool f32) {
   q.dw_splits = q.dw_split.of(tiles_of(q.dw_tile, wi, width), rows);
   q.dw_split.most = q.dw_splits;  // a narrower last piece has no room for more
   q.b_dw = take(q.dw_splits > 1 ? int64_t(q.dw_splits) * q.piece * q.kp * 4 : 0);
-  q.b_db = take(q.dw_splits > 1 ? int64_t(q.dw_splits) * q.piece * 4 : 0);
+  q.b_db = take((rows + tile_bi(q.gtile) - 1) / tile_bi(q.gtile) * int64_t(tile_wi(q.gtile)) * q.vpad * 4);
   q.bwd_bytes = at;
   return q;
 }
@@ -595,7 +616,7 @@ void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
 }
 
 // dx [rows][width] contiguous in x's type; rows [0, classes) of dw [..][ldd] and of db in ``grad_dt``
-// (added to when ``accumulate``); dx, db, or dw and db may be null.
+// (added to when ``accumulate``); each of dx, dw and db may be null.
 void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int64_t classes, int64_t vocab, int dt,
                      uintptr_t ws, uintptr_t xc, uintptr_t bias32, uintptr_t inv, uintptr_t lab, uintptr_t stat,
                      uintptr_t dev, uintptr_t amax, uintptr_t gloss, uintptr_t dx, uintptr_t dw, int64_t ldd,
@@ -629,6 +650,8 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
   p.G = reinterpret_cast<uint16_t*>(base + q.b_g);
   p.ldg = q.piece;
   p.gplane = rows * q.piece;
+  p.sums = db ? reinterpret_cast<float*>(base + q.b_db) : nullptr;
+  p.sums_ld = q.vpad;
   const float* gl = reinterpret_cast<const float*>(gloss);
   Emit e{};
   e.f = f32 ? 1.f / kGScale : 1.f;
@@ -681,20 +704,33 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
       a.e.nj = int(width);
       a.e.vec = whole_rows(dw, ldd, a.e.bf16);
       a.e.accumulate = accumulate;
-      a.bout = db ? reinterpret_cast<void*>(db + uintptr_t(v0) * gsz) : nullptr;
       if (q.dw_splits > 1) {
         a.slab = reinterpret_cast<float*>(base + q.b_dw);
         a.lds = q.kp;
-        a.bslab = db ? reinterpret_cast<float*>(base + q.b_db) : nullptr;
       }
       const int64_t grid = tiles_of(q.dw_tile, v1 - v0, width) * q.dw_splits;
-      if (f32) gemm<true, 3, true, true, true>(q.dw_tile, a, grid, st);
-      else if (q.two) launch_gemm<Sq<false, 2, true, true>, true>(a, grid, st);
-      else gemm<false, 1, true, true, true>(q.dw_tile, a, grid, st);
-      if (a.slab) finish(q.dw_tile, a, a.I.n, nullptr, st);
+      if (f32) gemm<true, 3, true, true, false>(q.dw_tile, a, grid, st);
+      else if (q.two) launch_gemm<Sq<false, 2, true, true>, false>(a, grid, st);
+      else gemm<false, 1, true, true, false>(q.dw_tile, a, grid, st);
+      if (a.slab) finish(q.dw_tile, a, a.I.n, nullptr, {}, st);
     }
   }
-  if (dx) finish(q.dx_tile, x, int(rows), reinterpret_cast<const int*>(inv), st);
+  ColumnSums c{};
+  if (db) {
+    c.part = p.sums;
+    c.ld = q.vpad;
+    c.n = int(classes);
+    c.rows_dev = &d->n;
+    c.bi = tile_bi(q.gtile);
+    c.per = tile_wi(q.gtile);
+    c.out = reinterpret_cast<void*>(db);
+    c.e.f = 1.f;
+    c.e.gl = e.gl;
+    c.e.gn = e.gn;
+    c.e.bf16 = grad_dt == kBF16;
+    c.e.accumulate = accumulate;
+  }
+  finish(q.dx_tile, x, dx ? int(rows) : 0, reinterpret_cast<const int*>(inv), c, st);
 }
 
 }  // namespace voda

@@ -127,25 +127,20 @@ class _LinearXentFn(torch.autograd.Function):
             # into the optimizer's flat gradients where it owns every gradient that is asked for
             direct = ((need_w or need_b) and (not need_w or _direct(wp)) and (not need_b or _direct(bp))
                       and (not (need_w and need_b) or flat_grad(wp).dtype == flat_grad(bp).dtype))
-            gdt = torch.float32
             if direct:
                 gdt = flat_grad(wp if need_w else bp).dtype
                 direct = gdt in (torch.float32, torch.bfloat16)
-            if need_w or need_b:
-                if direct and need_w:
-                    dw = flat_grad(wp)
-                else:
-                    gdt = gdt if direct else weight.dtype
-                    dw = torch.empty(V, K, dtype=gdt, device=dev)
-                if need_b:
-                    db = flat_grad(bp) if direct else torch.empty(V, dtype=gdt, device=dev)
-                if not direct and C < V:
-                    dw[C:].zero_()
-                    if db is not None:
-                        db[C:].zero_()
+            if not direct:
+                gdt = weight.dtype
+            if need_w:
+                dw = flat_grad(wp) if direct else torch.empty(V, K, dtype=gdt, device=dev)
+            if need_b:
+                db = flat_grad(bp) if direct else torch.empty(V, dtype=gdt, device=dev)
+            if not direct and C < V:
+                for t in (dw, db):
+                    if t is not None:
+                        t[C:].zero_()
             ws = torch.empty(max(ctx.nb, 256), dtype=torch.uint8, device=dev)
-            if direct and not need_w:
-                dw.zero_()
             N.hip().linear_xent_bwd(w.data_ptr(), w.stride(0), rows, K, C, V, N.dtype_code(ctx.x_dtype), ws.data_ptr(),
                                     p[0], p[1], p[2], p[3], p[4], p[5], p[6], g.data_ptr(), N.ptr(dx),
                                     N.ptr(dw), dw.stride(0) if dw is not None else K, N.ptr(db), N.dtype_code(gdt),
@@ -156,8 +151,6 @@ class _LinearXentFn(torch.autograd.Function):
             if need_b:
                 _ready(bp)
             dw = db = None
-        if not need_w:
-            dw = None
         if db is not None and db.dtype != bp.dtype:
             db = db.to(bp.dtype)
         return dx, dw, db, None, None, None
