@@ -378,14 +378,15 @@ void linear_act8_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
   if (a.slab) finish(q.y_tile, a, int(rows), nullptr, {}, st);
 }
 
-// dx [rows][ldo] in x's type (added to when ``dx_add``); dw [out][ldd] and db [out] in ``grad_dt``
-// (added to when ``accumulate``); dx, db, or dw and db may be null.  dy: bf16 rows of whole 16-byte vectors.
+// dx [rows][width] in x's type (added to when ``dx_add``); dw [out][ldd] in ``grad_dt`` and db [out] in
+// ``db_dt`` (added to when ``accumulate``); dx, db, or dw and db may be null.  dy: bf16 rows of whole 16-byte vectors.
 void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintptr_t qp, uintptr_t qs, uintptr_t dx,
-                     bool dx_add, uintptr_t dw, int64_t ldd, uintptr_t db, int grad_dt, bool accumulate, int64_t rows,
+                     bool dx_add, uintptr_t dw, int64_t ldd, uintptr_t db, int grad_dt, int db_dt, bool accumulate, int64_t rows,
                      int64_t width, int64_t out, int dt, bool gelu, uintptr_t amax, uintptr_t ws, uintptr_t stream) {
   check_act8(rows, width, out, dt);
   const bool f32 = dt == kF32;
-  VODA_CHECK(grad_dt == kF32 || grad_dt == kBF16, "linear_act8: weight gradients must be fp32 or bf16");
+  VODA_CHECK((grad_dt == kF32 || grad_dt == kBF16) && (db_dt == kF32 || db_dt == kBF16),
+             "linear_act8: weight and bias gradients must be fp32 or bf16");
   VODA_CHECK(f32 || (w % 16 == 0 && ldw % 8 == 0 && ldw >= up(width, 8)),
              "linear_act8: bf16 weight rows must be 16-byte aligned and whole 16-byte vectors");
   VODA_CHECK(f32 || (dy % 16 == 0 && ldy % 8 == 0 && ldy >= up(out, 8)),
@@ -476,6 +477,7 @@ void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintpt
   a.e.vec = whole_rows(dw, ldd, a.e.bf16);
   a.e.accumulate = accumulate;
   a.bout = reinterpret_cast<void*>(db);
+  a.bout_bf16 = db_dt == kBF16;
   if (q.dw_s > 1) {
     a.slab = reinterpret_cast<float*>(base + q.b_dw);
     a.lds = q.kp;
@@ -491,6 +493,7 @@ void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintpt
     c.ld = c.n = int(out);
     c.parts = q.dw_s;
     c.out = a.bout;
+    c.bf16 = a.bout_bf16;
     c.e = a.e;
     finish(q.dw_tile, a, int(out), nullptr, c, st);
   }

@@ -509,7 +509,8 @@ struct GemmArgs {
   int64_t lds;
   int add;
   float* bslab;          // [split][I.n] partial sums of I over k (col I), or null
-  void* bout;            // their result when there is no slab, in out's type
+  void* bout;            // their result when there is no slab
+  int bout_bf16;
   Emit e;
 
   __device__ __forceinline__ int rows() const { return ni_dev ? min(I.n, *ni_dev) : I.n; }
@@ -527,9 +528,9 @@ __device__ __forceinline__ void split_range(int nk, int splits, int s, int bk, i
 }
 
 // a sum over I alone: without J's factor
-__device__ __forceinline__ void emit_sum(const Emit& e, const Emit::Once& o, void* out, int i, float v) {
+__device__ __forceinline__ void emit_sum(const Emit& e, const Emit::Once& o, void* out, bool bf16, int i, float v) {
   v = v * o.a * o.b;
-  if (e.bf16) {
+  if (bf16) {
     uint16_t* o = static_cast<uint16_t*>(out) + i;
     *o = f2bf(v + (e.accumulate ? bf2f(*o) : 0.f));
   } else {
@@ -573,7 +574,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm_kernel(GemmArgs p) {
         const float tot = isum[b] + __shfl_xor(isum[b], 32, 64);
         if (w.h == 0 && i < I.n) {
           if (p.bslab) p.bslab[int64_t(s) * p.I.n + i] = tot;
-          else emit_sum(p.e, once, p.bout, i, tot);
+          else emit_sum(p.e, once, p.bout, p.bout_bf16, i, tot);
         }
       }
     }
@@ -593,7 +594,8 @@ struct ColumnSums {
   const int* rows_dev;
   int bi, per;
   void* out;
-  Emit e;             // factors (without J's), type and whether to add
+  int bf16;
+  Emit e;             // factors (without J's) and whether to add
 };
 
 // Sums the splits of a product's slab and stores the result; ``inv`` (or null) maps an output row to its
@@ -640,7 +642,7 @@ static __global__ __launch_bounds__(256) void finish_kernel(FinishArgs p) {
     float v = 0.f;
 #pragma unroll 8
     for (int s = 0; s < parts; ++s) v += p.c.part[int64_t(s) * p.c.ld + i];
-    emit_sum(p.c.e, p.c.e.once(p.c.e.nj), p.c.out, i, v);
+    emit_sum(p.c.e, p.c.e.once(p.c.e.nj), p.c.out, p.c.bf16, i, v);
   }
 }
 
@@ -813,11 +815,14 @@ struct Extent {
 };
 inline Extent extent_of(int tile, int64_t ni, int64_t nj, const Split& split, int64_t nk) {
   Extent x{1, 1};
-  for (int64_t t = 1, n = tiles_of(tile, ni, 1); t <= n; ++t) {
-    const int64_t tiles = t * tiles_of(tile, 1, nj), s = split.of(tiles, nk), rows = s * std::min(ni, t * tile_bi(tile));
-    x.grid = std::max(x.grid, tiles * s);
-    x.slab_rows = std::max(x.slab_rows, rows);
-  }
+  const int64_t n = tiles_of(tile, ni, 1), tj = tiles_of(tile, 1, nj);
+  auto add = [&](int64_t t) {
+    const int64_t s = split.of(t * tj, nk);
+    x.grid = std::max(x.grid, t * tj * s);
+    x.slab_rows = std::max(x.slab_rows, s * std::min(ni, t * tile_bi(tile)));
+  };
+  for (int64_t t = 1; t < n && t * tj <= split.slots; ++t) add(t);  // past the slots there is one split
+  add(n);
   return x;
 }
 

@@ -67,7 +67,26 @@ struct GatherArgs {
   int bias_n;
   const float* amax; // fp32: partial maxima of x
   int gather_blocks;
+  const int* counts; // labelled rows of each kCountRows, or null: count them here
 };
+
+// Many rows: how many of each 1024 are labelled.
+constexpr int kCountRows = 1024;
+__global__ __launch_bounds__(256) void xent_count_kernel(const int64_t* __restrict__ labels, int rows, int64_t ignore,
+                                                         int classes, int* __restrict__ counts) {
+  __shared__ int cnt[4];
+  int c = 0;
+#pragma unroll
+  for (int k = 0; k < kCountRows / 256; ++k) {
+    const int r = blockIdx.x * kCountRows + 256 * k + threadIdx.x;
+    c += r < rows && labelled(labels[r], ignore, classes);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
+  if ((threadIdx.x & 63) == 0) cnt[threadIdx.x >> 6] = c;
+  __syncthreads();
+  if (threadIdx.x == 0) counts[blockIdx.x] = cnt[0] + cnt[1] + cnt[2] + cnt[3];
+}
 
 // Labelled rows of x together, and what goes with them; then the bias in fp32.
 template <bool F32>
@@ -91,11 +110,17 @@ __global__ __launch_bounds__(256) void xent_gather_kernel(GatherArgs p) {
     if (blockIdx.x == 0 && t == 0) p.dev->inv_x = pow2_inverse(scale);
   }
   // labelled rows in front of this workgroup's: every workgroup counts them itself (8 bytes a row
-  // out of the L2), which is cheaper than a second launch
+  // out of the L2), cheaper than a second launch up to some thousand rows, or from the counts
   const int r0 = blockIdx.x * kGatherRows;
-  int c = 0;
+  int c = 0, from = 0;
+  if (p.counts) {
+    const int segs = r0 / kCountRows;
 #pragma unroll 8
-  for (int r = t; r < r0; r += 256) c += labelled(p.labels[r], p.ignore, p.classes);
+    for (int k = t; k < segs; k += 256) c += p.counts[k];
+    from = segs * kCountRows;
+  }
+#pragma unroll 8
+  for (int r = from + t; r < r0; r += 256) c += labelled(p.labels[r], p.ignore, p.classes);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
   if (lane == 0) cnt[wave] = c;
@@ -161,7 +186,7 @@ __global__ __launch_bounds__(256) void xent_gather_kernel(GatherArgs p) {
 
 struct LogitArgs {
   Operand X, W;
-  int width, classes, tj;
+  int width, tj;
   int v0, v1;           // vocabulary columns of this launch
   const float* bias32;
   const XentDev* dev;
@@ -311,7 +336,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
 #pragma unroll
         for (int e = 0; e < 8; ++e) sums[e] += __shfl_xor(sums[e], o, 64);
       if (w.lane < EI) {
-        float* o = p.sums + int64_t(ti * T::WI + w.wi) * p.sums_ld + j0 + w.wj * T::TJ * 32 + 8 * w.lane;
+        float* o = p.sums + int64_t(ti * T::WI + w.wi) * p.sums_ld + (j0 - p.v0) + w.wj * T::TJ * 32 + 8 * w.lane;
         *reinterpret_cast<float4*>(o) = make_float4(sums[0], sums[1], sums[2], sums[3]);
         *reinterpret_cast<float4*>(o + 4) = make_float4(sums[4], sums[5], sums[6], sums[7]);
       }
@@ -457,13 +482,14 @@ struct XentPlan {
   Extent dx;
   int64_t fwd_bytes, bwd_bytes;
   // offsets into the forward's workspace
-  int64_t o_wp, o_part, o_zlab, o_tie, o_lsum, o_csum;
+  int64_t o_wp, o_part, o_zlab, o_tie, o_lsum, o_csum, o_counts;
   // offsets into the backward's
   int64_t b_wp, b_g, b_dx, b_dw, b_db;
 };
 
 constexpr int64_t kGBytes = int64_t(512) << 20;  // G of one piece of the vocabulary
 constexpr int kTwoRows = 128;
+constexpr int kCountFrom = 4096;  // rows from which xent_count runs: 10240 rows gather in 6 + 3 us instead of 14
 
 XentPlan xent_plan(int rows, int width, int classes, bool f32) {
   XentPlan q{};
@@ -491,6 +517,7 @@ XentPlan xent_plan(int rows, int width, int classes, bool f32) {
   const int64_t jb = (rows + 15) / 16;
   q.o_lsum = take(jb * 8);
   q.o_csum = take(jb * 4);
+  q.o_counts = take(rows > kCountFrom ? (rows + kCountRows - 1) / kCountRows * int64_t(4) : 0);
   q.fwd_bytes = at;
   at = 0;
   q.b_wp = take(f32 ? int64_t(classes) * q.kp * 4 : 0);
@@ -513,7 +540,7 @@ XentPlan xent_plan(int rows, int width, int classes, bool f32) {
   q.dw_splits = q.dw_split.of(tiles_of(q.dw_tile, wi, width), rows);
   q.dw_split.most = q.dw_splits;  // a narrower last piece has no room for more
   q.b_dw = take(q.dw_splits > 1 ? int64_t(q.dw_splits) * q.piece * q.kp * 4 : 0);
-  q.b_db = take((rows + tile_bi(q.gtile) - 1) / tile_bi(q.gtile) * int64_t(tile_wi(q.gtile)) * q.vpad * 4);
+  q.b_db = take((rows + tile_bi(q.gtile) - 1) / tile_bi(q.gtile) * int64_t(tile_wi(q.gtile)) * q.piece * 4);
   q.bwd_bytes = at;
   return q;
 }
@@ -579,6 +606,13 @@ void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
   g.bias_n = q.vpad;
   g.amax = am;
   g.gather_blocks = int((rows + kGatherRows - 1) / kGatherRows);
+  if (rows > kCountFrom) {
+    int* counts = reinterpret_cast<int*>(base + q.o_counts);
+    hipLaunchKernelGGL(xent_count_kernel, dim3(unsigned((rows + kCountRows - 1) / kCountRows)), dim3(256), 0, st, g.labels,
+                       int(rows), ignore, int(classes), counts);
+    check_launch();
+    g.counts = counts;
+  }
   const dim3 gg(unsigned(g.gather_blocks + (q.vpad + 255) / 256));
   if (f32) hipLaunchKernelGGL((xent_gather_kernel<true>), gg, dim3(256), 0, st, g);
   else hipLaunchKernelGGL((xent_gather_kernel<false>), gg, dim3(256), 0, st, g);
@@ -593,7 +627,6 @@ void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
     p.W = {wp, q.kp, classes * q.kp, int(classes)};
   }
   p.width = q.kp;
-  p.classes = int(classes);
   p.v0 = 0;
   p.v1 = int(classes);
   p.bias32 = g.bias32;
@@ -615,15 +648,16 @@ void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
   check_launch();
 }
 
-// dx [rows][width] contiguous in x's type; rows [0, classes) of dw [..][ldd] and of db in ``grad_dt``
-// (added to when ``accumulate``); each of dx, dw and db may be null.
+// dx [rows][width] contiguous in x's type; rows [0, classes) of dw [..][ldd] in ``grad_dt`` and of db in
+// ``db_dt`` (added to when ``accumulate``); each of dx, dw and db may be null.
 void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int64_t classes, int64_t vocab, int dt,
                      uintptr_t ws, uintptr_t xc, uintptr_t bias32, uintptr_t inv, uintptr_t lab, uintptr_t stat,
                      uintptr_t dev, uintptr_t amax, uintptr_t gloss, uintptr_t dx, uintptr_t dw, int64_t ldd,
-                     uintptr_t db, int grad_dt, bool accumulate, uintptr_t stream) {
+                     uintptr_t db, int grad_dt, int db_dt, bool accumulate, uintptr_t stream) {
   check_xent(rows, width, classes, vocab);
   VODA_CHECK(dt == kF32 || dt == kBF16, "linear_xent: x must be fp32 or bf16");
-  VODA_CHECK(grad_dt == kF32 || grad_dt == kBF16, "linear_xent: weight gradients must be fp32 or bf16");
+  VODA_CHECK((grad_dt == kF32 || grad_dt == kBF16) && (db_dt == kF32 || db_dt == kBF16),
+             "linear_xent: weight and bias gradients must be fp32 or bf16");
   const bool f32 = dt == kF32;
   VODA_CHECK(f32 || (w % 16 == 0 && ldw % 8 == 0 && ldw >= up(width, 8)),
              "linear_xent: bf16 weight rows must be 16-byte aligned and whole 16-byte vectors");
@@ -642,7 +676,6 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
     p.W = {wp, q.kp, classes * q.kp, int(classes)};
   }
   p.width = q.kp;
-  p.classes = int(classes);
   p.bias32 = reinterpret_cast<const float*>(bias32);
   p.dev = d;
   p.lab = reinterpret_cast<const int*>(lab);
@@ -651,11 +684,10 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
   p.ldg = q.piece;
   p.gplane = rows * q.piece;
   p.sums = db ? reinterpret_cast<float*>(base + q.b_db) : nullptr;
-  p.sums_ld = q.vpad;
-  const float* gl = reinterpret_cast<const float*>(gloss);
+  p.sums_ld = q.piece;
   Emit e{};
   e.f = f32 ? 1.f / kGScale : 1.f;
-  e.gl = gl;
+  e.gl = reinterpret_cast<const float*>(gloss);
   e.gn = &d->n;
   const int gsz = grad_dt == kF32 ? 4 : 2;
   GemmArgs x{};
@@ -672,9 +704,21 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
   x.e.bf16 = !f32;
   x.e.nj = int(width);
   x.e.vec = whole_rows(dx, width, !f32);
-  for (int v0 = 0; v0 < q.vpad; v0 += q.piece) {
+  ColumnSums c{};  // db of a piece
+  if (db) {
+    c.part = p.sums;
+    c.ld = q.piece;
+    c.rows_dev = &d->n;
+    c.bi = tile_bi(q.gtile);
+    c.per = tile_wi(q.gtile);
+    c.bf16 = db_dt == kBF16;
+    c.e.f = 1.f;
+    c.e.gl = e.gl;
+    c.e.gn = e.gn;
+    c.e.accumulate = accumulate;
+  }
+  for (int v0 = 0; v0 < classes; v0 += q.piece) {
     const int v1 = int(std::min<int64_t>(classes, v0 + q.piece));
-    if (v1 <= v0) break;
     p.v0 = v0;
     p.v1 = v1;
     if (f32) launch_logits<true, true, true>(p, q.gtile, st);
@@ -714,23 +758,11 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
       else gemm<false, 1, true, true, false>(q.dw_tile, a, grid, st);
       if (a.slab) finish(q.dw_tile, a, a.I.n, nullptr, {}, st);
     }
+    c.n = v1 - v0;
+    c.out = reinterpret_cast<void*>(db + uintptr_t(v0) * (db_dt == kF32 ? 4 : 2));
+    // dx is whole after the last piece
+    finish(q.dx_tile, x, dx && v1 == classes ? int(rows) : 0, reinterpret_cast<const int*>(inv), c, st);
   }
-  ColumnSums c{};
-  if (db) {
-    c.part = p.sums;
-    c.ld = q.vpad;
-    c.n = int(classes);
-    c.rows_dev = &d->n;
-    c.bi = tile_bi(q.gtile);
-    c.per = tile_wi(q.gtile);
-    c.out = reinterpret_cast<void*>(db);
-    c.e.f = 1.f;
-    c.e.gl = e.gl;
-    c.e.gn = e.gn;
-    c.e.bf16 = grad_dt == kBF16;
-    c.e.accumulate = accumulate;
-  }
-  finish(q.dx_tile, x, dx ? int(rows) : 0, reinterpret_cast<const int*>(inv), c, st);
 }
 
 }  // namespace voda

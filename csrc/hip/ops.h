@@ -69,7 +69,7 @@ void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
 void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int64_t classes, int64_t vocab, int dt,
                      uintptr_t ws, uintptr_t xc, uintptr_t bias32, uintptr_t inv, uintptr_t lab, uintptr_t stat,
                      uintptr_t dev, uintptr_t amax, uintptr_t gloss, uintptr_t dx, uintptr_t dw, int64_t ldd,
-                     uintptr_t db, int grad_dt, bool accumulate, uintptr_t stream);
+                     uintptr_t db, int grad_dt, int db_dt, bool accumulate, uintptr_t stream);
 
 // ---- Linear with an 8-bit input checkpoint (act8.hip) ----
 std::vector<int64_t> linear_act8_sizes(int64_t rows, int64_t width, int64_t out, int dt, bool copy);
@@ -80,7 +80,7 @@ void linear_act8_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
                      uintptr_t qp, uintptr_t qs, int64_t rows, int64_t width, int64_t out, int dt, bool gelu, bool copy,
                      uintptr_t amax, uintptr_t ws, uintptr_t stream);
 void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintptr_t qp, uintptr_t qs, uintptr_t dx,
-                     bool dx_add, uintptr_t dw, int64_t ldd, uintptr_t db, int grad_dt, bool accumulate, int64_t rows,
+                     bool dx_add, uintptr_t dw, int64_t ldd, uintptr_t db, int grad_dt, int db_dt, bool accumulate, int64_t rows,
                      int64_t width, int64_t out, int dt, bool gelu, uintptr_t amax, uintptr_t ws, uintptr_t stream);
 
 // ---- fused softmax cross-entropy (xent.hip) ----

@@ -127,4 +127,4 @@ def test_the_host_refuses():
     with pytest.raises(ValueError):  # bf16 rows off 16 bytes need the copy
         h.linear_act8_fwd(2, 8, 16, 8, 0, 0, 0, 16, 0, 4, 8, 8, 1, False, False, 0, 256, 0)
     with pytest.raises(ValueError):
-        h.linear_act8_bwd(2, 8, 16, 8, 16, 0, 0, False, 0, 8, 0, 0, False, 4, 8, 8, 1, False, 0, 256, 0)
+        h.linear_act8_bwd(2, 8, 16, 8, 16, 0, 0, False, 0, 8, 0, 0, 0, False, 4, 8, 8, 1, False, 0, 256, 0)

@@ -101,6 +101,30 @@ def test_strides_and_shapes(dtype):
     assert all(torch.equal(p, q) for p, q in zip(g1, g2))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_expanded_operands(dtype):
+    """Rows that are all one row: of the gradient (a sum over the rows behind the layer), the input and the
+    weight."""
+    x, w, b, _ = _inputs(40, 64, 48, dtype, bias=True)
+    x1, w1 = (t.detach()[:1].expand(*t.shape) for t in (x, w))
+    dy = torch.randn(1, 48, device=DEV).to(dtype).expand(40, 48)
+    assert dy.stride(0) == 0
+    for xe, we in ((x, w), (x1.requires_grad_(), w1.requires_grad_())):
+        y = linear_act8(xe, we, b)
+        got = torch.autograd.grad(y, (xe, we, b), dy)
+        ref = _run(xe.detach().contiguous().requires_grad_(), we.detach().contiguous().requires_grad_(), b,
+                   dy.contiguous(), None)
+        assert all(torch.equal(g, r) for g, r in zip((y, *got), ref))
+
+
+@pytest.mark.parametrize("rows", [20, 900])
+def test_bias_of_another_type(rows):
+    x, w, b, dy = _inputs(rows, 72, 48, torch.bfloat16, bias=True)
+    b = b.detach().float().requires_grad_()
+    got = _check(x, w, b, dy, "gelu")
+    assert got[3].dtype == torch.float32
+
+
 def test_offsets_past_32_bits():
     x, w, b, dy = _inputs(700, 64, 700, torch.bfloat16, bias=True)
     want = _check(x, w, b, dy, None)

@@ -202,6 +202,33 @@ def test_offsets_past_32_bits():
         assert torch.equal(g, r)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [4096, 4097, 150000])
+def test_many_rows(rows, dtype):
+    """Past the row count from which the labelled rows are counted beforehand."""
+    x, w, b, y = _inputs(rows, 16, 50, 50, dtype, bias=True, ignored=0.5)
+    y[:2500] = -100
+    _check(x, w, b, y, 50)
+
+
+@pytest.mark.parametrize("rows", [20, 900])
+def test_bias_of_another_type(rows):
+    x, w, b, y = _inputs(rows, 64, 300, 290, torch.bfloat16, bias=True)
+    _, grads = _check(x, w, b.detach().float().requires_grad_(), y, 290)
+    assert grads[2].dtype == torch.float32
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_expanded_operands(dtype):
+    x, w, b, y = _inputs(40, 64, 300, 300, dtype, bias=False)
+    x1, w1 = (t.detach()[:1].expand(*t.shape) for t in (x, w))
+    want = _check(x1.contiguous().requires_grad_(), w1.contiguous().requires_grad_(), None, y, 300)
+    x1.requires_grad_(), w1.requires_grad_()
+    loss = linear_cross_entropy(x1, w1, y)[0]
+    assert torch.equal(loss, want[0])
+    assert all(torch.equal(g, r) for g, r in zip(torch.autograd.grad(loss, (x1, w1)), want[1]))
+
+
 @pytest.mark.parametrize("need", [(True, False, False), (False, True, False), (False, False, True), (False, True, True)])
 def test_gradients_asked_for(need):
     x, w, b, y = _inputs(50, 64, 300, 290, torch.bfloat16, bias=True)

@@ -154,8 +154,8 @@ class _LinearAct8Fn(torch.autograd.Function):
             hb.done = False
         if dy.dtype != dt:
             dy = dy.to(dt)
-        if dy.stride(1) != 1:
-            dy = dy.contiguous()
+        if dy.stride(1) != 1 or dy.stride(0) < out:
+            dy = dy.contiguous()  # (an expanded gradient's rows overlap)
         acc = ctx.sink_in.take() if ctx.sink_in is not None and need_x else None
         if acc is not None:
             acc = acc.reshape(rows, K).to(dt).contiguous()
@@ -183,30 +183,27 @@ class _LinearAct8Fn(torch.autograd.Function):
             w = weight if f32 else _rows16(weight)
             if need_x:
                 dx = acc if acc is not None else torch.empty(rows, K, dtype=dt, device=dev)
-            gdt = weight.dtype
-            direct = need_w and _direct(wp) and (not need_b or _direct(bp)) and flat_grad(wp).dtype in (
-                torch.float32, torch.bfloat16) and (not need_b or flat_grad(bp).dtype == flat_grad(wp).dtype)
-            if direct:
-                dw, db = flat_grad(wp), flat_grad(bp) if need_b else None
-                gdt = dw.dtype
-            elif need_w:
-                dw = torch.empty(out, K, dtype=gdt, device=dev)
-                db = torch.empty(out, dtype=gdt, device=dev) if need_b else None
+            # into the optimizer's flat gradients where it owns every gradient that is asked for
+            direct = need_w and all(_direct(t) and flat_grad(t).dtype in (torch.float32, torch.bfloat16)
+                                    for t, need in ((wp, True), (bp, need_b)) if need)
+            if need_w:
+                dw = flat_grad(wp) if direct else torch.empty(out, K, dtype=weight.dtype, device=dev)
+                if need_b:
+                    db = flat_grad(bp) if direct else torch.empty(out, dtype=bp.dtype, device=dev)
             elif need_b:
-                db = dy[:, :out].float().sum(0)
+                db = dy[:, :out].float().sum(0).to(bp.dtype)
             ws = torch.empty(max(nb, 256), dtype=torch.uint8, device=dev)
             if need_x or need_w:
                 h.linear_act8_bwd(dy.data_ptr(), dy.stride(0), w.data_ptr(), w.stride(0), q.data_ptr(), s.data_ptr(),
                                   N.ptr(dx), acc is not None, N.ptr(dw), dw.stride(0) if need_w else K,
-                                  N.ptr(db) if need_w else 0, N.dtype_code(gdt), bool(direct), rows, K, out,
+                                  N.ptr(db) if need_w else 0, N.dtype_code(dw.dtype) if need_w else N.DT_F32,
+                                  N.dtype_code(db.dtype) if db is not None else N.DT_F32, bool(direct), rows, K, out,
                                   N.dtype_code(dt), gelu, N.ptr(amax), ws.data_ptr(), N.stream_of(dy))
         if direct:
             _ready(wp)
             if need_b:
                 _ready(bp)
             dw = db = None
-        if db is not None and db.dtype != bp.dtype:
-            db = db.to(bp.dtype)
         return dx, dw, db, None, None, None
 
 

@@ -8,7 +8,7 @@ those whose first-maximum class is the label, and their count, all device tensor
 hipGraph-capturable).
 
 * The forward keeps two numbers a row (largest logit, sum of exponentials); the backward computes the
-  logits again, piece by piece of the vocabulary, in a workspace of at most 256 MB (or one piece of 256
+  logits again, piece by piece of the vocabulary, in a workspace of at most 512 MB (or one piece of 256
   columns), and gives ``x``, ``weight`` and ``bias`` their gradients.  BERT-base's MLM head over 8192
   positions would keep 0.5 GB of bf16 logits and as much gradient.
 * A row whose label is ``ignore_index`` or lies outside [0, num_classes) is left out before any
@@ -60,7 +60,8 @@ def linear_cross_entropy_ref(x: torch.Tensor, weight: torch.Tensor, labels: torc
 
 def _rows16(w: torch.Tensor) -> torch.Tensor:
     """w with 16-byte rows of whole 16-byte vectors (bf16): w itself, or a zero-padded copy."""
-    if w.stride(1) == 1 and w.stride(0) % 8 == 0 and w.shape[1] % 8 == 0 and w.data_ptr() % 16 == 0:
+    ld = w.stride(0)
+    if w.stride(1) == 1 and ld % 8 == 0 and ld >= w.shape[1] and w.shape[1] % 8 == 0 and w.data_ptr() % 16 == 0:
         return w
     return F.pad(w, (0, -w.shape[1] % 8)).contiguous()
 
@@ -120,39 +121,32 @@ class _LinearXentFn(torch.autograd.Function):
         with _on(dev):
             p = keep.data_ptr()
             p = [p + a for a in ctx.at]
-            g = gloss  # fp32, as the loss is
             w = weight if f32 else _rows16(weight)
             if need_x:
                 dx = torch.empty(rows, K, dtype=ctx.x_dtype, device=dev)
             # into the optimizer's flat gradients where it owns every gradient that is asked for
-            direct = ((need_w or need_b) and (not need_w or _direct(wp)) and (not need_b or _direct(bp))
-                      and (not (need_w and need_b) or flat_grad(wp).dtype == flat_grad(bp).dtype))
-            if direct:
-                gdt = flat_grad(wp if need_w else bp).dtype
-                direct = gdt in (torch.float32, torch.bfloat16)
-            if not direct:
-                gdt = weight.dtype
+            direct = (need_w or need_b) and all(_direct(t) and flat_grad(t).dtype in (torch.float32, torch.bfloat16)
+                                                for t, need in ((wp, need_w), (bp, need_b)) if need)
             if need_w:
-                dw = flat_grad(wp) if direct else torch.empty(V, K, dtype=gdt, device=dev)
+                dw = flat_grad(wp) if direct else torch.empty(V, K, dtype=weight.dtype, device=dev)
             if need_b:
-                db = flat_grad(bp) if direct else torch.empty(V, dtype=gdt, device=dev)
+                db = flat_grad(bp) if direct else torch.empty(V, dtype=bp.dtype, device=dev)
             if not direct and C < V:
                 for t in (dw, db):
                     if t is not None:
                         t[C:].zero_()
             ws = torch.empty(max(ctx.nb, 256), dtype=torch.uint8, device=dev)
             N.hip().linear_xent_bwd(w.data_ptr(), w.stride(0), rows, K, C, V, N.dtype_code(ctx.x_dtype), ws.data_ptr(),
-                                    p[0], p[1], p[2], p[3], p[4], p[5], p[6], g.data_ptr(), N.ptr(dx),
-                                    N.ptr(dw), dw.stride(0) if dw is not None else K, N.ptr(db), N.dtype_code(gdt),
-                                    bool(direct), N.stream_of(weight))
+                                    p[0], p[1], p[2], p[3], p[4], p[5], p[6], gloss.data_ptr(), N.ptr(dx),
+                                    N.ptr(dw), dw.stride(0) if need_w else K, N.ptr(db),
+                                    N.dtype_code(dw.dtype) if need_w else N.DT_F32,
+                                    N.dtype_code(db.dtype) if need_b else N.DT_F32, bool(direct), N.stream_of(weight))
         if direct:
             if need_w:
                 _ready(wp)
             if need_b:
                 _ready(bp)
             dw = db = None
-        if db is not None and db.dtype != bp.dtype:
-            db = db.to(bp.dtype)
         return dx, dw, db, None, None, None
 
 
