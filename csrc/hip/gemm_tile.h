@@ -379,7 +379,8 @@ struct Emit {
   const uint8_t* q;         // e4m3 checkpoint [i][ldq] whose gelu' multiplies, or null
   const uint8_t* qs;        // its scales [i][ldq / 32]
   int64_t ldq;
-  // factors: f times I's and J's inverse plane scales times *gl / max(*gn, 1), each pointer or null
+  // factors: f times I's and J's inverse plane scales times *gl / max(*gn, 1), each pointer or null (fi
+  // only with fj)
   float f;
   const float* fi;
   const float* fj;
@@ -408,7 +409,7 @@ struct Emit {
   __device__ __forceinline__ void eight(const Once& o, int i, int j, float (&v)[8], bool keep = true) const {
     if (j >= nj) return;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = keep ? v[e] * o.a * o.b * o.c : 0.f;
+    for (int e = 0; e < 8; ++e) v[e] = !keep ? 0.f : fj ? v[e] * o.a * o.b * o.c : v[e] * o.a;
     if (q) {  // ldq % 32 == 0
       const uint2 u = *reinterpret_cast<const uint2*>(q + int64_t(i) * ldq + j);
       const float s = __uint_as_float(uint32_t(qs[int64_t(i) * (ldq >> 5) + (j >> 5)]) << 23);
