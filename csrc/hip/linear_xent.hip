@@ -346,8 +346,9 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
 
 // Joins the slots of ROWS rows a workgroup: 1024 / ROWS groups of ROWS threads each take every so-manieth
 // slot.  The last workgroup to finish adds the workgroups' sums up, in their order.  16 rows where
-// there are few (their slots are read by 64 groups at once), 64 otherwise (a fourth of the workgroups
-// for the count that finds the last one).
+// there are few (their slots are read by 64 groups at once: 20 rows of 469 slots 14.6 -> 5.8 us, 1280 of
+// 239 8.0 -> 7.1), 64 otherwise (a fourth of the workgroups for the count that finds the last one: 10240
+// rows of 118 slots 21.6 -> 10.9).
 constexpr int kJoinWaves = 16;
 template <int kJoinRows>
 __global__ __launch_bounds__(64 * kJoinWaves) void xent_join_kernel(const float2* __restrict__ part, int slots, int cap,
@@ -489,7 +490,9 @@ struct XentPlan {
 
 constexpr int64_t kGBytes = int64_t(512) << 20;  // G of one piece of the vocabulary
 constexpr int kTwoRows = 128;
-constexpr int kCountFrom = 4096;  // rows from which xent_count runs: 10240 rows gather in 6 + 3 us instead of 14
+// rows from which xent_count runs: the gather takes 6.2 / 9.2 / 15.9 / 42 us without it at 8192 / 16384 /
+// 32768 / 65536 rows of 64, 4.8 / 5.3 / 6.3 / 8.8 with it, and it takes 2.8 and a launch
+constexpr int kCountFrom = 12288;
 
 XentPlan xent_plan(int rows, int width, int classes, bool f32) {
   XentPlan q{};

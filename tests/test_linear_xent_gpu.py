@@ -203,7 +203,7 @@ def test_offsets_past_32_bits():
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("rows", [4096, 4097, 150000])
+@pytest.mark.parametrize("rows", [12288, 12289, 150000])
 def test_many_rows(rows, dtype):
     """Past the row count from which the labelled rows are counted beforehand."""
     x, w, b, y = _inputs(rows, 16, 50, 50, dtype, bias=True, ignored=0.5)
