@@ -7,7 +7,8 @@
 // Checkpoint: blocks of 32 features of one row, each e4m3 times the smallest power of two 2^e,
 // e >= -126, with the block's largest finite |x| <= 448 2^e.  The scaling is exact, so the one rounding
 // is e4m3's (at most 2^-4 of the value, or 2^(e-10) for the smallest); only what would round past fp32's
-// own range stays at 240 2^120, within 2^-4 too.  Infinite and NaN elements are held as NaN.  33 bytes for 32 features against 64 (bf16) or 128 (fp32).
+// own range stays at 240 2^120, within 2^-4 too.  Infinite and NaN elements are held as NaN.  33 bytes
+// for 32 features against 64 (bf16) or 128 (fp32).
 //
 //  * act8_pack reads x once and writes the checkpoint and, where the product cannot take x as it is,
 //    act(x) as the product's operand (bf16, or the two fp16 planes of fp32).  It moves 8 features a
@@ -258,8 +259,9 @@ Act8Plan act8_plan(int64_t rows, int64_t width, int64_t out, bool f32, bool copy
 void check_act8(int64_t rows, int64_t width, int64_t out, int dt) {
   VODA_CHECK(rows > 0 && rows < (1 << 30) && width > 0 && width <= (1 << 20) && out > 0 && out <= (1 << 20),
              "linear_act8: sizes out of range");
-  VODA_CHECK(up(rows, 32) / 32 * (up(width > out ? width : out, 128) / 128) < (int64_t(1) << 31) &&
-                 up(rows * up(width, 32), 256) / 256 < (int64_t(1) << 31),
+  // a launch holds less than 2^32 threads: 256 x 128 a workgroup of 256, eight features a thread of the packing
+  VODA_CHECK(up(rows, 128) / 128 * (up(width > out ? width : out, 256) / 256) < (1 << 24) &&
+                 rows * up(width, 32) <= (int64_t(1) << 34),
              "linear_act8: rows x features too large");
   VODA_CHECK(dt == kF32 || dt == kBF16, "linear_act8: fp32 or bf16");
 }
@@ -379,10 +381,11 @@ void linear_act8_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
 }
 
 // dx [rows][width] in x's type (added to when ``dx_add``); dw [out][ldd] in ``grad_dt`` and db [out] in
-// ``db_dt`` (added to when ``accumulate``); dx, db, or dw and db may be null.  dy: bf16 rows of whole 16-byte vectors.
+// ``db_dt`` (added to when ``accumulate``); dx, db, or dw and db may be null, and the checkpoint where
+// neither dw nor the GELU asks for it.  dy: bf16 rows of whole 16-byte vectors.
 void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintptr_t qp, uintptr_t qs, uintptr_t dx,
-                     bool dx_add, uintptr_t dw, int64_t ldd, uintptr_t db, int grad_dt, int db_dt, bool accumulate, int64_t rows,
-                     int64_t width, int64_t out, int dt, bool gelu, uintptr_t amax, uintptr_t ws, uintptr_t stream) {
+                     bool dx_add, uintptr_t dw, int64_t ldd, uintptr_t db, int grad_dt, int db_dt, bool accumulate,
+                     int64_t rows, int64_t width, int64_t out, int dt, bool gelu, uintptr_t amax, uintptr_t ws, uintptr_t stream) {
   check_act8(rows, width, out, dt);
   const bool f32 = dt == kF32;
   VODA_CHECK((grad_dt == kF32 || grad_dt == kBF16) && (db_dt == kF32 || db_dt == kBF16),
@@ -392,6 +395,7 @@ void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintpt
   VODA_CHECK(f32 || (dy % 16 == 0 && ldy % 8 == 0 && ldy >= up(out, 8)),
              "linear_act8: bf16 gradient rows must be 16-byte aligned and whole 16-byte vectors");
   VODA_CHECK(qp % 16 == 0 && ws % 256 == 0, "linear_act8: workspaces must be aligned");
+  VODA_CHECK((qp && qs) || (!dw && !gelu), "linear_act8: the backward needs the checkpoint");
   const Act8Plan q = act8_plan(rows, width, out, f32, true);
   hipStream_t st = as_stream(stream);
   uint8_t* base = reinterpret_cast<uint8_t*>(ws);
@@ -432,7 +436,7 @@ void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintpt
     a.e.nj = int(width);
     a.e.vec = whole_rows(dx, width, !f32);
     a.e.accumulate = dx_add;
-      if (gelu) {
+    if (gelu) {
       a.e.q = q8;
       a.e.qs = s8;
       a.e.ldq = q.kq;

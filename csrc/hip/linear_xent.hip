@@ -16,9 +16,10 @@
 // launches are sized for all rows and the workgroups behind n end at once).  An ignored row costs
 // nothing, its dx is exactly zero and nothing that it holds, NaN included, reaches any output.
 //
-// bf16 inputs: G is rounded once to bf16 (2^-9 of each element, random in sign, against the same
-// rounding of the sums to bf16 at the end); the one-hot part is subtracted before that rounding and
-// g/n multiplied after the sums.  fp32 inputs: two fp16 planes an operand (gemm_tile.h); G 2^15.
+// bf16 inputs: G is rounded once to bf16 for the two products (at most 2^-8 of each element, random in
+// sign, against the same rounding of the sums to bf16 at the end), up to 128 rows kept in two planes;
+// the one-hot part is subtracted before that rounding and g/n multiplied after the sums.  db sums G as it
+// was before.  fp32 inputs: two fp16 planes an operand (gemm_tile.h); G 2^15.
 // Sums over rows and splits have a fixed order: the same call gives the same bits.
 #include "gemm_tile.h"
 #include "ops.h"
@@ -552,7 +553,9 @@ void check_xent(int64_t rows, int64_t width, int64_t classes, int64_t vocab) {
   VODA_CHECK(rows > 0 && rows <= (1 << 24), "linear_xent: 1 to 2^24 rows");
   VODA_CHECK(width > 0 && width <= (1 << 20), "linear_xent: width 1 to 2^20");
   VODA_CHECK(classes > 0 && classes <= vocab && vocab <= (1 << 24), "linear_xent: 1 <= classes <= vocabulary <= 2^24");
-  VODA_CHECK(up(rows, 32) / 32 * (up(classes, 128) / 128) < (int64_t(1) << 31), "linear_xent: rows x vocabulary too large");
+  // a launch holds less than 2^32 threads: 256 x 128 a workgroup of 256, eight outputs a thread of the finish
+  VODA_CHECK(up(rows, 128) / 128 * (up(classes, 256) / 256) < (1 << 24), "linear_xent: rows x vocabulary too large");
+  VODA_CHECK(rows * up(width, 8) <= (int64_t(1) << 34), "linear_xent: rows x width too large");
 }
 
 }  // namespace

@@ -82,6 +82,22 @@ def test_what_is_kept():
         torch.testing.assert_close(layer(x), F.linear(F.gelu(x, approximate="tanh"), layer.weight, layer.bias))
 
 
+def test_a_frozen_weight_keeps_no_checkpoint():
+    """Without the GELU dx needs none; with it the slope does."""
+    g = torch.Generator().manual_seed(5)
+    for act, extra in ((None, 0), ("gelu", 64 * 256 + 64 * 8)):
+        x, layer = torch.randn(64, 256, generator=g).requires_grad_(), Act8Linear(256, 32, act=act)
+        layer.weight.requires_grad_(False)
+        dy, sizes = torch.randn(64, 32, generator=g), []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: sizes.append(t.numel() * t.element_size()) or t, lambda t: t):
+            y = layer(x)
+        assert sum(sizes) == layer.weight.numel() * 4 + extra
+        gx, gb = torch.autograd.grad(y, (x, layer.bias), dy)
+        layer.weight.requires_grad_(True)
+        wx, wb = torch.autograd.grad(layer(x), (x, layer.bias), dy)
+        assert torch.equal(gx, wx) and torch.equal(gb, wb)
+
+
 def test_shapes_and_empty():
     layer = Act8Linear(6, 3)
     assert layer(torch.zeros(2, 5, 6)).shape == (2, 5, 3)
@@ -121,7 +137,8 @@ def test_the_host_refuses():
     from vodascheduler_amd.ops import _native
 
     h = _native.hip()
-    for rows, K, N, dt in ((0, 8, 8, 0), (8, 0, 8, 0), (8, 8, 0, 0), (8, 8, 8, 2), (8, 1 << 21, 8, 0), (1 << 30, 8, 8, 0)):
+    for rows, K, N, dt in ((0, 8, 8, 0), (8, 0, 8, 0), (8, 8, 0, 0), (8, 8, 8, 2), (8, 1 << 21, 8, 0), (1 << 30, 8, 8, 0),
+                           (1 << 20, 1 << 15, 8, 1), (1 << 22, 8, 1 << 18, 1)):  # more than a launch's 2^32 threads
         with pytest.raises(ValueError):
             h.linear_act8_sizes(rows, K, N, dt, True)
     with pytest.raises(ValueError):  # bf16 rows off 16 bytes need the copy

@@ -117,6 +117,37 @@ def test_expanded_operands(dtype):
         assert all(torch.equal(g, r) for g, r in zip((y, *got), ref))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("act", [None, "gelu"])
+def test_single_rows_of_any_stride(dtype, act):
+    """A matrix of one row is contiguous whatever its row stride says."""
+    x, w, b, dy = _inputs(1, 64, 1, dtype, bias=True)
+    want = _check(x, w, b, dy, act)
+    turned = lambda t: t.detach().reshape(-1, 1).clone().t()  # noqa: E731
+    x1, w1 = turned(x), turned(w)
+    assert x1.stride() == (1, 1) and w1.is_contiguous()
+    for o, r in zip(_run(x1.requires_grad_(), w1.requires_grad_(), b, dy, act), want):
+        assert torch.equal(o, r)
+    x, w, b, dy = _inputs(1, 40, 48, dtype, bias=True)
+    want = _check(x, w, b, dy, act)
+    for o, r in zip(_run(x, w, b, turned(dy), act), want):
+        assert torch.equal(o, r)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("N", [72, 27])
+def test_a_frozen_weight(N, dtype):
+    """dx and db by themselves; db of the same sums in another order: each within (rows + 1) 2^-24 of the
+    sum of magnitudes, and a rounding to the type."""
+    x, w, b, dy = _inputs(300, 64, N, dtype, bias=True)
+    full = _check(x, w, b, dy, None)
+    y = linear_act8(x, w.detach(), b)
+    gx, gb = torch.autograd.grad(y, (x, b), dy)
+    assert torch.equal(gx, full[1])
+    err = (gb.double() - full[3].double()).abs()
+    assert (err <= 2 * 301 * 2.0 ** -24 * dy.double().abs().sum(0) + torch.finfo(dtype).eps * full[3].double().abs()).all()
+
+
 @pytest.mark.parametrize("rows", [20, 900])
 def test_bias_of_another_type(rows):
     x, w, b, dy = _inputs(rows, 72, 48, torch.bfloat16, bias=True)
@@ -220,6 +251,21 @@ def test_same_bits_every_time_and_on_another_stream():
                 got = _run(x, w, b, dy, "gelu")
             torch.cuda.synchronize()
             assert all(torch.equal(g, r) for g, r in zip(got, first))
+
+
+def test_two_streams_at_once():
+    ins = [_inputs(900, 200, 136, torch.float32, bias=True, seed=s) for s in (1, 2)]
+    want = [_check(*t, "gelu") for t in ins]
+    streams = [torch.cuda.Stream() for _ in ins]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(6):
+        for s, t, o in zip(streams, ins, got):
+            with torch.cuda.stream(s):
+                o.append(_run(*t, "gelu"))
+    torch.cuda.synchronize()
+    for o, r in zip(got, want):
+        assert all(torch.equal(p, q) for run in o for p, q in zip(run, r))
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])

@@ -101,12 +101,26 @@ def test_the_host_refuses_sizes_out_of_range():
 
     h = _native.hip()
     assert all(v > 0 for v in h.linear_xent_sizes(20, 256, 15000, 15000, False)[:2])
-    for rows, K, C, V in ((0, 8, 8, 8), (1 << 25, 8, 8, 8), (4, 0, 8, 8), (4, 8, 0, 8), (4, 8, 9, 8), (4, 8, 8, 1 << 25)):
+    for rows, K, C, V in ((0, 8, 8, 8), (1 << 25, 8, 8, 8), (4, 0, 8, 8), (4, 8, 0, 8), (4, 8, 9, 8), (4, 8, 8, 1 << 25),
+                          (1 << 24, 8, 1 << 16, 1 << 16), (1 << 22, 1 << 13, 8, 8)):  # more than a launch's 2^32 threads
         with pytest.raises(ValueError):
             h.linear_xent_sizes(rows, K, C, V, False)
     # bf16 weight rows that are no whole 16-byte vectors never reach a kernel
     with pytest.raises(ValueError):
         h.linear_xent_fwd(0, 8, 8, 8, 0, 0, 0, -100, 4, 8, 8, 8, 1, *([0] * 11), 0)
+
+
+def test_rows_of_whole_vectors():
+    """Any bf16 matrix becomes one whose rows the products can read, its values unchanged and zeros behind."""
+    from vodascheduler_amd.ops.linear_xent import _rows16
+
+    full = torch.arange(1.0, 5 * 41).bfloat16().reshape(4, 51)
+    line = torch.arange(1.0, 65).bfloat16()[:, None]
+    for t in (full, full[:, :48], full[:, 1:49], full.t(), full[:1].expand(4, 51), full[:1, :48].expand(4, 48),
+              line.t(), line[:61].t(), line, line[:1]):
+        r = _rows16(t)
+        assert r.stride(1) == 1 and r.shape[1] % 8 == 0 and r.stride(0) % 8 == 0 and r.stride(0) >= r.shape[1]
+        assert r.data_ptr() % 16 == 0 and torch.equal(r[:, :t.shape[1]], t) and not r[:, t.shape[1]:].any()
 
 
 def test_the_workspace_is_bounded():

@@ -283,6 +283,36 @@ def test_same_bits_every_time_and_on_another_stream():
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_single_rows_of_any_stride(dtype):
+    """A matrix of one row is contiguous whatever its row stride says."""
+    turned = lambda t: t.detach().reshape(-1, 1).clone().t().requires_grad_()  # noqa: E731
+    for V in (130, 1):
+        x, w, b, y = _inputs(1, 64, V, V, dtype, bias=True, ignored=0.0)
+        want = _check(x, w, b, y, V)
+        leaves = [turned(x), turned(w) if V == 1 else w, b]
+        assert leaves[0].stride() == (1, 1)
+        loss = linear_cross_entropy(leaves[0], leaves[1], y, b, V)[0]
+        assert torch.equal(loss, want[0])
+        assert all(torch.equal(g, r) for g, r in zip(torch.autograd.grad(loss, leaves), want[1]))
+
+
+def test_two_streams_at_once():
+    ins = [_inputs(700, 200, 1300, 1290, torch.float32, bias=True, seed=s) for s in (1, 2)]
+    want = [_check(*t, 1290) for t in ins]
+    streams = [torch.cuda.Stream() for _ in ins]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(6):
+        for s, (x, w, b, y), o in zip(streams, ins, got):
+            with torch.cuda.stream(s):
+                loss = linear_cross_entropy(x, w, y, b, 1290)[0]
+                o.append((loss.detach(), *torch.autograd.grad(loss, (x, w, b))))
+    torch.cuda.synchronize()
+    for o, r in zip(got, want):
+        assert all(torch.equal(p, q) for run in o for p, q in zip(run, (r[0], *r[1])))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_captured_and_replayed(dtype):
     """Two graphs of one program replayed in turn with eager work between, the number of labelled rows
     another each time."""

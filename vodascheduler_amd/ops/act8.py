@@ -12,11 +12,13 @@ BERT-base's FFN keeps 0.79 + 3.17 KB a token this way instead of 1.5 + 6 + 6 KB 
 
 ``act8_pack`` / ``act8_unpack`` are the checkpoint by itself: ``scale`` is the smallest power of two (at
 least 2^-126) that keeps the block's largest finite value within 448, so the only rounding is e4m3's
-and nothing saturates; infinities and NaN come back as NaN.
+(what would round past fp32's range stays at 240 2^120); infinities and NaN come back as NaN.
 
-Types: bf16 or fp32 ``x`` and ``weight`` alike (fp32 at fp32 accuracy), ``bias`` of either.  Any sizes and
-row strides.  Gradients that the fused optimizer owns go straight into its flat buffer (ops/dense.py's
-contract).  Only first derivatives.  ``Act8Linear`` is the layer, with ``FusedLinear``'s parameters.
+Types: bf16 or fp32 ``x`` and ``weight`` alike (fp32 at fp32 accuracy for finite inputs; an infinite one gives
+NaN or infinity where it takes part), ``bias`` of either.  Any sizes and row strides.  Gradients that the
+fused optimizer owns go straight into its flat buffer (ops/dense.py's contract).  Without a gradient of
+``weight`` and without the GELU no checkpoint is kept.  Only first derivatives.  ``Act8Linear`` is the
+layer, with ``FusedLinear``'s parameters.
 """
 from __future__ import annotations
 
@@ -26,7 +28,7 @@ from torch.autograd.function import once_differentiable
 
 from ..utils.flat import flat_grad
 from . import _native as N
-from .dense import FusedLinear, _direct, _ready
+from .dense import FusedLinear, _direct, _ready, colsum_accumulate_
 from .ffn import gelu_tanh_grad_ref
 from .linear_xent import _on, _rows16
 
@@ -112,7 +114,8 @@ class _LinearAct8Fn(torch.autograd.Function):
         ctx.params = (weight, bias)
         ctx.gelu, ctx.dims, ctx.x_dtype = gelu, (rows, K, out), x.dtype
         ctx.sink_in, ctx.bias_handoff = sink_in, bias_handoff
-        keep = any(ctx.needs_input_grad[:3])
+        # for dw, and for the GELU's slope in dx
+        keep = ctx.needs_input_grad[1] or gelu and ctx.needs_input_grad[0]
         if not x.is_cuda:
             wide = x.float()
             y = F.linear(F.gelu(wide, approximate="tanh") if gelu else wide, weight.float(),
@@ -161,7 +164,7 @@ class _LinearAct8Fn(torch.autograd.Function):
             acc = acc.reshape(rows, K).to(dt).contiguous()
         dx = dw = db = None
         if not dy.is_cuda:
-            c = _unpack_ref(q, s, K, torch.float32)
+            c = None if q is None else _unpack_ref(q, s, K, torch.float32)
             g = dy.float()
             if need_x:
                 dx = g @ weight.float()
@@ -191,10 +194,12 @@ class _LinearAct8Fn(torch.autograd.Function):
                 if need_b:
                     db = flat_grad(bp) if direct else torch.empty(out, dtype=bp.dtype, device=dev)
             elif need_b:
-                db = dy[:, :out].float().sum(0).to(bp.dtype)
+                db = torch.zeros(dy.shape[1], dtype=torch.float32, device=dev)
+                colsum_accumulate_(dy, db)
+                db = db[:out].to(bp.dtype)
             ws = torch.empty(max(nb, 256), dtype=torch.uint8, device=dev)
             if need_x or need_w:
-                h.linear_act8_bwd(dy.data_ptr(), dy.stride(0), w.data_ptr(), w.stride(0), q.data_ptr(), s.data_ptr(),
+                h.linear_act8_bwd(dy.data_ptr(), dy.stride(0), w.data_ptr(), w.stride(0), N.ptr(q), N.ptr(s),
                                   N.ptr(dx), acc is not None, N.ptr(dw), dw.stride(0) if need_w else K,
                                   N.ptr(db) if need_w else 0, N.dtype_code(dw.dtype) if need_w else N.DT_F32,
                                   N.dtype_code(db.dtype) if db is not None else N.DT_F32, bool(direct), rows, K, out,

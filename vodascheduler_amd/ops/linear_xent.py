@@ -63,7 +63,10 @@ def _rows16(w: torch.Tensor) -> torch.Tensor:
     ld = w.stride(0)
     if w.stride(1) == 1 and ld % 8 == 0 and ld >= w.shape[1] and w.shape[1] % 8 == 0 and w.data_ptr() % 16 == 0:
         return w
-    return F.pad(w, (0, -w.shape[1] % 8)).contiguous()
+    # (not F.pad: it keeps a single row's stride, whatever that is)
+    out = w.new_zeros(w.shape[0], -(-w.shape[1] // 8) * 8)
+    out[:, :w.shape[1]] = w
+    return out
 
 
 def _on(device: torch.device):
