@@ -163,7 +163,7 @@ def build(nodes: dict[int, dict], links: list[dict], source: str = "") -> Topolo
                 t.numa[idx[b]] = cpu_order[a]
     # the peers' xGMI links to each other are not visible from a 1-GPU container: a GPU that
     # reaches every other GPU directly implies the vendor's all-to-all mesh (MI355X UBB)
-    if order and any(sum(1 for (x, _y) in t.xgmi if x == i) == len(order) - 1 for i in range(len(order))):
+    if t.xgmi and any(sum(1 for (x, _y) in t.xgmi if x == i) == len(order) - 1 for i in range(len(order))):
         w = max(t.xgmi.values())
         bw = max(t.xgmi_bw_mbs.values()) if t.xgmi_bw_mbs else 0
         for i in range(len(order)):
