@@ -60,18 +60,24 @@ def linear_cross_entropy_ref(x: torch.Tensor, weight: torch.Tensor, labels: torc
 
 def _rows16(w: torch.Tensor) -> torch.Tensor:
     """w with 16-byte rows of whole 16-byte vectors (bf16): w itself, or a zero-padded copy."""
-    ld = w.stride(0)
-    if w.stride(1) == 1 and ld % 8 == 0 and ld >= w.shape[1] and w.shape[1] % 8 == 0 and w.data_ptr() % 16 == 0:
+    ld, step = w.stride()
+    width = w.shape[1]
+    if step == 1 and ld % 8 == 0 and ld >= width and width % 8 == 0 and w.data_ptr() % 16 == 0:
         return w
     # (not F.pad: it keeps a single row's stride, whatever that is)
-    out = w.new_zeros(w.shape[0], -(-w.shape[1] // 8) * 8)
-    out[:, :w.shape[1]] = w
+    out = w.new_zeros(w.shape[0], -(-width // 8) * 8)
+    out[:, :width] = w
     return out
 
 
+# torch's own accessor, where it has one: 0.5 us instead of 3.5 in a call whose whole forward takes 30
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_HERE = nullcontext()
+
+
 def _on(device: torch.device):
-    """Context with ``device`` current (nothing to do where it is already)."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    """Context with the GPU ``device`` current (nothing to do where it is already)."""
+    return _HERE if device.index == _current_device() else torch.cuda.device(device)
 
 
 class _LinearXentFn(torch.autograd.Function):
