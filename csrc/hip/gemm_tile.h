@@ -110,7 +110,10 @@ struct Stage {
   const uint16_t* src[kPer];
   int off[COL ? 2 * T : BK / 16];
 
-  static __device__ __forceinline__ int swz(int row) { return (row / (8 / (CPR < 8 ? CPR : 8))) & (CPR - 1); }
+  // The LDS serves 16 lanes of 16 bytes a clock, 256 bytes: the rows that share a place in 256 bytes
+  // differ in their swizzle among any 16 neighbouring rows
+  static_assert(CPR <= 16, "rows of at most 256 bytes");
+  static __device__ __forceinline__ int swz(int row) { return (row / (16 / CPR)) & (CPR - 1); }
 
   // place of this lane's chunk in wave-instruction q: its row / column and k inside the stage
   static __device__ __forceinline__ void place(int q, int lane, int& r, int& k) {

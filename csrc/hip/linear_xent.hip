@@ -34,6 +34,10 @@ namespace {
 using namespace gt;
 
 constexpr float kLog2e = 1.4426950408889634f;
+// bf16 inputs: exponents go as one fma, z log2(e) - c, c the row's constant, while the row's largest logit
+// is at most this; past it (masks of the type's lowest value alone in a row, infinities) c would leave
+// fp32's range, and (z - max) log2(e) is exact where z is the largest
+constexpr float kTame = 0x1p100f;
 constexpr int kGatherRows = 32;   // rows a gather workgroup
 constexpr float kGScale = 32768.f;  // G's planes hold G 2^15: |G| <= 1
 
@@ -197,7 +201,8 @@ struct LogitArgs {
   float2* part;
   float* zlab;
   int* tie;
-  // backward: (max, 1 / sum exp) of each row, G [rows][ldg] (fp32 inputs: two planes)
+  // backward: of each row (log2 of the sum of all exponentials, -1), or (max, 1 / sum exp past it);
+  // G [rows][ldg] (fp32 inputs: two planes)
   const float2* stat;
   uint16_t* G;
   int64_t ldg, gplane;
@@ -217,10 +222,19 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
   int ti, tj, s;
   tile_at(blockIdx.x, live, ni, p.tj, kGroup, ti, tj, s);
   const int i0 = ti * T::BI, j0 = p.v0 + tj * T::BJ;
+  const typename T::Where w;
+  // of this lane's rows, on their way while the products run
+  int lab[T::TI];
+  float2 stat[T::TI];
+#pragma unroll
+  for (int c = 0; c < T::TI; ++c) {
+    const int i = min(i0 + w.i(c), X.n - 1);
+    lab[c] = p.lab[i];
+    if constexpr (BWD) stat[c] = p.stat[i];
+  }
   f32x16 acc[T::TJ][T::TI];
   float unused[T::TI];
   T::template run<false>(smem, X, p.W, i0, j0, 0, p.width, acc, unused);
-  const typename T::Where w;
   float sx = 1.f, sw = 1.f;
   if constexpr (F16) {
     sx = p.dev->inv_x;
@@ -249,7 +263,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
     if constexpr (!BWD) {
       const int i = i0 + w.i(c);
       const bool live = i < X.n;
-      const int y = live ? p.lab[i] : -1;
+      const int y = live ? lab[c] : -1;
       float m = -INFINITY;
 #pragma unroll
       for (int a = 0; a < T::TJ; ++a)
@@ -258,10 +272,18 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
       m = fmaxf(m, __shfl_xor(m, 32, 64));
       const float ms = m == -INFINITY ? 0.f : m;  // all -inf: a sum of zeros
       float sum = 0.f;
+      if (!F16 && __all(fabsf(ms) <= kTame)) {
+        const float mc = ms * kLog2e;
 #pragma unroll
-      for (int a = 0; a < T::TJ; ++a)
+        for (int a = 0; a < T::TJ; ++a)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f((acc[a][c][r] - ms) * kLog2e);
+          for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[a][c][r], kLog2e, -mc));
+      } else {
+#pragma unroll
+        for (int a = 0; a < T::TJ; ++a)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f((acc[a][c][r] - ms) * kLog2e);
+      }
       sum += __shfl_xor(sum, 32, 64);
       const int slot = tj * T::WJ + w.wj;
       if (live && w.h == 0) p.part[int64_t(slot) * p.X.n + i] = make_float2(m, sum);
@@ -282,42 +304,61 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
         const float z2 = __shfl_xor(z, 32, 64);
         if (!has) z = z2;
         int t = 0;
+        if (__ballot(here && z == m)) {  // only then can the label be the row's first maximum
 #pragma unroll
-        for (int a = 0; a < T::TJ; ++a)
+          for (int a = 0; a < T::TJ; ++a)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) t |= int(j0 + w.j(a, r >> 2) + (r & 3) < y && acc[a][c][r] == z);
-        t |= __shfl_xor(t, 32, 64);
+            for (int r = 0; r < 16; ++r) t |= int(j0 + w.j(a, r >> 2) + (r & 3) < y && acc[a][c][r] == z);
+          t |= __shfl_xor(t, 32, 64);
+        }
         if (here && w.h == 0) {
           p.zlab[i] = z;
           p.tie[i] = t;
         }
       }
     } else {
-      float bias[8];
+      float bias[8];  // times log2(e) where the exponents are one fma
       bool have = false;
       through_lds<T>(smem, w, acc, c, [&](int r, int j, float(&v)[8]) {
+        const float sm = __shfl(stat[c].x, r & 31, 64), sy = __shfl(stat[c].y, r & 31, 64);
+        const int y = __shfl(lab[c], r & 31, 64) - (j0 + j);
         if (i0 + r >= X.n) return;
         if (!have) {  // a lane's columns stay the same
           const float* b = p.bias32 + j0 + j;
           const float4 x = *reinterpret_cast<const float4*>(b), y = *reinterpret_cast<const float4*>(b + 4);
           bias[0] = x.x; bias[1] = x.y; bias[2] = x.z; bias[3] = x.w;
           bias[4] = y.x; bias[5] = y.y; bias[6] = y.z; bias[7] = y.w;
+          if constexpr (!F16) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) bias[e] *= kLog2e;
+          }
           have = true;
         }
-        const float2 st = p.stat[i0 + r];
-        const int y = p.lab[i0 + r] - (j0 + j);
         uint16_t* g = p.G + int64_t(i0 + r) * p.ldg + (j0 - p.v0) + j;
+        float d[8];
+        if constexpr (F16) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[e] = __builtin_amdgcn_exp2f((v[e] * sx * sw + bias[e] - sm) * kLog2e) * sy;
+        } else if (sy < 0.f) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[e] = __builtin_amdgcn_exp2f(fmaf(v[e], kLog2e, bias[e] - sm));
+        } else {
+          const float* b = p.bias32 + j0 + j;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[e] = __builtin_amdgcn_exp2f((v[e] + b[e] - sm) * kLog2e) * sy;
+        }
+        if (__ballot(unsigned(y) < 8u)) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e == y) d[e] -= 1.f;
+        }
         uint16_t hi[8], lo[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          float z = v[e];
-          if constexpr (F16) z = z * sx * sw;
-          float d = __builtin_amdgcn_exp2f((z + bias[e] - st.x) * kLog2e) * st.y;
-          if (e == y) d -= 1.f;
-          sums[e] += d;
-          if constexpr (F16) split2(d * kGScale, hi[e], lo[e]);
-          else hi[e] = f2bf(d);
-          if constexpr (TWO && !F16) lo[e] = f2bf(d - bf2f(hi[e]));
+          sums[e] += d[e];
+          if constexpr (F16) split2(d[e] * kGScale, hi[e], lo[e]);
+          else hi[e] = f2bf(d[e]);
+          if constexpr (TWO && !F16) lo[e] = f2bf(d[e] - bf2f(hi[e]));
         }
         auto eight = [](const uint16_t(&a)[8]) {
           return make_uint4(a[0] | (uint32_t(a[1]) << 16), a[2] | (uint32_t(a[3]) << 16), a[4] | (uint32_t(a[5]) << 16),
@@ -356,7 +397,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void xent_join_kernel(const float2
                                                                     int slot_cols, const float* __restrict__ zlab,
                                                                     const int* __restrict__ tie,
                                                                     const int* __restrict__ lab, XentDev* dev,
-                                                                    float2* __restrict__ stat, double* __restrict__ lsum,
+                                                                    float2* __restrict__ stat, bool one,
+                                                                    double* __restrict__ lsum,
                                                                     int* __restrict__ csum, float* __restrict__ loss,
                                                                     int64_t* __restrict__ correct) {
   constexpr int kJoinGroups = 64 * kJoinWaves / kJoinRows, kQ = 64 / kJoinRows;
@@ -410,7 +452,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void xent_join_kernel(const float2
     int ok = 0;
     if (live && q == 0) {
       const float z = zlab[i];
-      stat[i] = make_float2(m, 1.f / s);
+      // past 2^100, infinite or NaN: the two numbers apart
+      stat[i] = one && fabsf(m) <= kTame ? make_float2(fmaf(m, kLog2e, log2f(s)), -1.f) : make_float2(m, 1.f / s);
       // (max - z) first: exact where the label's logit is the largest or near it
       l = double(m - z) + double(logf(s));
       ok = z == m && before < z && !tie[i] && s == s;
@@ -645,7 +688,7 @@ void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
   else launch_logits<false, false, false>(p, q.tile, st);
   auto join = [&](auto kernel, int per) {
     hipLaunchKernelGGL(kernel, dim3(unsigned((rows + per - 1) / per)), dim3(64 * kJoinWaves), 0, st, p.part, q.slots, int(rows),
-                       tile_slot(q.tile), p.zlab, p.tie, g.lab, d, reinterpret_cast<float2*>(stat),
+                       tile_slot(q.tile), p.zlab, p.tie, g.lab, d, reinterpret_cast<float2*>(stat), !f32,
                        reinterpret_cast<double*>(base + q.o_lsum), reinterpret_cast<int*>(base + q.o_csum),
                        reinterpret_cast<float*>(loss), reinterpret_cast<int64_t*>(correct));
   };
