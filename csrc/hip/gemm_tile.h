@@ -27,6 +27,7 @@
 #include "common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace voda {
 namespace gt {
@@ -133,8 +134,8 @@ struct Stage {
     for (int u = 0; u < kPer; ++u) {
       int r, k;
       place(wave * kPer + u, lane, r, k);
-      if constexpr (COL)  // a chunk of 8 columns past the end: zeros, never stored
-        src[u] = r0 + r < o.n ? o.p + int64_t(k0 + k) * o.ld + r0 + r : nullptr;
+      if constexpr (COL)  // chunks of 8 columns past the last one read that one, never stored
+        src[u] = o.p + int64_t(k0 + k) * o.ld + min(r0 + r, (o.n - 1) & ~7);
       else
         src[u] = o.p + int64_t(min(r0 + r, o.n - 1)) * o.ld + k0 + k;
     }
@@ -162,8 +163,7 @@ struct Stage {
     const int q = wave * kPer + u;
     int r, k;
     place(q, lane, r, k);
-    const bool ok = k < left && (!COL || src[u] != nullptr);
-    dma16(ok ? static_cast<const void*>(src[u] + shift) : zero_chunk,
+    dma16(k < left ? static_cast<const void*>(src[u] + shift) : zero_chunk,
           __builtin_amdgcn_readfirstlane(uint32_t(size_t((lds_void*)(lds + 1024 * q)))));
   }
 
@@ -230,13 +230,13 @@ struct Tile {
     const int total = NP * steps;
     const int64_t stepi = IT ? BK * I.ld : BK, stepj = JT ? BK * J.ld : BK;
     int at = 0, prod = 0;  // next stage to issue: its step and product
-    // instruction u of the next stage into ``lds``; stages past the last one read zeros
+    // instruction u of the next stage into ``lds``
     int64_t shi = 0, shj = 0;
     int left = 0;
     auto aim = [&] {
       const bool lo_i = NP == 3 ? prod == 1 : NP == 2 ? prod == 0 : false;
       const bool lo_j = NP == 3 && prod == 0;
-      left = prod < NP ? k1 - k0 - at * BK : 0;
+      left = k1 - k0 - at * BK;
       shi = at * stepi + (lo_i ? I.plane : 0);
       shj = at * stepj + (lo_j ? J.plane : 0);
       if (++at >= steps) { at = 0; ++prod; }
@@ -247,6 +247,7 @@ struct Tile {
     };
 #pragma unroll
     for (int s = 0; s < ST; ++s) {
+      if (s >= total) break;
       aim();
 #pragma unroll
       for (int u = 0; u < kPer; ++u) issue(u, smem + s * kStage);
@@ -259,11 +260,19 @@ struct Tile {
 #pragma unroll
       for (int a = 0; a < TJ; ++a) fj[set][a] = sj.frag(li + SI::kBytes, a, kk);
     };
-    wait_vm_barrier<(ST - 1) * kPer>();
+    // until at most n stages are on their way, then the barrier
+    auto wait_stages = [](int n) {
+      if (ST > 3 && n >= 3) wait_vm_barrier<(ST > 3 ? 3 * kPer : 0)>();
+      else if (ST > 2 && n >= 2) wait_vm_barrier<(ST > 2 ? 2 * kPer : 0)>();
+      else if (n >= 1) wait_vm_barrier<kPer>();
+      else wait_vm_barrier<0>();
+    };
+    wait_stages(total - 1);
     fetch(0, 0, 0);
-    int buf = 0;
+    int buf = 0, st = 0;
     constexpr int mf = TI * TJ;
-    for (int st = 0; st < total; ++st) {
+    // one stage; ``more``: a stage is left to issue into the buffer that it frees
+    auto stage = [&](auto more) {
       if (NP > 1 && F16 && st == (NP - 1) * steps) {
 #pragma unroll
         for (int a = 0; a < TJ; ++a)
@@ -277,9 +286,13 @@ struct Tile {
       for (int kk = 0; kk < BK / 16; ++kk) {
         const bool tail = kk + 1 == BK / 16;
         if (tail) {
-          wait_vm_barrier<(ST - 2) * kPer>();
-          aim();
-          fetch(next, 0, 0);
+          if constexpr (more.value) {
+            wait_vm_barrier<(ST - 2) * kPer>();
+            aim();
+          } else {
+            wait_stages(total - 2 - st);
+          }
+          fetch(next, 0, 0);  // past the last stage: never used
         }
         if constexpr (SUM) {
           // the reduction's sum of I: the hi plane in the last product, lo where it runs with J's hi
@@ -297,9 +310,11 @@ struct Tile {
           acc[x / TI][x % TI] = mfma<F16>(fj[kk & 1][x / TI], fi[kk & 1][x % TI], acc[x / TI][x % TI]);
           // between two products: a DMA instruction or two of the refill, or a fragment of the next step
           if (tail) {
-            constexpr int per = (kPer + mf - 1) / mf;
+            if constexpr (more.value) {
+              constexpr int per = (kPer + mf - 1) / mf;
 #pragma unroll
-            for (int y = x * per; y < (x + 1) * per && y < kPer; ++y) issue(y, smem + buf * kStage);
+              for (int y = x * per; y < (x + 1) * per && y < kPer; ++y) issue(y, smem + buf * kStage);
+            }
           } else {
             constexpr int nf = TI + TJ;
             const uint8_t* li = smem + buf * kStage;
@@ -314,7 +329,9 @@ struct Tile {
         }
       }
       buf = next;
-    }
+    };
+    for (; st + ST < total; ++st) stage(std::true_type{});
+    for (; st < total; ++st) stage(std::false_type{});
     wait_vm_barrier<0>();
   }
 };

@@ -223,14 +223,15 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
   tile_at(blockIdx.x, live, ni, p.tj, kGroup, ti, tj, s);
   const int i0 = ti * T::BI, j0 = p.v0 + tj * T::BJ;
   const typename T::Where w;
-  // of this lane's rows, on their way while the products run
+  // of this lane's rows, on their way while the products run (the forward, which needs the label alone,
+  // has no register for it)
   int lab[T::TI];
   float2 stat[T::TI];
 #pragma unroll
-  for (int c = 0; c < T::TI; ++c) {
+  for (int c = 0; c < (BWD ? T::TI : 0); ++c) {
     const int i = min(i0 + w.i(c), X.n - 1);
     lab[c] = p.lab[i];
-    if constexpr (BWD) stat[c] = p.stat[i];
+    stat[c] = p.stat[i];
   }
   f32x16 acc[T::TJ][T::TI];
   float unused[T::TI];
@@ -263,7 +264,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
     if constexpr (!BWD) {
       const int i = i0 + w.i(c);
       const bool live = i < X.n;
-      const int y = live ? lab[c] : -1;
+      const int y = live ? p.lab[i] : -1;
       float m = -INFINITY;
 #pragma unroll
       for (int a = 0; a < T::TJ; ++a)
