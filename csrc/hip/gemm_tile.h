@@ -425,14 +425,27 @@ struct Emit {
                                        : static_cast<const float*>(bias)[j + e];
     return o;
   }
+  // the checkpoint of columns j .. j+7 of row i
+  struct Check {
+    uint2 u;
+    uint32_t s;
+  };
+  __device__ __forceinline__ Check check(int i, int j) const {
+    Check c = {make_uint2(0, 0), 0};
+    if (q && j < nj) {  // ldq % 32 == 0
+      c.u = *reinterpret_cast<const uint2*>(q + int64_t(i) * ldq + j);
+      c.s = qs[int64_t(i) * (ldq >> 5) + (j >> 5)];
+    }
+    return c;
+  }
   // columns j .. j+7 of row i (j % 8 == 0); ``keep`` false: the row is zero whatever the factors are
-  __device__ __forceinline__ void eight(const Once& o, int i, int j, float (&v)[8], bool keep = true) const {
+  __device__ __forceinline__ void eight(const Once& o, const Check& c, int i, int j, float (&v)[8], bool keep = true) const {
     if (j >= nj) return;
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = !keep ? 0.f : fj ? v[e] * o.a * o.b * o.c : v[e] * o.a;
-    if (q) {  // ldq % 32 == 0
-      const uint2 u = *reinterpret_cast<const uint2*>(q + int64_t(i) * ldq + j);
-      const float s = __uint_as_float(uint32_t(qs[int64_t(i) * (ldq >> 5) + (j >> 5)]) << 23);
+    if (q) {
+      const uint2 u = c.u;
+      const float s = __uint_as_float(c.s << 23);
       v[0] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u.x, 0) * s);
       v[1] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u.x, 1) * s);
       v[2] *= gelu_tanh_grad(__builtin_amdgcn_cvt_f32_fp8(u.x, 2) * s);
@@ -578,7 +591,8 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm_kernel(GemmArgs p) {
   float isum[T::TI];
   T::template run<SUM>(smem, I, p.J, i0, j0, k0, k1, acc, isum, want);
   // through_lds gives a lane the same columns each time
-  const Emit::Once once = p.e.once(j0 + w.wj * T::TJ * 32 + 8 * (w.lane % (4 * T::TJ)));
+  const int once_j = j0 + w.wj * T::TJ * 32 + 8 * (w.lane % (4 * T::TJ));
+  const Emit::Once once = p.e.once(once_j);
   Emit o = p.e;
   if (p.slab) {
     o.out = p.slab + int64_t(s) * I.n * p.lds;
@@ -587,6 +601,10 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm_kernel(GemmArgs p) {
     o.vec = 1;
     o.accumulate = p.add;
   }
+  // a lane's rows, RP apart from one call to the next: each row's checkpoint is read a call ahead
+  constexpr int RP = 16 / T::TJ;
+  auto ahead = [&](int r) { return p.slab ? Emit::Check{} : p.e.check(min(i0 + r, I.n - 1), once_j); };
+  Emit::Check next = ahead(w.wi * T::TI * 32 + w.lane / (4 * T::TJ));
 #pragma unroll
   for (int b = 0; b < T::TI; ++b) {
     const int i = i0 + w.i(b);
@@ -600,9 +618,11 @@ __global__ __launch_bounds__(T::kThreads, 2) void gemm_kernel(GemmArgs p) {
       }
     }
     through_lds<T>(smem, w, acc, b, [&](int r, int c, float(&v)[8]) {
+      const Emit::Check now = next;
+      next = ahead(r + RP);
       if (i0 + r >= I.n) return;
       if (p.slab) o.put(i0 + r, j0 + c, v);
-      else o.eight(once, i0 + r, j0 + c, v);
+      else o.eight(once, now, i0 + r, j0 + c, v);
     });
   }
 }
@@ -656,7 +676,7 @@ static __global__ __launch_bounds__(256) void finish_kernel(FinishArgs p) {
     for (int o = 1; o < LANES; o <<= 1)
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += __shfl_xor(v[e], o, 64);
-    if (part == 0) p.g.e.eight(p.g.e.once(j), i, j, v, src >= 0);
+    if (part == 0) p.g.e.eight(p.g.e.once(j), p.g.e.check(i, j), i, j, v, src >= 0);
   } else if (p.c.part && t - n < p.c.n && part == 0) {
     const int i = int(t - n);
     const int parts = p.c.rows_dev ? (*p.c.rows_dev + p.c.bi - 1) / p.c.bi * p.c.per : p.c.parts;
