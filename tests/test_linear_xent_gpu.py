@@ -135,6 +135,40 @@ def test_a_label_that_is_masked_and_a_row_of_nothing_but_masks(rows):
     assert torch.isnan(linear_cross_entropy(x, w, y, b)[0])
 
 
+@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_every_class_at_the_lowest_value(dtype, rows):
+    """No logit differs from the mask: a uniform softmax, so G is 1/C less the label's one."""
+    C, K = 300, 48
+    x, w, b, y = _inputs(rows, K, C, C, dtype, bias=True, ignored=0.0)
+    with torch.no_grad():
+        b[:] = torch.finfo(dtype).min
+    loss, correct, n = linear_cross_entropy(x, w, y, b)
+    gx, gw, gb = torch.autograd.grad(loss, (x, w, b))
+    assert int(correct) == int((y == 0).sum()) and int(n) == rows
+    # log C of a sum of C ones, and the exponents' few units
+    assert abs(float(loss) - torch.tensor(float(C)).double().log().item()) < (C + 16) * 2.0 ** -24
+    G = (torch.full((rows, C), 1 / C, dtype=torch.float64, device=DEV) - torch.nn.functional.one_hot(y, C)) / rows
+    hold = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -20  # of G as an operand, and of the result
+    for g, l, r in ((gx, G, w), (gw, G.t(), x), (gb, G.t(), torch.ones(rows, 1, dtype=dtype, device=DEV))):
+        want, size = l @ r.double(), l.abs() @ r.double().abs()
+        assert ((g.double().reshape(want.shape) - want).abs() <= 2 * hold * size + (C + rows) * 2.0 ** -23 * size).all()
+
+
+def test_rows_past_fp32_s_ordinary_range_beside_others():
+    """Logits near 2^110 in some rows: one class takes all of their softmax; the rows between are as ever."""
+    x, w, b, y = _inputs(90, 48, 300, 300, torch.bfloat16, bias=True, ignored=0.0)
+    big = torch.arange(90, device=DEV) % 4 == 1
+    with torch.no_grad():
+        x[big] *= 2.0 ** 110
+    loss, grads = _check(x, w, b, y, 300)
+    assert all(torch.isfinite(t).all() for t in (loss, *grads))
+    top = (x[big].double() @ w.double().t()).argmax(1)
+    W = w.detach().double()
+    want, size = (W[top] - W[y[big]]) / 90, (W[top].abs() + W[y[big]].abs()) / 90
+    assert ((grads[0][big].double() - want).abs() <= 2.0 ** -7 * size).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("what", ["x", "w"])
 def test_non_finite_inputs_reach_the_loss(what, dtype):
