@@ -7,7 +7,7 @@ It returns the same ``(loss, correct, n_valid)``: the mean loss over the labelle
 those whose first-maximum class is the label, and their count, all device tensors (no host sync,
 hipGraph-capturable).
 
-* The forward keeps two numbers a row (largest logit, sum of exponentials); the backward computes the
+* The forward keeps two numbers a row (for the sum of its exponentials); the backward computes the
   logits again, piece by piece of the vocabulary, in a workspace of at most 512 MB (or one piece of 256
   columns), and gives ``x``, ``weight`` and ``bias`` their gradients.  BERT-base's MLM head over 8192
   positions would keep 0.5 GB of bf16 logits and as much gradient.
