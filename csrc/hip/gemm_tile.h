@@ -846,6 +846,13 @@ inline int choose_tile(int64_t ni, int64_t nj, int64_t nk, int np, bool col_i, b
   // over a long reduction); over a short one kWide's epilogue, which nothing hides, costs more than that
   if (w >= 192 && nk * np >= 1536 && (w + 255) / 256 * 10 <= (b + 255) / 256 * 6) return kWide;
   if (b >= 256) return kBig;
+  // a split reduction fills the chip with the largest tile too, at twice kSq's slabs: with 1820 to 3456 steps
+  // a split it won ([8704 x 15000]^T . [8704 x 256] in bf16 and qkv's gradients in fp32, 448 -> 438 and 411 ->
+  // 401 us a pass), with 900 to 1150 it lost (qkv's in bf16, 164 -> 172)
+  if (split) {
+    const int64_t s = split_of(kWide).of(w, nk);
+    if (w * s >= 192 && nk / s * np >= 1536) return kWide;
+  }
   return q * (split ? split_of(kSq).of(q, nk) : 1) > 256 ? kSq : kDeep;
 }
 
