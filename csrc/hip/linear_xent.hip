@@ -33,11 +33,11 @@ namespace {
 
 using namespace gt;
 
+// Exponents go as (z - max) log2(e): 0 where z is the largest, whatever its size, and the subtraction is
+// exact near it.  One fma, z log2(e) - c with c = max log2(e), would save an instruction an element and 2 % of
+// a pass, but c's own rounding, |c| 2^-24, would be in every exponent: a sum that misses 1, a negative loss
+// from |max| near 30 on, and infinite sums of a slot whose classes are masked by -1e10.
 constexpr float kLog2e = 1.4426950408889634f;
-// bf16 inputs: exponents go as one fma, z log2(e) - c, c the row's constant, while the row's largest logit
-// is at most this; past it (masks of the type's lowest value alone in a row, infinities) c would leave
-// fp32's range, and (z - max) log2(e) is exact where z is the largest
-constexpr float kTame = 0x1p100f;
 constexpr int kGatherRows = 32;   // rows a gather workgroup
 constexpr float kGScale = 32768.f;  // G's planes hold G 2^15: |G| <= 1
 
@@ -201,8 +201,7 @@ struct LogitArgs {
   float2* part;
   float* zlab;
   int* tie;
-  // backward: of each row (log2 of the sum of all exponentials, -1), or (max, 1 / sum exp past it);
-  // G [rows][ldg] (fp32 inputs: two planes)
+  // backward: (max, 1 / sum exp) of each row; G [rows][ldg] (fp32 inputs: two planes)
   const float2* stat;
   uint16_t* G;
   int64_t ldg, gplane;
@@ -273,18 +272,10 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
       m = fmaxf(m, __shfl_xor(m, 32, 64));
       const float ms = m == -INFINITY ? 0.f : m;  // all -inf: a sum of zeros
       float sum = 0.f;
-      if (!F16 && __all(fabsf(ms) <= kTame)) {
-        const float mc = ms * kLog2e;
 #pragma unroll
-        for (int a = 0; a < T::TJ; ++a)
+      for (int a = 0; a < T::TJ; ++a)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[a][c][r], kLog2e, -mc));
-      } else {
-#pragma unroll
-        for (int a = 0; a < T::TJ; ++a)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f((acc[a][c][r] - ms) * kLog2e);
-      }
+        for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f((acc[a][c][r] - ms) * kLog2e);
       sum += __shfl_xor(sum, 32, 64);
       const int slot = tj * T::WJ + w.wj;
       if (live && w.h == 0) p.part[int64_t(slot) * p.X.n + i] = make_float2(m, sum);
@@ -318,7 +309,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
         }
       }
     } else {
-      float bias[8];  // times log2(e) where the exponents are one fma
+      float bias[8];
       bool have = false;
       through_lds<T>(smem, w, acc, c, [&](int r, int j, float(&v)[8]) {
         const float sm = __shfl(stat[c].x, r & 31, 64), sy = __shfl(stat[c].y, r & 31, 64);
@@ -329,24 +320,14 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
           const float4 x = *reinterpret_cast<const float4*>(b), y = *reinterpret_cast<const float4*>(b + 4);
           bias[0] = x.x; bias[1] = x.y; bias[2] = x.z; bias[3] = x.w;
           bias[4] = y.x; bias[5] = y.y; bias[6] = y.z; bias[7] = y.w;
-          if constexpr (!F16) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) bias[e] *= kLog2e;
-          }
           have = true;
         }
         uint16_t* g = p.G + int64_t(i0 + r) * p.ldg + (j0 - p.v0) + j;
         float d[8];
-        if constexpr (F16) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) d[e] = __builtin_amdgcn_exp2f((v[e] * sx * sw + bias[e] - sm) * kLog2e) * sy;
-        } else if (sy < 0.f) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) d[e] = __builtin_amdgcn_exp2f(fmaf(v[e], kLog2e, bias[e] - sm));
-        } else {
-          const float* b = p.bias32 + j0 + j;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) d[e] = __builtin_amdgcn_exp2f((v[e] + b[e] - sm) * kLog2e) * sy;
+        for (int e = 0; e < 8; ++e) {
+          if constexpr (F16) v[e] = v[e] * sx * sw;
+          d[e] = __builtin_amdgcn_exp2f((v[e] + bias[e] - sm) * kLog2e) * sy;
         }
         if (__ballot(unsigned(y) < 8u)) {
 #pragma unroll
@@ -398,7 +379,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void xent_join_kernel(const float2
                                                                     int slot_cols, const float* __restrict__ zlab,
                                                                     const int* __restrict__ tie,
                                                                     const int* __restrict__ lab, XentDev* dev,
-                                                                    float2* __restrict__ stat, bool one,
+                                                                    float2* __restrict__ stat,
                                                                     double* __restrict__ lsum,
                                                                     int* __restrict__ csum, float* __restrict__ loss,
                                                                     int64_t* __restrict__ correct) {
@@ -453,8 +434,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void xent_join_kernel(const float2
     int ok = 0;
     if (live && q == 0) {
       const float z = zlab[i];
-      // past 2^100, infinite or NaN: the two numbers apart
-      stat[i] = one && fabsf(m) <= kTame ? make_float2(fmaf(m, kLog2e, log2f(s)), -1.f) : make_float2(m, 1.f / s);
+      stat[i] = make_float2(m, 1.f / s);
       // (max - z) first: exact where the label's logit is the largest or near it
       l = double(m - z) + double(logf(s));
       ok = z == m && before < z && !tie[i] && s == s;
@@ -689,7 +669,7 @@ void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
   else launch_logits<false, false, false>(p, q.tile, st);
   auto join = [&](auto kernel, int per) {
     hipLaunchKernelGGL(kernel, dim3(unsigned((rows + per - 1) / per)), dim3(64 * kJoinWaves), 0, st, p.part, q.slots, int(rows),
-                       tile_slot(q.tile), p.zlab, p.tie, g.lab, d, reinterpret_cast<float2*>(stat), !f32,
+                       tile_slot(q.tile), p.zlab, p.tie, g.lab, d, reinterpret_cast<float2*>(stat),
                        reinterpret_cast<double*>(base + q.o_lsum), reinterpret_cast<int*>(base + q.o_csum),
                        reinterpret_cast<float*>(loss), reinterpret_cast<int64_t*>(correct));
   };

@@ -1,0 +1,97 @@
+"""ops/linear_xent.py over the whole range of logits: classes masked by any finite value, rows whose logits
+are large. Beside the formulas' bounds (tests/xent_bounds.py), cases whose logits are exact products, so
+that the softmax is known to the last few bits."""
+import math
+
+import pytest
+import torch
+
+from vodascheduler_amd.ops.linear_xent import linear_cross_entropy
+
+from test_linear_xent_gpu import _check, _inputs
+from xent_bounds import U
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda", 0)
+TYPES = [torch.bfloat16, torch.float32]
+
+
+@pytest.mark.parametrize("rows", [3, 40, 300])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mask", [-1e4, -1.3e6, -1e9, -1e10, -1e20, -1e30])
+def test_classes_masked_by_a_finite_bias(mask, dtype, rows):
+    """Whole slots of classes at any low value take no part, and leave the others as they are."""
+    x, w, b, y = _inputs(rows, 48, 700, 700, dtype, bias=True)
+    y = torch.where(y >= 0, y % 10 + 600, y)
+    with torch.no_grad():
+        b[:400] = mask
+    loss, grads = _check(x, w, b, y, 700)
+    assert torch.isfinite(loss) and float(grads[1][:400].float().abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("value", [-1e4, 1.3e6, -1.1e9, 1e10, -1e20, 1e30])
+def test_every_class_at_one_value(value, dtype, rows):
+    """w = 0: every logit is the bias, whatever its size, so the softmax is uniform."""
+    C, K = 300, 48
+    x, _, _, y = _inputs(rows, K, C, C, dtype, bias=False, ignored=0.0)
+    w = torch.zeros(C, K, dtype=dtype, device=DEV, requires_grad=True)
+    b = torch.full((C,), value, dtype=dtype, device=DEV, requires_grad=True)
+    loss, correct, n = linear_cross_entropy(x, w, y, b)
+    gx, gw, gb = torch.autograd.grad(loss, (x, w, b))
+    assert int(correct) == int((y == 0).sum()) and int(n) == rows
+    # log C of a sum of C ones, to the few units of the logarithm and the result
+    assert abs(float(loss) - math.log(C)) <= 8 * U * math.log(C)
+    G = (torch.full((rows, C), 1 / C, dtype=torch.float64, device=DEV) - torch.nn.functional.one_hot(y, C)) / rows
+    # G is 1 / C (the reciprocal's two units) less one, held as an operand; then sums of rows and a rounding
+    hold = 2.0 ** -8 if dtype == torch.bfloat16 else 4 * U
+    half = torch.finfo(dtype).eps / 2
+    assert float(gx.float().abs().max()) == 0.0
+    for g, r in ((gw, x.double()), (gb, torch.ones(rows, 1, dtype=torch.float64, device=DEV))):
+        want, size = G.t() @ r, G.abs().t() @ r.abs()
+        assert ((g.double().reshape(want.shape) - want).abs() <= (hold + (rows + 8) * U) * size + half * want.abs()).all()
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("top", [30.25, 1000.0, 1.3e6, 1.1e9, 1e10, 1e20, 1e29])
+def test_rows_of_large_logits(top, dtype, rows):
+    """Logits top, 0 and -top, each one product of one term and so exact: a row with its label alone at the
+    top has loss 0 and no gradient, one that shares the top with another class log 2 and a half each."""
+    C, K = 300, 16
+    x = torch.zeros(rows, K, device=DEV)
+    at = torch.tensor(top).to(dtype).item()
+    x[:, 0], x[:, 1] = at, at
+    w = torch.zeros(C, K, device=DEV)
+    w[7, 0], w[100:, 0] = 1, -1
+    x, w = x.to(dtype).requires_grad_(), w.to(dtype).requires_grad_()
+    y = torch.full((rows,), 7, device=DEV)
+    tail = 99 * math.exp(-at) + 200 * math.exp(-2 * at)  # of the classes below; 1e-12 at 30
+    loss, correct, _ = linear_cross_entropy(x, w, y)
+    gx, gw = torch.autograd.grad(loss, (x, w))
+    assert 0.0 <= float(loss) <= 2 * tail + 1e-30 and int(correct) == rows
+    # dw: the softmax (below tail) times at, over the rows' mean
+    assert float(gw.double().abs().max()) <= 4 * tail * at + 1e-30 and float(gx.double().abs().max()) <= 4 * tail + 1e-30
+    with torch.no_grad():
+        w[200, 0] = 1
+    loss, correct, _ = linear_cross_entropy(x, w, y)
+    gx, gw = torch.autograd.grad(loss, (x, w))
+    assert abs(float(loss) - math.log(2)) <= 4 * U + tail and int(correct) == rows
+    want = torch.zeros(C, K, dtype=torch.float64, device=DEV)
+    want[7, :2], want[200, :2] = -at / 2, at / 2
+    # the halves are exact; the mean's factor, the sums over rows and the result's rounding are not
+    off = torch.finfo(dtype).eps / 2 + (rows + 8) * U
+    assert ((gw.double() - want).abs() <= off * want.abs() + 4 * tail * at + 1e-30).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_confident_row_s_loss_is_not_negative(dtype):
+    """The sum of exponentials holds the largest one's, exactly 1."""
+    for seed in range(24):
+        x, w, _, _ = _inputs(1, 64, 300, 300, dtype, bias=False, seed=seed, ignored=0.0)
+        with torch.no_grad():
+            x *= 2.0 ** (seed // 2)
+        y = (x.float() @ w.float().t()).argmax(1)
+        assert float(linear_cross_entropy(x, w, y)[0]) >= 0.0
