@@ -11,13 +11,13 @@
 // for 32 features against 64 (bf16) or 128 (fp32).
 //
 //  * act8_pack reads x once and writes the checkpoint and, where the product cannot take x as it is,
-//    act(x) as the product's operand (bf16, or the two fp16 planes of fp32).  It moves 8 features a
+//    act(x) as the product's operand (bf16, or the three planes of fp32).  It moves 8 features a
 //    thread; a block's maximum is two shuffles inside a quad of lanes.
 //  * act8_unpack writes act(c) for dw's product: the GELU is then computed once an element, not once
 //    for each of dw's row tiles.  bf16 holds an identity c exactly (four significant bits).
 //  * The three products are gemm_tile.h's; gelu'(c) is applied in dx's epilogue from the checkpoint.
-//    fp32: x, w and dy as two fp16 planes, three 16-bit products; an identity c fits one plane, so
-//    its dw takes two.
+//    fp32: x, w and dy as three bf16 planes, six 16-bit products; an identity c is exact in one plane, so
+//    its dw takes three.
 #include "gemm_tile.h"
 #include "ops.h"
 
@@ -34,10 +34,8 @@ struct PackArgs {
   uint8_t* q;       // [rows][kq], kq = width up to whole blocks of 32; null: no checkpoint
   uint8_t* qs;      // [rows][kq / 32]
   int kq;
-  uint16_t* o;      // act(x): [rows][kq] bf16, or two fp16 planes; or null
+  uint16_t* o;      // act(x): [rows][kq] bf16, or three planes; or null
   int64_t plane;
-  const float* amax;
-  float* inv;
 };
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.4028235e38f; }
@@ -77,29 +75,22 @@ __device__ __forceinline__ uint4 pack8_bf16(const float (&v)[8]) {
   return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
-// planes of 8 values; ``lo`` may be null (one plane)
-__device__ __forceinline__ void store8_planes(const float (&v)[8], float s, uint16_t* hi, uint16_t* lo) {
-  uint16_t h[8], l[8];
+// the three planes of 8 values
+__device__ __forceinline__ void store8_planes(const float (&v)[8], uint16_t* o, int64_t plane) {
+  uint16_t q[3][8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) split_safe(v[e], s, h[e], l[e]);
-  auto quad = [](const uint16_t* a) {
-    return make_uint4(a[0] | (uint32_t(a[1]) << 16), a[2] | (uint32_t(a[3]) << 16), a[4] | (uint32_t(a[5]) << 16),
-                      a[6] | (uint32_t(a[7]) << 16));
-  };
-  *reinterpret_cast<uint4*>(hi) = quad(h);
-  if (lo) *reinterpret_cast<uint4*>(lo) = quad(l);
+  for (int e = 0; e < 8; ++e) split3(v[e], q[0][e], q[1][e], q[2][e]);
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const uint16_t* a = q[k];
+    *reinterpret_cast<uint4*>(o + k * plane) =
+        make_uint4(a[0] | (uint32_t(a[1]) << 16), a[2] | (uint32_t(a[3]) << 16), a[4] | (uint32_t(a[5]) << 16),
+                   a[6] | (uint32_t(a[7]) << 16));
+  }
 }
 
 template <bool F32>
 __global__ __launch_bounds__(256) void act8_pack_kernel(PackArgs p) {
-  __shared__ float lds[4];
-  float scale = 1.f;
-  if constexpr (F32) {
-    if (p.o) {  // |gelu(x)| <= |x|: x's scale serves act(x)
-      scale = split_scale(amax_of(p.amax, lds));
-      if (blockIdx.x == 0 && threadIdx.x == 0) *p.inv = pow2_inverse(scale);
-    }
-  }
   const int eights = p.kq >> 3;  // a multiple of 4: a quad of lanes is one block of 32
   const int64_t n = int64_t(p.rows) * eights;
   const int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x;
@@ -135,7 +126,7 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(PackArgs p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = gelu_tanh_f(v[e]);
   }
-  if constexpr (F32) store8_planes(v, scale, p.o + 8 * t, p.o + p.plane + 8 * t);
+  if constexpr (F32) store8_planes(v, p.o + 8 * t, p.plane);
   else *reinterpret_cast<uint4*>(p.o + 8 * t) = pack8_bf16(v);
 }
 
@@ -143,11 +134,9 @@ struct UnpackArgs {
   const uint8_t* q;
   const uint8_t* qs;
   int64_t n;       // groups of 8
-  int gelu, planes;
-  uint16_t* o;     // act(c): bf16, or one or two fp16 planes
+  int gelu;
+  uint16_t* o;     // act(c): bf16, or (fp32 with the GELU) three planes
   int64_t plane;
-  const float* amax;
-  float* inv;
 };
 
 __device__ __forceinline__ void unpack8(const uint8_t* q, const uint8_t* qs, int64_t t, float (&v)[8]) {
@@ -163,14 +152,8 @@ __device__ __forceinline__ void unpack8(const uint8_t* q, const uint8_t* qs, int
   v[7] = __builtin_amdgcn_cvt_f32_fp8(u.y, 3) * s;
 }
 
-template <bool F32>
+template <bool PLANES>
 __global__ __launch_bounds__(256) void act8_unpack_kernel(UnpackArgs p) {
-  __shared__ float lds[4];
-  float scale = 1.f;
-  if constexpr (F32) {
-    scale = split_scale(amax_of(p.amax, lds));
-    if (blockIdx.x == 0 && threadIdx.x == 0) *p.inv = pow2_inverse(scale);
-  }
   const int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (t >= p.n) return;
   float v[8];
@@ -179,7 +162,7 @@ __global__ __launch_bounds__(256) void act8_unpack_kernel(UnpackArgs p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = gelu_tanh_f(v[e]);
   }
-  if constexpr (F32) store8_planes(v, scale, p.o + 8 * t, p.planes == 2 ? p.o + p.plane + 8 * t : nullptr);
+  if constexpr (PLANES) store8_planes(v, p.o + 8 * t, p.plane);
   else *reinterpret_cast<uint4*>(p.o + 8 * t) = pack8_bf16(v);
 }
 
@@ -210,22 +193,22 @@ struct Act8Plan {
   Split y_split, dx_split, dw_split;
   int y_s, dx_s, dw_s;
   bool copy;                     // the forward's product reads a copy that act8_pack writes
-  // forward workspace: planes' inverse scales, x's operand, w's planes, slab
-  int64_t f_inv, f_x, f_w, f_slab, fwd;
-  // backward workspace: dy's maxima, inverse scales, dy's planes, w's planes, act(c), slabs
-  int64_t b_amax, b_inv, b_dy, b_w, b_c, b_dx, b_dw, b_db, bwd;
+  // forward workspace: x's operand, slab
+  int64_t f_x, f_slab, fwd;
+  // backward workspace: dy's planes, act(c), slabs
+  int64_t b_dy, b_c, b_dx, b_dw, b_db, bwd;
 };
 
-Act8Plan act8_plan(int64_t rows, int64_t width, int64_t out, bool f32, bool copy) {
+Act8Plan act8_plan(int64_t rows, int64_t width, int64_t out, bool f32, bool gelu, bool copy) {
   Act8Plan q{};
   q.kq = int(up(width, 32));
   q.kp = int(up(width, 8));
   q.np8 = int(up(out, 8));
   q.copy = copy;
-  const int np = f32 ? 3 : 1;
+  const int np = f32 ? 6 : 1;
   q.y_tile = choose_tile(rows, out, width, np, false, true);
   q.dx_tile = choose_tile(rows, width, out, np, false, true);
-  q.dw_tile = choose_tile(out, width, rows, np, true, true);
+  q.dw_tile = choose_tile(out, width, rows, f32 && !gelu ? 3 : np, true, true);
   q.y_split = split_of(q.y_tile);
   q.dx_split = split_of(q.dx_tile);
   q.dw_split = split_of(q.dw_tile);
@@ -238,17 +221,12 @@ Act8Plan act8_plan(int64_t rows, int64_t width, int64_t out, bool f32, bool copy
     at = up(at + bytes, 256);
     return o;
   };
-  q.f_inv = take(f32 ? 16 : 0);
-  q.f_x = take(copy ? rows * q.kq * (f32 ? 4 : 2) : 0);
-  q.f_w = take(f32 ? out * q.kp * 4 : 0);
+  q.f_x = take(copy ? rows * q.kq * (f32 ? 6 : 2) : 0);
   q.f_slab = take(q.y_s > 1 ? q.y_s * rows * up(out, 8) * 4 : 0);
   q.fwd = at;
   at = 0;
-  q.b_amax = take(f32 ? kAmaxBlocks * 4 : 0);
-  q.b_inv = take(f32 ? 16 : 0);
-  q.b_dy = take(f32 ? rows * q.np8 * 4 : 0);
-  q.b_w = take(f32 ? out * q.kp * 4 : 0);
-  q.b_c = take(rows * q.kq * (f32 ? 4 : 2));
+  q.b_dy = take(f32 ? rows * q.np8 * 6 : 0);
+  q.b_c = take(rows * q.kq * (f32 && gelu ? 6 : 2));
   q.b_dx = take(q.dx_s > 1 ? q.dx_s * rows * q.kp * 4 : 0);
   q.b_dw = take(q.dw_s > 1 ? q.dw_s * out * q.kp * 4 : 0);
   q.b_db = take(q.dw_s > 1 ? q.dw_s * out * 4 : 0);
@@ -269,9 +247,9 @@ void check_act8(int64_t rows, int64_t width, int64_t out, int dt) {
 }  // namespace
 
 // (forward workspace, backward workspace) bytes, features up to 32, outputs up to 8
-std::vector<int64_t> linear_act8_sizes(int64_t rows, int64_t width, int64_t out, int dt, bool copy) {
+std::vector<int64_t> linear_act8_sizes(int64_t rows, int64_t width, int64_t out, int dt, bool copy, bool gelu) {
   check_act8(rows, width, out, dt);
-  const Act8Plan q = act8_plan(rows, width, out, dt == kF32, copy);
+  const Act8Plan q = act8_plan(rows, width, out, dt == kF32, gelu, copy);
   return {q.fwd, q.bwd, q.kq, q.np8};
 }
 
@@ -310,25 +288,21 @@ void act8_values(uintptr_t qp, uintptr_t qs, int64_t rows, int64_t width, int dt
   check_launch();
 }
 
-// y [rows][out] contiguous; the checkpoint (q, qs) is written where q is not null; ``amax`` (fp32):
-// 2 kAmaxBlocks floats, kept for the backward.
+// y [rows][out] contiguous; the checkpoint (q, qs) is written where q is not null; ``wp`` (fp32):
+// workspace for w's planes, [3][out][width up to 8].
 void linear_act8_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr_t bias, int bias_dt, uintptr_t y,
                      uintptr_t qp, uintptr_t qs, int64_t rows, int64_t width, int64_t out, int dt, bool gelu, bool copy,
-                     uintptr_t amax, uintptr_t ws, uintptr_t stream) {
+                     uintptr_t wp, uintptr_t ws, uintptr_t stream) {
   check_act8(rows, width, out, dt);
   const bool f32 = dt == kF32;
   VODA_CHECK(f32 || (w % 16 == 0 && ldw % 8 == 0 && ldw >= up(width, 8)),
              "linear_act8: bf16 weight rows must be 16-byte aligned and whole 16-byte vectors");
   VODA_CHECK(copy || (!f32 && !gelu && x % 16 == 0 && ldx % 8 == 0 && width % 8 == 0),
              "linear_act8: this input needs a copy");
-  VODA_CHECK(qp % 16 == 0 && ws % 256 == 0, "linear_act8: workspaces must be aligned");
-  const Act8Plan q = act8_plan(rows, width, out, f32, copy);
+  VODA_CHECK(qp % 16 == 0 && ws % 256 == 0 && wp % 16 == 0 && (wp || !f32), "linear_act8: workspaces must be aligned");
+  const Act8Plan q = act8_plan(rows, width, out, f32, gelu, copy);
   hipStream_t st = as_stream(stream);
   uint8_t* base = reinterpret_cast<uint8_t*>(ws);
-  float* inv = reinterpret_cast<float*>(base + q.f_inv);
-  float* am = reinterpret_cast<float*>(amax);
-  const Rows rw = {reinterpret_cast<const float*>(w), ldw, int(out), int(width)};
-  if (f32) gt::amax({reinterpret_cast<const float*>(x), ldx, int(rows), int(width)}, &rw, nullptr, 0, 0, am, st);
   PackArgs p{};
   p.x = reinterpret_cast<const void*>(x);
   p.ldx = ldx;
@@ -341,8 +315,6 @@ void linear_act8_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
   p.kq = q.kq;
   p.o = copy ? reinterpret_cast<uint16_t*>(base + q.f_x) : nullptr;
   p.plane = rows * q.kq;
-  p.amax = am;
-  p.inv = inv;
   if (p.q || p.o) {
     const dim3 grid(blocks(rows * (q.kq >> 3)));
     if (f32) hipLaunchKernelGGL((act8_pack_kernel<true>), grid, dim3(256), 0, st, p);
@@ -352,17 +324,10 @@ void linear_act8_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
   GemmArgs a{};
   a.I = copy ? Operand{p.o, q.kq, p.plane, int(rows)} : Operand{reinterpret_cast<const uint16_t*>(x), ldx, 0, int(rows)};
   a.J = {reinterpret_cast<const uint16_t*>(w), ldw, 0, int(out)};
-  if (f32) {
-    uint16_t* wp = reinterpret_cast<uint16_t*>(base + q.f_w);
-    split(rw, wp, q.kp, out * q.kp, am + kAmaxBlocks, inv + 1, st);
-    a.J = {wp, q.kp, out * q.kp, int(out)};
-    a.e.fi = inv;
-    a.e.fj = inv + 1;
-  }
+  if (f32) a.J = split({reinterpret_cast<const float*>(w), ldw, int(out), int(width)}, wp, q.kp, st);
   a.nk = q.kp;
   a.split = q.y_split;
   a.nk_split = a.nk;
-  a.e.f = 1.f;
   a.e.out = reinterpret_cast<void*>(y);
   a.e.ldo = out;
   a.e.bf16 = !f32;
@@ -375,8 +340,8 @@ void linear_act8_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
     a.lds = up(out, 8);
   }
   const int64_t grid_y = tiles_of(q.y_tile, rows, out) * q.y_s;
-  if (f32) gemm<true, 3, false, false, false>(q.y_tile, a, grid_y, st);
-  else gemm<false, 1, false, false, false>(q.y_tile, a, grid_y, st);
+  if (f32) gemm<6, false, false, false>(q.y_tile, a, grid_y, st);
+  else gemm<1, false, false, false>(q.y_tile, a, grid_y, st);
   if (a.slab) finish(q.y_tile, a, int(rows), nullptr, {}, st);
 }
 
@@ -385,7 +350,7 @@ void linear_act8_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
 // neither dw nor the GELU asks for it.  dy: bf16 rows of whole 16-byte vectors.
 void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintptr_t qp, uintptr_t qs, uintptr_t dx,
                      bool dx_add, uintptr_t dw, int64_t ldd, uintptr_t db, int grad_dt, int db_dt, bool accumulate,
-                     int64_t rows, int64_t width, int64_t out, int dt, bool gelu, uintptr_t amax, uintptr_t ws, uintptr_t stream) {
+                     int64_t rows, int64_t width, int64_t out, int dt, bool gelu, uintptr_t wp, uintptr_t ws, uintptr_t stream) {
   check_act8(rows, width, out, dt);
   const bool f32 = dt == kF32;
   VODA_CHECK((grad_dt == kF32 || grad_dt == kBF16) && (db_dt == kF32 || db_dt == kBF16),
@@ -394,30 +359,18 @@ void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintpt
              "linear_act8: bf16 weight rows must be 16-byte aligned and whole 16-byte vectors");
   VODA_CHECK(f32 || (dy % 16 == 0 && ldy % 8 == 0 && ldy >= up(out, 8)),
              "linear_act8: bf16 gradient rows must be 16-byte aligned and whole 16-byte vectors");
-  VODA_CHECK(qp % 16 == 0 && ws % 256 == 0, "linear_act8: workspaces must be aligned");
+  VODA_CHECK(qp % 16 == 0 && ws % 256 == 0 && wp % 16 == 0 && (wp || !f32 || !dx), "linear_act8: workspaces must be aligned");
   VODA_CHECK((qp && qs) || (!dw && !gelu), "linear_act8: the backward needs the checkpoint");
-  const Act8Plan q = act8_plan(rows, width, out, f32, true);
+  const Act8Plan q = act8_plan(rows, width, out, f32, gelu, true);
   hipStream_t st = as_stream(stream);
   uint8_t* base = reinterpret_cast<uint8_t*>(ws);
-  float* inv = reinterpret_cast<float*>(base + q.b_inv);  // of dy, w, act(c)
-  const float* am = reinterpret_cast<const float*>(amax);
   const uint8_t* q8 = reinterpret_cast<const uint8_t*>(qp);
   const uint8_t* s8 = reinterpret_cast<const uint8_t*>(qs);
   Operand DY = {reinterpret_cast<const uint16_t*>(dy), ldy, 0, int(rows)};
   Operand W = {reinterpret_cast<const uint16_t*>(w), ldw, 0, int(out)};
   if (f32) {
-    const Rows rdy = {reinterpret_cast<const float*>(dy), ldy, int(rows), int(out)};
-    float* dam = reinterpret_cast<float*>(base + q.b_amax);
-    gt::amax(rdy, nullptr, nullptr, 0, 0, dam, st);
-    uint16_t* dyp = reinterpret_cast<uint16_t*>(base + q.b_dy);
-    split(rdy, dyp, q.np8, rows * q.np8, dam, inv, st);
-    DY = {dyp, q.np8, rows * q.np8, int(rows)};
-    if (dx) {
-      uint16_t* wp = reinterpret_cast<uint16_t*>(base + q.b_w);
-      split({reinterpret_cast<const float*>(w), ldw, int(out), int(width)}, wp, q.kp, out * q.kp, am + kAmaxBlocks, inv + 1,
-            st);
-      W = {wp, q.kp, out * q.kp, int(out)};
-    }
+    DY = split({reinterpret_cast<const float*>(dy), ldy, int(rows), int(out)}, reinterpret_cast<uintptr_t>(base + q.b_dy), q.np8, st);
+    if (dx) W = split({reinterpret_cast<const float*>(w), ldw, int(out), int(width)}, wp, q.kp, st);
   }
   if (dx) {
     GemmArgs a{};
@@ -427,9 +380,6 @@ void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintpt
     a.nk = int(out);
     a.split = q.dx_split;
     a.nk_split = a.nk;
-    a.e.f = 1.f;
-    a.e.fi = f32 ? inv : nullptr;
-    a.e.fj = f32 ? inv + 1 : nullptr;
     a.e.out = reinterpret_cast<void*>(dx);
     a.e.ldo = width;
     a.e.bf16 = !f32;
@@ -446,8 +396,8 @@ void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintpt
       a.lds = q.kp;
     }
     const int64_t grid_x = tiles_of(q.dx_tile, rows, width) * q.dx_s;
-    if (f32) gemm<true, 3, false, true, false>(q.dx_tile, a, grid_x, st);
-    else gemm<false, 1, false, true, false>(q.dx_tile, a, grid_x, st);
+    if (f32) gemm<6, false, true, false>(q.dx_tile, a, grid_x, st);
+    else gemm<1, false, true, false>(q.dx_tile, a, grid_x, st);
     if (a.slab) finish(q.dx_tile, a, int(rows), nullptr, {}, st);
   }
   if (!dw) return;
@@ -456,12 +406,9 @@ void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintpt
   u.qs = s8;
   u.n = rows * (q.kq >> 3);
   u.gelu = gelu;
-  u.planes = gelu ? 2 : 1;
   u.o = reinterpret_cast<uint16_t*>(base + q.b_c);
   u.plane = rows * q.kq;
-  u.amax = am;
-  u.inv = inv + 2;
-  if (f32) hipLaunchKernelGGL((act8_unpack_kernel<true>), dim3(blocks(u.n)), dim3(256), 0, st, u);
+  if (f32 && gelu) hipLaunchKernelGGL((act8_unpack_kernel<true>), dim3(blocks(u.n)), dim3(256), 0, st, u);
   else hipLaunchKernelGGL((act8_unpack_kernel<false>), dim3(blocks(u.n)), dim3(256), 0, st, u);
   check_launch();
   GemmArgs a{};
@@ -471,9 +418,6 @@ void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintpt
   a.nk = int(rows);
   a.split = q.dw_split;
   a.nk_split = a.nk;
-  a.e.f = 1.f;
-  a.e.fi = f32 ? inv : nullptr;
-  a.e.fj = f32 ? inv + 2 : nullptr;
   a.e.out = reinterpret_cast<void*>(dw);
   a.e.ldo = ldd;
   a.e.bf16 = grad_dt == kBF16;
@@ -488,9 +432,9 @@ void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintpt
     a.bslab = db ? reinterpret_cast<float*>(base + q.b_db) : nullptr;
   }
   const int64_t grid_w = tiles_of(q.dw_tile, out, width) * q.dw_s;
-  if (f32 && gelu) gemm<true, 3, true, true, true>(q.dw_tile, a, grid_w, st);
-  else if (f32) gemm<true, 2, true, true, true>(q.dw_tile, a, grid_w, st);
-  else gemm<false, 1, true, true, true>(q.dw_tile, a, grid_w, st);
+  if (f32 && gelu) gemm<6, true, true, true>(q.dw_tile, a, grid_w, st);
+  else if (f32) gemm<3, true, true, true>(q.dw_tile, a, grid_w, st);
+  else gemm<1, true, true, true>(q.dw_tile, a, grid_w, st);
   if (a.slab) {
     ColumnSums c{};
     c.part = a.bslab;

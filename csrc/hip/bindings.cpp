@@ -49,7 +49,8 @@ PYBIND11_MODULE(_vodahip, m) {
   m.def("linear_xent_sizes", &linear_xent_sizes);
   m.def("linear_xent_fwd", &linear_xent_fwd);
   m.def("linear_xent_bwd", &linear_xent_bwd);
-  m.def("linear_act8_sizes", &linear_act8_sizes);
+  m.def("linear_act8_sizes", &linear_act8_sizes, py::arg("rows"), py::arg("width"), py::arg("out"), py::arg("dt"),
+        py::arg("copy"), py::arg("gelu") = true);
   m.def("act8_pack", &act8_pack);
   m.def("act8_values", &act8_values);
   m.def("linear_act8_fwd", &linear_act8_fwd);

@@ -17,11 +17,12 @@
 //    fragments are in registers, so the buffer is refilled (one DMA instruction between two products)
 //    and the next stage's first fragments are read while they run.  Chunks past the reduction's end
 //    read a zero chunk; rows past an operand's end read its last row (never stored).
-//  * fp32 operands run as two fp16 planes, x 2^a = hi + 2^-11 lo: hi is x's first 11 bits, lo the
-//    next 11, so an element is held to 2^-24 of its size, or 2^-50 of the largest element where that
-//    is more (a: the power of two that brings the tensor's largest element to [2^14, 2^15)).
-//    Three products: hi.lo and lo.hi first, one exact scaling of the accumulators by 2^-11, then
-//    hi.hi; lo.lo, 2^-24 of the result, is left out.  Half the matrix work of a three-way bf16 split.
+//  * fp32 operands run as three bf16 planes, x = hi + mid + lo exactly: each is what the planes before it
+//    leave, rounded to bf16, and 3 x 8 bits are fp32's 24.  bf16 has fp32's exponents, so the planes hold an
+//    element by itself, whatever else its row or tensor holds (down to 2^-110, below which lo, then
+//    mid, run out of exponents).  Six products, the smallest first: mid.lo, lo.mid (2^-27 of the result each)
+//    and lo.lo are left out.  Two fp16 planes would do with three products, but hold an element only to
+//    2^-50 of the largest that shares its scale: one row of 1e16 in a tensor, and the others are gone.
 #pragma once
 
 #include "common.h"
@@ -33,16 +34,11 @@ namespace voda {
 namespace gt {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x4_v __attribute__((__vector_size__(4 * sizeof(__bf16))));
 typedef __attribute__((address_space(3))) bf16x4_v lds_bf16x4;
 typedef __attribute__((address_space(3))) void lds_void;
-
-constexpr float kLoScale = 1.f / 2048.f;  // weight of an fp16 lo plane
-constexpr int kSplitExp = 15;             // hi planes: the largest element lies below 2^15
 
 // what chunks past a reduction's end read
 static __device__ __attribute__((aligned(16))) uint32_t zero_chunk[4];
@@ -50,7 +46,7 @@ static __device__ __attribute__((aligned(16))) uint32_t zero_chunk[4];
 struct Operand {
   const uint16_t* p;
   int64_t ld;     // elements between rows (row operand: between i; col operand: between k)
-  int64_t plane;  // elements between the hi and the lo plane
+  int64_t plane;  // elements between two planes
   int n;          // rows i (>= 1)
 };
 
@@ -73,26 +69,17 @@ __device__ __forceinline__ uint2 tr_read(const uint8_t* base, int off) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(base + off)));
 }
 
-template <bool F16>
 __device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
-  if constexpr (F16)
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
 // sum of a fragment's eight elements, in fp32
-template <bool F16>
 __device__ __forceinline__ float sum8(uint4 f) {
   const uint32_t u[4] = {f.x, f.y, f.z, f.w};
   float s = 0.f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if constexpr (F16)
-      s = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, u[e]), f16x2{1, 1}, s, false);
-    else
-      s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, u[e]), bf16x2{1, 1}, s, false);
-  }
+  for (int e = 0; e < 4; ++e)
+    s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, u[e]), bf16x2{1, 1}, s, false);
   return s;
 }
 
@@ -178,9 +165,8 @@ struct Stage {
 };
 
 // Tile of WJ x WI waves, each TJ x TI 32 x 32 blocks: BJ = 32 WJ TJ columns, BI = 32 WI TI rows.
-// NP products: 1 (plain 16-bit operands), 2 (I in two planes, J in one), 3 (both in two planes).  A lo
-// plane weighs 2^-11 in fp16 and 1 in bf16, whose exponent needs no help.
-template <bool F16, int NP, bool IT, bool JT, int WJ_, int WI_, int TJ_, int TI_, int BK_, int ST_>
+// NP products: 1 (plain 16-bit operands), 2 or 3 (I in that many planes, J in one), 6 (both in three).
+template <int NP, bool IT, bool JT, int WJ_, int WI_, int TJ_, int TI_, int BK_, int ST_>
 struct Tile {
   static constexpr int WJ = WJ_, WI = WI_, TJ = TJ_, TI = TI_, BK = BK_, ST = ST_;
   static constexpr int NW = WJ * WI, kThreads = 64 * NW;
@@ -190,8 +176,12 @@ struct Tile {
   static constexpr int kStage = SI::kBytes + SJ::kBytes;
   static constexpr int kLds = ST * kStage;
   static constexpr int kPer = SI::kPer + SJ::kPer;
-  static constexpr float kLo = F16 ? kLoScale : 1.f;  // weight of a lo plane
+  static_assert(NP == 1 || NP == 2 || NP == 3 || NP == 6, "products");
   static_assert(ST >= 2 && (ST - 1) * kPer < 64 && BK % 32 == 0, "ring depth");
+
+  // planes of product p: (2 0) (0 2) (1 1) (1 0) (0 1) (0 0), or I's from the last on
+  static __device__ __forceinline__ int plane_i(int p) { return NP == 6 ? (0x52 >> (2 * p)) & 3 : NP - 1 - p; }
+  static __device__ __forceinline__ int plane_j(int p) { return NP == 6 ? (0x118 >> (2 * p)) & 3 : 0; }
 
   struct Where {
     int lane, wave, h, il, wi, wj;
@@ -209,7 +199,7 @@ struct Tile {
   };
 
   // acc[tj][ti] = the tile's products over k in [k0, k1).  SUM and ``want``: also the sums of I over k
-  // (of its planes' value, in hi units) for this lane's rows i; half h of the wave holds half of them.
+  // (all its planes) for this lane's rows i; half h of the wave holds half of them.
   template <bool SUM>
   static __device__ __forceinline__ void run(uint8_t* smem, const Operand& I, const Operand& J, int i0, int j0, int k0,
                                              int k1, f32x16 (&acc)[TJ][TI], float (&isum)[TI], bool want = false) {
@@ -234,11 +224,9 @@ struct Tile {
     int64_t shi = 0, shj = 0;
     int left = 0;
     auto aim = [&] {
-      const bool lo_i = NP == 3 ? prod == 1 : NP == 2 ? prod == 0 : false;
-      const bool lo_j = NP == 3 && prod == 0;
       left = k1 - k0 - at * BK;
-      shi = at * stepi + (lo_i ? I.plane : 0);
-      shj = at * stepj + (lo_j ? J.plane : 0);
+      shi = at * stepi + plane_i(prod) * I.plane;
+      shj = at * stepj + plane_j(prod) * J.plane;
       if (++at >= steps) { at = 0; ++prod; }
     };
     auto issue = [&](int u, uint8_t* lds) {
@@ -270,17 +258,10 @@ struct Tile {
     wait_stages(total - 1);
     fetch(0, 0, 0);
     int buf = 0, st = 0;
+    int sum_prod = 0, sum_at = 0;  // SUM: product and step of the stage that runs
     constexpr int mf = TI * TJ;
     // one stage; ``more``: a stage is left to issue into the buffer that it frees
     auto stage = [&](auto more) {
-      if (NP > 1 && F16 && st == (NP - 1) * steps) {
-#pragma unroll
-        for (int a = 0; a < TJ; ++a)
-#pragma unroll
-          for (int b = 0; b < TI; ++b)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[a][b][r] *= kLo;
-      }
       const int next = buf + 1 == ST ? 0 : buf + 1;
 #pragma unroll
       for (int kk = 0; kk < BK / 16; ++kk) {
@@ -295,19 +276,15 @@ struct Tile {
           fetch(next, 0, 0);  // past the last stage: never used
         }
         if constexpr (SUM) {
-          // the reduction's sum of I: the hi plane in the last product, lo where it runs with J's hi
-          const bool lo = NP == 3 ? st >= steps && st < 2 * steps : NP == 2 ? st < steps : false;
-          if (want && (lo || st >= (NP - 1) * steps)) {
+          // each of I's planes once, where it runs with J's first
+          if (want && plane_j(sum_prod) == 0) {
 #pragma unroll
-            for (int b = 0; b < TI; ++b) {
-              const float s = sum8<F16>(fi[kk & 1][b]);
-              isum[b] += lo ? s * kLo : s;
-            }
+            for (int b = 0; b < TI; ++b) isum[b] += sum8(fi[kk & 1][b]);
           }
         }
 #pragma unroll
         for (int x = 0; x < mf; ++x) {
-          acc[x / TI][x % TI] = mfma<F16>(fj[kk & 1][x / TI], fi[kk & 1][x % TI], acc[x / TI][x % TI]);
+          acc[x / TI][x % TI] = mfma(fj[kk & 1][x / TI], fi[kk & 1][x % TI], acc[x / TI][x % TI]);
           // between two products: a DMA instruction or two of the refill, or a fragment of the next step
           if (tail) {
             if constexpr (more.value) {
@@ -329,6 +306,7 @@ struct Tile {
         }
       }
       buf = next;
+      if (SUM && ++sum_at == steps) { sum_at = 0; ++sum_prod; }
     };
     for (; st + ST < total; ++st) stage(std::true_type{});
     for (; st < total; ++st) stage(std::false_type{});
@@ -366,26 +344,21 @@ struct Split {
   }
 };
 
-// fp32 -> its two planes, of x 2^a
-__device__ __forceinline__ void split2(float xs, uint16_t& hi, uint16_t& lo) {
-  const _Float16 h = static_cast<_Float16>(xs);
-  hi = __builtin_bit_cast(uint16_t, h);
-  lo = f2h((xs - static_cast<float>(h)) * 2048.f);
+// fp32 -> its three planes.  A finite x that would round past bf16's largest takes that one; an infinite or
+// NaN x is hi alone.
+__device__ __forceinline__ void split3(float x, uint16_t& hi, uint16_t& mid, uint16_t& lo) {
+  const bool finite = fabsf(x) <= 3.4028235e38f;
+  hi = f2bf(x);
+  if (finite && (hi & 0x7fff) == 0x7f80) --hi;
+  const float r = x - bf2f(hi);  // exact, as is what follows
+  mid = f2bf(r);
+  lo = f2bf(r - bf2f(mid));
+  if (!finite) mid = lo = 0;
 }
-
-// 2^a for a tensor whose largest finite |element| is amax: amax 2^a in [2^14, 2^15)
-__device__ __forceinline__ float split_scale(float amax) {
-  if (!(amax > 0.f)) return 1.f;
-  const int e = int((__float_as_uint(amax) >> 23) & 255) - 127;  // floor(log2); subnormal: -127
-  return __uint_as_float(uint32_t(min(kSplitExp - 1 - e, 126) + 127) << 23);
-}
-
-// 1 / 2^a, exact (2^a is between 2^-113 and 2^126)
-__device__ __forceinline__ float pow2_inverse(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
 // ---- stores -----------------------------------------------------------------------------------
 
-// What becomes of a product: out = (sum of its splits) * factors [* gelu'(checkpoint)] [+ bias]
+// What becomes of a product: out = (sum of its splits) * factor [* gelu'(checkpoint)] [+ bias]
 // [+ out], in fp32 until the one rounding to out's type.
 struct Emit {
   void* out;
@@ -399,25 +372,18 @@ struct Emit {
   const uint8_t* q;         // e4m3 checkpoint [i][ldq] whose gelu' multiplies, or null
   const uint8_t* qs;        // its scales [i][ldq / 32]
   int64_t ldq;
-  // factors: f times I's and J's inverse plane scales times *gl / max(*gn, 1), each pointer or null (fi
-  // only with fj)
-  float f;
-  const float* fi;
-  const float* fj;
+  // the factor: *gl / max(*gn, 1), or 1 without them
   const float* gl;
   const int* gn;
 
-  // what a kernel reads once: the factors (one after the other: a product of two may leave fp32's range
-  // where the result does not) and the bias of a lane's eight columns
+  // what a kernel reads once: the factor and the bias of a lane's eight columns
   struct Once {
-    float a, b, c;
+    float a;
     float bias[8];
   };
   __device__ __forceinline__ Once once(int j) const {
     Once o;
-    o.a = gl ? f * (*gl / float(max(*gn, 1))) : f;
-    o.b = fi ? *fi : 1.f;
-    o.c = fj ? *fj : 1.f;
+    o.a = gl ? *gl / float(max(*gn, 1)) : 1.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       o.bias[e] = !bias || j + e >= nj ? 0.f
@@ -438,11 +404,11 @@ struct Emit {
     }
     return c;
   }
-  // columns j .. j+7 of row i (j % 8 == 0); ``keep`` false: the row is zero whatever the factors are
+  // columns j .. j+7 of row i (j % 8 == 0); ``keep`` false: the row is zero whatever the factor is
   __device__ __forceinline__ void eight(const Once& o, const Check& c, int i, int j, float (&v)[8], bool keep = true) const {
     if (j >= nj) return;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = !keep ? 0.f : fj ? v[e] * o.a * o.b * o.c : v[e] * o.a;
+    for (int e = 0; e < 8; ++e) v[e] = !keep ? 0.f : v[e] * o.a;
     if (q) {
       const uint2 u = c.u;
       const float s = __uint_as_float(c.s << 23);
@@ -561,9 +527,9 @@ __device__ __forceinline__ void split_range(int nk, int splits, int s, int bk, i
   k1 = min(nk, k0 + per * bk);
 }
 
-// a sum over I alone: without J's factor
+// a sum over I alone
 __device__ __forceinline__ void emit_sum(const Emit& e, const Emit::Once& o, void* out, bool bf16, int i, float v) {
-  v = v * o.a * o.b;
+  v = v * o.a;
   if (bf16) {
     uint16_t* o = static_cast<uint16_t*>(out) + i;
     *o = f2bf(v + (e.accumulate ? bf2f(*o) : 0.f));
@@ -636,7 +602,7 @@ struct ColumnSums {
   int bi, per;
   void* out;
   int bf16;
-  Emit e;             // factors (without J's) and whether to add
+  Emit e;             // the factor and whether to add
 };
 
 // Sums the splits of a product's slab and stores the result; ``inv`` (or null) maps an output row to its
@@ -689,83 +655,18 @@ static __global__ __launch_bounds__(256) void finish_kernel(FinishArgs p) {
 
 // ---- fp32 -> planes ----------------------------------------------------------------------------
 
-constexpr int kAmaxBlocks = 1024;  // partial maxima a tensor
-
-// the largest of a tensor's partial maxima, by every thread of a block of 256
-__device__ __forceinline__ float amax_of(const float* part, float* lds4) {
-  float m = 0.f;
-#pragma unroll
-  for (int k = 0; k < kAmaxBlocks / 256; ++k) m = fmaxf(m, part[threadIdx.x + 256 * k]);
-  m = wave_max(m);
-  __syncthreads();  // lds4 may still be read from an earlier call
-  if ((threadIdx.x & 63) == 0) lds4[threadIdx.x >> 6] = m;
-  __syncthreads();
-  return fmaxf(fmaxf(lds4[0], lds4[1]), fmaxf(lds4[2], lds4[3]));
-}
-
-// an infinite or NaN element: hi carries it, lo is zero
-__device__ __forceinline__ void split_safe(float x, float scale, uint16_t& hi, uint16_t& lo) {
-  split2(x * scale, hi, lo);
-  if (!(fabsf(x) <= 3.4028235e38f)) lo = 0;
-}
-
 struct Rows {
   const float* p;
   int64_t ld;
   int n, width;
 };
 
-// Partial maxima [2][kAmaxBlocks] of the finite |elements| of a and b (grid: 2 kAmaxBlocks, or half of
-// it for a alone).  With ``labels``, of the rows of a whose label is in [0, classes) and not ``ignore``.
-static __global__ __launch_bounds__(256) void amax_kernel(Rows a, Rows b, const int64_t* __restrict__ labels, int64_t ignore,
-                                                   int classes, float* __restrict__ part) {
-  const bool second = blockIdx.x >= kAmaxBlocks;
-  const Rows x = second ? b : a;
-  const int blk = second ? blockIdx.x - kAmaxBlocks : blockIdx.x;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  auto of = [](float v) { return fabsf(v) <= 3.4028235e38f ? fabsf(v) : 0.f; };
-  const bool vec = (x.ld & 3) == 0 && (x.width & 3) == 0 && (reinterpret_cast<uintptr_t>(x.p) & 15) == 0;
-  float m = 0.f;
-  for (int r = blk * 4 + wave; r < x.n; r += kAmaxBlocks * 4) {
-    if (!second && labels) {
-      const int64_t y = labels[r];
-      if (y == ignore || y < 0 || y >= classes) continue;
-    }
-    const float* row = x.p + int64_t(r) * x.ld;
-    if (vec) {
-#pragma unroll 4
-      for (int c = 4 * lane; c < x.width; c += 256) {
-        const float4 u = *reinterpret_cast<const float4*>(row + c);
-        m = fmaxf(m, fmaxf(fmaxf(of(u.x), of(u.y)), fmaxf(of(u.z), of(u.w))));
-      }
-    } else {
-      for (int c = lane; c < x.width; c += 64) m = fmaxf(m, of(row[c]));
-    }
-  }
-  __shared__ float lds[4];
-  m = wave_max(m);
-  if (lane == 0) lds[wave] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
-}
-
-inline void amax(const Rows& a, const Rows* b, const int64_t* labels, int64_t ignore, int classes, float* part,
-                 hipStream_t st) {
-  hipLaunchKernelGGL(amax_kernel, dim3(b ? 2 * kAmaxBlocks : kAmaxBlocks), dim3(256), 0, st, a, b ? *b : a, labels, ignore,
-                     classes, part);
-  check_launch();
-}
-
 __device__ __forceinline__ uint2 pack4(const uint16_t (&v)[4]) {
   return make_uint2(v[0] | (uint32_t(v[1]) << 16), v[2] | (uint32_t(v[3]) << 16));
 }
 
-// x's rows as two fp16 planes [n][kp] (zeros from width to kp), and 2^-a to *inv; one quad a thread
-static __global__ __launch_bounds__(256) void split_kernel(Rows x, uint16_t* __restrict__ out, int kp, int64_t plane,
-                                                    const float* __restrict__ part, float* __restrict__ inv) {
-  __shared__ float lds[4];
-  const float s = split_scale(amax_of(part, lds));
-  if (blockIdx.x == 0 && threadIdx.x == 0) *inv = pow2_inverse(s);
+// x's rows as three planes [n][kp] (zeros from width to kp), one quad a thread
+static __global__ __launch_bounds__(256) void split_kernel(Rows x, uint16_t* __restrict__ out, int kp, int64_t plane) {
   const int quads = kp >> 2;
   const bool vec = (x.ld & 3) == 0 && (x.width & 3) == 0 && (reinterpret_cast<uintptr_t>(x.p) & 15) == 0;
   const int64_t n = int64_t(x.n) * quads;
@@ -787,18 +688,22 @@ static __global__ __launch_bounds__(256) void split_kernel(Rows x, uint16_t* __r
       for (int e = 0; e < 4; ++e)
         if (c + e < x.width) v[e] = row[e];
     }
-    uint16_t hi[4], lo[4];
+    uint16_t hi[4], mid[4], lo[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) split_safe(v[e], s, hi[e], lo[e]);
+    for (int e = 0; e < 4; ++e) split3(v[e], hi[e], mid[e], lo[e]);
     *reinterpret_cast<uint2*>(out + 4 * t) = pack4(hi);
-    *reinterpret_cast<uint2*>(out + plane + 4 * t) = pack4(lo);
+    *reinterpret_cast<uint2*>(out + plane + 4 * t) = pack4(mid);
+    *reinterpret_cast<uint2*>(out + 2 * plane + 4 * t) = pack4(lo);
   }
 }
 
-inline void split(const Rows& x, uint16_t* out, int kp, int64_t plane, const float* part, float* inv, hipStream_t st) {
-  hipLaunchKernelGGL(split_kernel, dim3(stream_grid(int64_t(x.n) * (kp >> 2), 256, 8192)), dim3(256), 0, st, x, out, kp,
-                     plane, part, inv);
+// the planes in ``out`` [3][n][kp], as an operand
+inline Operand split(const Rows& x, uintptr_t out, int kp, hipStream_t st) {
+  uint16_t* o = reinterpret_cast<uint16_t*>(out);
+  const int64_t plane = int64_t(x.n) * kp;
+  hipLaunchKernelGGL(split_kernel, dim3(stream_grid(int64_t(x.n) * (kp >> 2), 256, 8192)), dim3(256), 0, st, x, o, kp, plane);
   check_launch();
+  return {o, kp, plane, x.n};
 }
 
 // ---- choices shared by the operators -------------------------------------------------------------
@@ -818,11 +723,11 @@ inline int whole_rows(uintptr_t p, int64_t ld, bool bf16) { return p % 16 == 0 &
 //         loads' latency (2 us a stage) then.  [1001 x 331] . [331 x 1348] in fp32 36 -> 20 us, but
 //         [8192 x 2304]^T . [8192 x 768] in bf16, which splits into two a CU, 50 -> 64;
 //   kFew  128 x 32 (row operands), for a handful of rows, whose products only stream the weights.
-template <bool F16, int NP, bool IT, bool JT> using Wide = Tile<F16, NP, IT, JT, 2, 4, 4, 2, 64, 2>;
-template <bool F16, int NP, bool IT, bool JT> using Big = Tile<F16, NP, IT, JT, 2, 2, 4, 2, 32, 3>;
-template <bool F16, int NP, bool IT, bool JT> using Sq = Tile<F16, NP, IT, JT, 2, 2, 2, 2, 64, 2>;
-template <bool F16, int NP, bool IT, bool JT> using Deep = Tile<F16, NP, IT, JT, 2, 2, 2, 2, 64, 4>;
-template <bool F16, int NP, bool IT, bool JT> using Few = Tile<F16, NP, IT, JT, 4, 1, 1, 1, 64, 3>;
+template <int NP, bool IT, bool JT> using Wide = Tile<NP, IT, JT, 2, 4, 4, 2, 64, 2>;
+template <int NP, bool IT, bool JT> using Big = Tile<NP, IT, JT, 2, 2, 4, 2, 32, 3>;
+template <int NP, bool IT, bool JT> using Sq = Tile<NP, IT, JT, 2, 2, 2, 2, 64, 2>;
+template <int NP, bool IT, bool JT> using Deep = Tile<NP, IT, JT, 2, 2, 2, 2, 64, 4>;
+template <int NP, bool IT, bool JT> using Few = Tile<NP, IT, JT, 4, 1, 1, 1, 64, 3>;
 
 enum { kWide = 0, kBig = 1, kSq = 2, kDeep = 3, kFew = 4 };
 inline int tile_bj(int t) { return t <= kBig ? 256 : 128; }
@@ -880,13 +785,13 @@ inline void launch_gemm(const GemmArgs& p, int64_t grid, hipStream_t st) {
   check_launch();
 }
 
-template <bool F16, int NP, bool IT, bool JT, bool SUM>
+template <int NP, bool IT, bool JT, bool SUM>
 inline void gemm(int tile, const GemmArgs& p, int64_t grid, hipStream_t st) {
-  if (tile == kWide) launch_gemm<Wide<F16, NP, IT, JT>, SUM>(p, grid, st);
-  else if (tile == kBig) launch_gemm<Big<F16, NP, IT, JT>, SUM>(p, grid, st);
-  else if (tile == kSq) launch_gemm<Sq<F16, NP, IT, JT>, SUM>(p, grid, st);
-  else if (tile == kDeep) launch_gemm<Deep<F16, NP, IT, JT>, SUM>(p, grid, st);
-  else if constexpr (!IT) launch_gemm<Few<F16, NP, IT, JT>, SUM>(p, grid, st);
+  if (tile == kWide) launch_gemm<Wide<NP, IT, JT>, SUM>(p, grid, st);
+  else if (tile == kBig) launch_gemm<Big<NP, IT, JT>, SUM>(p, grid, st);
+  else if (tile == kSq) launch_gemm<Sq<NP, IT, JT>, SUM>(p, grid, st);
+  else if (tile == kDeep) launch_gemm<Deep<NP, IT, JT>, SUM>(p, grid, st);
+  else if constexpr (!IT) launch_gemm<Few<NP, IT, JT>, SUM>(p, grid, st);
 }
 
 inline void finish(int tile, const GemmArgs& g, int rows, const int* inv, const ColumnSums& c, hipStream_t st) {

@@ -8,7 +8,7 @@
 // The logits of a tile live in the accumulators only.  Forward: one product x w^T whose epilogue
 // leaves a (max, sum exp) pair a row for each 32 * TJ columns of the vocabulary, joined by
 // xent_join.  Backward: piece by piece of the vocabulary the product runs again and leaves G of the
-// piece in a workspace (16 bits; fp32 inputs: two fp16 planes), which the two gradient products read.
+// piece in a workspace (16 bits; fp32 inputs: three bf16 planes), which the two gradient products read.
 // So 8 n C K operations instead of 6, and no memory that grows with n C.
 //
 // Rows whose label is ignored (or lies outside [0, C)) are left out at the start: xent_gather copies
@@ -19,7 +19,7 @@
 // bf16 inputs: G is rounded once to bf16 for the two products (at most 2^-8 of each element, random in
 // sign, against the same rounding of the sums to bf16 at the end), up to 128 rows kept in two planes;
 // the one-hot part is subtracted before that rounding and g/n multiplied after the sums.  db sums G as it
-// was before.  fp32 inputs: two fp16 planes an operand (gemm_tile.h); G 2^15.
+// was before.  fp32 inputs: three bf16 planes an operand (gemm_tile.h), G too.
 // Sums over rows and splits have a fixed order: the same call gives the same bits.
 #include "gemm_tile.h"
 #include "ops.h"
@@ -39,14 +39,11 @@ using namespace gt;
 // from |max| near 30 on, and infinite sums of a slot whose classes are masked by -1e10.
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kGatherRows = 32;   // rows a gather workgroup
-constexpr float kGScale = 32768.f;  // G's planes hold G 2^15: |G| <= 1
 
 // device scalars of one call
 struct XentDev {
   int n;           // labelled rows
   int done;        // workgroups of xent_join that are through
-  float inv_x;     // 2^-a of x's planes (fp32 inputs)
-  float inv_w;     // 2^-a of w's planes
 };
 
 __device__ __forceinline__ bool labelled(int64_t y, int64_t ignore, int classes) {
@@ -59,7 +56,7 @@ struct GatherArgs {
   int rows, width, classes, vec;
   const int64_t* labels;
   int64_t ignore;
-  uint16_t* xc;      // [rows][kp] (fp32: two planes)
+  uint16_t* xc;      // [rows][kp] (fp32: three planes)
   int kp;
   int64_t plane;
   int* inv;          // [rows]: place among the labelled rows, or -1
@@ -70,7 +67,6 @@ struct GatherArgs {
   int bias_bf16;
   float* bias32;     // [bias_n]: bias, 0 where there is none, -inf from classes on
   int bias_n;
-  const float* amax; // fp32: partial maxima of x
   int gather_blocks;
   const int* counts; // labelled rows of each kCountRows, or null: count them here
 };
@@ -106,14 +102,8 @@ __global__ __launch_bounds__(256) void xent_gather_kernel(GatherArgs p) {
                                    : static_cast<const float*>(p.bias)[v];
     return;
   }
-  __shared__ float lds[4];
   __shared__ int cnt[4];
   __shared__ int place[kGatherRows];
-  float scale = 1.f;
-  if constexpr (F32) {
-    scale = split_scale(amax_of(p.amax, lds));
-    if (blockIdx.x == 0 && t == 0) p.dev->inv_x = pow2_inverse(scale);
-  }
   // labelled rows in front of this workgroup's: every workgroup counts them itself (8 bytes a row
   // out of the L2), cheaper than a second launch up to some thousand rows, or from the counts
   const int r0 = blockIdx.x * kGatherRows;
@@ -158,23 +148,23 @@ __global__ __launch_bounds__(256) void xent_gather_kernel(GatherArgs p) {
       const float* row = static_cast<const float*>(p.x) + int64_t(r0 + u) * p.ldx;
       if (p.vec) {
         for (int k = 4 * lane; k < p.kp; k += 256) {
-          uint16_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
-          if (k < p.width) {
-            const float4 f = *reinterpret_cast<const float4*>(row + k);
-            const float v[4] = {f.x, f.y, f.z, f.w};
+          float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (k < p.width) f = *reinterpret_cast<const float4*>(row + k);
+          const float v[4] = {f.x, f.y, f.z, f.w};
+          uint16_t hi[4], mid[4], lo[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) split_safe(v[e], scale, hi[e], lo[e]);
-          }
-          *reinterpret_cast<uint2*>(o + k) = make_uint2(hi[0] | (uint32_t(hi[1]) << 16), hi[2] | (uint32_t(hi[3]) << 16));
-          *reinterpret_cast<uint2*>(o + p.plane + k) =
-              make_uint2(lo[0] | (uint32_t(lo[1]) << 16), lo[2] | (uint32_t(lo[3]) << 16));
+          for (int e = 0; e < 4; ++e) split3(v[e], hi[e], mid[e], lo[e]);
+          *reinterpret_cast<uint2*>(o + k) = pack4(hi);
+          *reinterpret_cast<uint2*>(o + p.plane + k) = pack4(mid);
+          *reinterpret_cast<uint2*>(o + 2 * p.plane + k) = pack4(lo);
         }
       } else {
         for (int k = lane; k < p.kp; k += 64) {
-          uint16_t hi = 0, lo = 0;
-          if (k < p.width) split_safe(row[k], scale, hi, lo);
+          uint16_t hi, mid, lo;
+          split3(k < p.width ? row[k] : 0.f, hi, mid, lo);
           o[k] = hi;
-          o[p.plane + k] = lo;
+          o[p.plane + k] = mid;
+          o[2 * p.plane + k] = lo;
         }
       }
     } else {
@@ -201,7 +191,7 @@ struct LogitArgs {
   float2* part;
   float* zlab;
   int* tie;
-  // backward: (max, 1 / sum exp) of each row; G [rows][ldg] (fp32 inputs: two planes)
+  // backward: (max, 1 / sum exp) of each row; G [rows][ldg] (fp32 inputs: three planes)
   const float2* stat;
   uint16_t* G;
   int64_t ldg, gplane;
@@ -211,7 +201,8 @@ struct LogitArgs {
 
 // Rows are the tile's i, vocabulary columns its j.  The epilogue is vector work that the matrix cores
 // wait for unless another workgroup of the CU is in its main loop: two workgroups a CU (72 KB of LDS each).
-template <class T, bool F16, bool BWD, bool TWO>
+// PL: planes of G.
+template <class T, bool BWD, int PL>
 __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[T::kLds];
   Operand X = p.X;
@@ -235,11 +226,6 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
   f32x16 acc[T::TJ][T::TI];
   float unused[T::TI];
   T::template run<false>(smem, X, p.W, i0, j0, 0, p.width, acc, unused);
-  float sx = 1.f, sw = 1.f;
-  if constexpr (F16) {
-    sx = p.dev->inv_x;
-    sw = p.dev->inv_w;
-  }
   // z = products + bias; columns past the classes get the bias's -inf
 #pragma unroll
   for (int a = 0; a < (BWD ? 0 : T::TJ); ++a) {
@@ -250,11 +236,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int c = 0; c < T::TI; ++c) {
-          float v = acc[a][c][4 * g + e];
-          if constexpr (F16) v = v * sx * sw;
-          acc[a][c][4 * g + e] = v + b[e];
-        }
+        for (int c = 0; c < T::TI; ++c) acc[a][c][4 * g + e] += b[e];
     }
   }
   float sums[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // BWD: of this lane's columns
@@ -325,29 +307,28 @@ __global__ __launch_bounds__(T::kThreads, 2) void xent_logits_kernel(LogitArgs p
         uint16_t* g = p.G + int64_t(i0 + r) * p.ldg + (j0 - p.v0) + j;
         float d[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if constexpr (F16) v[e] = v[e] * sx * sw;
-          d[e] = __builtin_amdgcn_exp2f((v[e] + bias[e] - sm) * kLog2e) * sy;
-        }
+        for (int e = 0; e < 8; ++e) d[e] = __builtin_amdgcn_exp2f((v[e] + bias[e] - sm) * kLog2e) * sy;
         if (__ballot(unsigned(y) < 8u)) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             if (e == y) d[e] -= 1.f;
         }
-        uint16_t hi[8], lo[8];
+        uint16_t q[PL][8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           sums[e] += d[e];
-          if constexpr (F16) split2(d[e] * kGScale, hi[e], lo[e]);
-          else hi[e] = f2bf(d[e]);
-          if constexpr (TWO && !F16) lo[e] = f2bf(d[e] - bf2f(hi[e]));
+#pragma unroll
+          for (int k = 0; k < PL; ++k) {  // each plane what those before it leave
+            q[k][e] = f2bf(d[e]);
+            d[e] -= bf2f(q[k][e]);
+          }
         }
         auto eight = [](const uint16_t(&a)[8]) {
           return make_uint4(a[0] | (uint32_t(a[1]) << 16), a[2] | (uint32_t(a[3]) << 16), a[4] | (uint32_t(a[5]) << 16),
                             a[6] | (uint32_t(a[7]) << 16));
         };
-        *reinterpret_cast<uint4*>(g) = eight(hi);
-        if constexpr (TWO) *reinterpret_cast<uint4*>(g + p.gplane) = eight(lo);
+#pragma unroll
+        for (int k = 0; k < PL; ++k) *reinterpret_cast<uint4*>(g + k * p.gplane) = eight(q[k]);
       });
     }
   }
@@ -474,23 +455,22 @@ int tile_wi(int t) { return t == kWide ? 4 : t == kFew ? 1 : 2; }
 // columns of one (max, sum) slot: a wave's part of the tile
 int tile_slot(int t) { return t <= kBig ? 128 : t == kFew ? 32 : 64; }
 
-template <bool F16, bool BWD, bool TWO>
+// NP products a logit (gemm_tile.h), PL planes of G
+template <int NP, bool BWD, int PL>
 void launch_logits(LogitArgs& p, int tile, hipStream_t st) {
-  constexpr int NP = F16 ? 3 : 1;
   p.tj = (p.v1 - p.v0 + tile_bj(tile) - 1) / tile_bj(tile);
   const dim3 grid(unsigned(tiles_of(tile, p.X.n, p.v1 - p.v0)));
   auto go = [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    hipLaunchKernelGGL((xent_logits_kernel<T, F16, BWD, TWO>), grid, dim3(T::kThreads), 0, st, p);
+    hipLaunchKernelGGL((xent_logits_kernel<T, BWD, PL>), grid, dim3(T::kThreads), 0, st, p);
   };
-  // bf16 G in two planes comes with few rows only
-  constexpr bool large = F16 || !TWO;
-  if (tile == kFew) go(static_cast<Few<F16, NP, false, false>*>(nullptr));
-  else if (!large || tile == kSq) go(static_cast<Sq<F16, NP, false, false>*>(nullptr));
+  constexpr bool large = PL != 2;  // G in two planes comes with few rows only
+  if (tile == kFew) go(static_cast<Few<NP, false, false>*>(nullptr));
+  else if (!large || tile == kSq) go(static_cast<Sq<NP, false, false>*>(nullptr));
   else if constexpr (large) {
-    if (tile == kBig) go(static_cast<Big<F16, NP, false, false>*>(nullptr));
-    else if (tile == kDeep) go(static_cast<Deep<F16, NP, false, false>*>(nullptr));
-    else go(static_cast<Wide<F16, NP, false, false>*>(nullptr));
+    if (tile == kBig) go(static_cast<Big<NP, false, false>*>(nullptr));
+    else if (tile == kDeep) go(static_cast<Deep<NP, false, false>*>(nullptr));
+    else go(static_cast<Wide<NP, false, false>*>(nullptr));
   }
   check_launch();
 }
@@ -503,14 +483,14 @@ namespace {
 
 struct XentPlan {
   int kp, vpad, piece, tile, slots, gtile, dx_tile, dw_tile, dw_splits;
-  bool two;               // G in two planes
+  int planes;             // of G
   Split dx_split, dw_split;
   Extent dx;
   int64_t fwd_bytes, bwd_bytes;
   // offsets into the forward's workspace
-  int64_t o_wp, o_part, o_zlab, o_tie, o_lsum, o_csum, o_counts;
+  int64_t o_part, o_zlab, o_tie, o_lsum, o_csum, o_counts;
   // offsets into the backward's
-  int64_t b_wp, b_g, b_dx, b_dw, b_db;
+  int64_t b_g, b_dx, b_dw, b_db;
 };
 
 constexpr int64_t kGBytes = int64_t(512) << 20;  // G of one piece of the vocabulary
@@ -521,12 +501,12 @@ constexpr int kCountFrom = 12288;
 
 XentPlan xent_plan(int rows, int width, int classes, bool f32) {
   XentPlan q{};
-  const int np = f32 ? 3 : 1;
+  const int np = f32 ? 6 : 1;
   // bf16: one rounding of G to bf16 is one more of the same size as the gradients' own, and over many
   // rows their errors add up to 1.2 times that one's; with a few rows one element can make up a
   // gradient, and the sum reaches twice.  There the products only stream the weights, and a second plane
   // costs nothing.
-  q.two = f32 || rows <= kTwoRows;
+  q.planes = f32 ? 3 : rows <= kTwoRows ? 2 : 1;
   q.kp = int(up(width, 8));
   q.vpad = int(up(classes, 256));
   auto tile = [&](int cols) { return rows > 32 && rows <= kTwoRows ? kSq : choose_tile(rows, cols, width, np, false, false); };
@@ -538,7 +518,6 @@ XentPlan xent_plan(int rows, int width, int classes, bool f32) {
     at = up(at + bytes, 256);
     return o;
   };
-  q.o_wp = take(f32 ? int64_t(classes) * q.kp * 4 : 0);
   q.o_part = take(int64_t(q.slots) * rows * 8);
   q.o_zlab = take(int64_t(rows) * 4);
   q.o_tie = take(int64_t(rows) * 4);
@@ -548,9 +527,8 @@ XentPlan xent_plan(int rows, int width, int classes, bool f32) {
   q.o_counts = take(rows > kCountFrom ? (rows + kCountRows - 1) / kCountRows * int64_t(4) : 0);
   q.fwd_bytes = at;
   at = 0;
-  q.b_wp = take(f32 ? int64_t(classes) * q.kp * 4 : 0);
   // pieces of equal width, so that none of them is a remainder that fills a few CUs
-  const int64_t row_bytes = int64_t(rows) * (q.two ? 4 : 2);
+  const int64_t row_bytes = int64_t(rows) * 2 * q.planes;
   const int64_t most = std::max<int64_t>(256, kGBytes / row_bytes / 256 * 256);
   const int64_t pieces = (q.vpad + most - 1) / most;
   q.piece = int(up((q.vpad + pieces - 1) / pieces, 256));
@@ -592,28 +570,22 @@ std::vector<int64_t> linear_xent_sizes(int64_t rows, int64_t width, int64_t clas
   return {q.fwd_bytes, q.bwd_bytes, q.kp, q.vpad, int64_t(sizeof(XentDev))};
 }
 
-// ``keep``: what the backward needs (x's compact rows, bias32, inv, lab, stat, dev and, for fp32, w's
-// partial maxima), each its own allocation of the caller.
+// What the backward needs (x's compact rows xc, bias32, inv, lab, stat, dev), each its own allocation of the
+// caller.  ``wp`` (fp32): workspace for w's planes, [3][classes][width up to 8].
 void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr_t bias, int bias_dt, uintptr_t labels,
                      int64_t ignore, int64_t rows, int64_t width, int64_t classes, int64_t vocab, int dt, uintptr_t ws,
                      uintptr_t xc, uintptr_t bias32, uintptr_t inv, uintptr_t lab, uintptr_t stat, uintptr_t dev,
-                     uintptr_t amax, uintptr_t loss, uintptr_t correct, uintptr_t n_out, uintptr_t stream) {
+                     uintptr_t wp, uintptr_t loss, uintptr_t correct, uintptr_t n_out, uintptr_t stream) {
   check_xent(rows, width, classes, vocab);
   VODA_CHECK(dt == kF32 || dt == kBF16, "linear_xent: x must be fp32 or bf16");
   const bool f32 = dt == kF32;
   VODA_CHECK(f32 || (w % 16 == 0 && ldw % 8 == 0 && ldw >= up(width, 8)),
              "linear_xent: bf16 weight rows must be 16-byte aligned and whole 16-byte vectors");
-  VODA_CHECK(xc % 16 == 0 && ws % 256 == 0, "linear_xent: workspaces must be aligned");
+  VODA_CHECK(xc % 16 == 0 && ws % 256 == 0 && wp % 16 == 0 && (wp || !f32), "linear_xent: workspaces must be aligned");
   const XentPlan q = xent_plan(int(rows), int(width), int(classes), f32);
   hipStream_t st = as_stream(stream);
   uint8_t* base = reinterpret_cast<uint8_t*>(ws);
   XentDev* d = reinterpret_cast<XentDev*>(dev);
-  float* am = reinterpret_cast<float*>(amax);
-  if (f32) {
-    const Rows rw = {reinterpret_cast<const float*>(w), ldw, int(classes), int(width)};
-    gt::amax({reinterpret_cast<const float*>(x), ldx, int(rows), int(width)}, &rw, reinterpret_cast<const int64_t*>(labels),
-             ignore, int(classes), am, st);
-  }
   GatherArgs g{};
   g.x = reinterpret_cast<const void*>(x);
   g.ldx = ldx;
@@ -634,7 +606,6 @@ void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
   g.bias_bf16 = bias_dt == kBF16;
   g.bias32 = reinterpret_cast<float*>(bias32);
   g.bias_n = q.vpad;
-  g.amax = am;
   g.gather_blocks = int((rows + kGatherRows - 1) / kGatherRows);
   if (rows > kCountFrom) {
     int* counts = reinterpret_cast<int*>(base + q.o_counts);
@@ -650,12 +621,7 @@ void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
   LogitArgs p{};
   p.X = {g.xc, q.kp, g.plane, int(rows)};
   p.W = {reinterpret_cast<const uint16_t*>(w), ldw, 0, int(classes)};
-  if (f32) {
-    uint16_t* wp = reinterpret_cast<uint16_t*>(base + q.o_wp);
-    split({reinterpret_cast<const float*>(w), ldw, int(classes), int(width)}, wp, q.kp, classes * q.kp, am + kAmaxBlocks,
-          &d->inv_w, st);
-    p.W = {wp, q.kp, classes * q.kp, int(classes)};
-  }
+  if (f32) p.W = split({reinterpret_cast<const float*>(w), ldw, int(classes), int(width)}, wp, q.kp, st);
   p.width = q.kp;
   p.v0 = 0;
   p.v1 = int(classes);
@@ -665,8 +631,8 @@ void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
   p.part = reinterpret_cast<float2*>(base + q.o_part);
   p.zlab = reinterpret_cast<float*>(base + q.o_zlab);
   p.tie = reinterpret_cast<int*>(base + q.o_tie);
-  if (f32) launch_logits<true, false, true>(p, q.tile, st);
-  else launch_logits<false, false, false>(p, q.tile, st);
+  if (f32) launch_logits<6, false, 1>(p, q.tile, st);
+  else launch_logits<1, false, 1>(p, q.tile, st);
   auto join = [&](auto kernel, int per) {
     hipLaunchKernelGGL(kernel, dim3(unsigned((rows + per - 1) / per)), dim3(64 * kJoinWaves), 0, st, p.part, q.slots, int(rows),
                        tile_slot(q.tile), p.zlab, p.tie, g.lab, d, reinterpret_cast<float2*>(stat),
@@ -682,7 +648,7 @@ void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
 // ``db_dt`` (added to when ``accumulate``); each of dx, dw and db may be null.
 void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int64_t classes, int64_t vocab, int dt,
                      uintptr_t ws, uintptr_t xc, uintptr_t bias32, uintptr_t inv, uintptr_t lab, uintptr_t stat,
-                     uintptr_t dev, uintptr_t amax, uintptr_t gloss, uintptr_t dx, uintptr_t dw, int64_t ldd,
+                     uintptr_t dev, uintptr_t wp, uintptr_t gloss, uintptr_t dx, uintptr_t dw, int64_t ldd,
                      uintptr_t db, int grad_dt, int db_dt, bool accumulate, uintptr_t stream) {
   check_xent(rows, width, classes, vocab);
   VODA_CHECK(dt == kF32 || dt == kBF16, "linear_xent: x must be fp32 or bf16");
@@ -691,7 +657,7 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
   const bool f32 = dt == kF32;
   VODA_CHECK(f32 || (w % 16 == 0 && ldw % 8 == 0 && ldw >= up(width, 8)),
              "linear_xent: bf16 weight rows must be 16-byte aligned and whole 16-byte vectors");
-  VODA_CHECK(xc % 16 == 0 && ws % 256 == 0, "linear_xent: workspaces must be aligned");
+  VODA_CHECK(xc % 16 == 0 && ws % 256 == 0 && wp % 16 == 0 && (wp || !f32), "linear_xent: workspaces must be aligned");
   const XentPlan q = xent_plan(int(rows), int(width), int(classes), f32);
   hipStream_t st = as_stream(stream);
   uint8_t* base = reinterpret_cast<uint8_t*>(ws);
@@ -699,12 +665,7 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
   LogitArgs p{};
   p.X = {reinterpret_cast<const uint16_t*>(xc), q.kp, rows * q.kp, int(rows)};
   p.W = {reinterpret_cast<const uint16_t*>(w), ldw, 0, int(classes)};
-  if (f32) {
-    uint16_t* wp = reinterpret_cast<uint16_t*>(base + q.b_wp);
-    split({reinterpret_cast<const float*>(w), ldw, int(classes), int(width)}, wp, q.kp, classes * q.kp,
-          reinterpret_cast<const float*>(amax) + kAmaxBlocks, &d->inv_w, st);
-    p.W = {wp, q.kp, classes * q.kp, int(classes)};
-  }
+  if (f32) p.W = split({reinterpret_cast<const float*>(w), ldw, int(classes), int(width)}, wp, q.kp, st);
   p.width = q.kp;
   p.bias32 = reinterpret_cast<const float*>(bias32);
   p.dev = d;
@@ -716,7 +677,6 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
   p.sums = db ? reinterpret_cast<float*>(base + q.b_db) : nullptr;
   p.sums_ld = q.piece;
   Emit e{};
-  e.f = f32 ? 1.f / kGScale : 1.f;
   e.gl = reinterpret_cast<const float*>(gloss);
   e.gn = &d->n;
   const int gsz = grad_dt == kF32 ? 4 : 2;
@@ -728,7 +688,6 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
   x.slab = reinterpret_cast<float*>(base + q.b_dx);
   x.lds = q.kp;
   x.e = e;
-  x.e.fj = f32 ? &d->inv_w : nullptr;
   x.e.out = reinterpret_cast<void*>(dx);
   x.e.ldo = width;
   x.e.bf16 = !f32;
@@ -742,7 +701,6 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
     c.bi = tile_bi(q.gtile);
     c.per = tile_wi(q.gtile);
     c.bf16 = db_dt == kBF16;
-    c.e.f = 1.f;
     c.e.gl = e.gl;
     c.e.gn = e.gn;
     c.e.accumulate = accumulate;
@@ -751,17 +709,17 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
     const int v1 = int(std::min<int64_t>(classes, v0 + q.piece));
     p.v0 = v0;
     p.v1 = v1;
-    if (f32) launch_logits<true, true, true>(p, q.gtile, st);
-    else if (q.two) launch_logits<false, true, true>(p, q.gtile, st);
-    else launch_logits<false, true, false>(p, q.gtile, st);
+    if (f32) launch_logits<6, true, 3>(p, q.gtile, st);
+    else if (q.planes == 2) launch_logits<1, true, 2>(p, q.gtile, st);
+    else launch_logits<1, true, 1>(p, q.gtile, st);
     if (dx) {
       x.J = {p.W.p + int64_t(v0) * p.W.ld, p.W.ld, p.W.plane, int(up(width, 8))};
       x.nk = v1 - v0;
       x.add = v0 > 0;
-      if (f32) gemm<true, 3, false, true, false>(q.dx_tile, x, q.dx.grid, st);
-      else if (!q.two) gemm<false, 1, false, true, false>(q.dx_tile, x, q.dx.grid, st);
-      else if (q.dx_tile == kFew) launch_gemm<Few<false, 2, false, true>, false>(x, q.dx.grid, st);
-      else launch_gemm<Sq<false, 2, false, true>, false>(x, q.dx.grid, st);
+      if (f32) gemm<6, false, true, false>(q.dx_tile, x, q.dx.grid, st);
+      else if (q.planes == 1) gemm<1, false, true, false>(q.dx_tile, x, q.dx.grid, st);
+      else if (q.dx_tile == kFew) launch_gemm<Few<2, false, true>, false>(x, q.dx.grid, st);
+      else launch_gemm<Sq<2, false, true>, false>(x, q.dx.grid, st);
     }
     if (dw) {
       GemmArgs a{};
@@ -771,7 +729,6 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
       a.nk = int(rows);
       a.split = q.dw_split;
       a.e = e;
-      a.e.fj = f32 ? &d->inv_x : nullptr;
       a.e.out = reinterpret_cast<void*>(dw + uintptr_t(int64_t(v0) * ldd * gsz));
       a.e.ldo = ldd;
       a.e.bf16 = grad_dt == kBF16;
@@ -783,9 +740,9 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
         a.lds = q.kp;
       }
       const int64_t grid = tiles_of(q.dw_tile, v1 - v0, width) * q.dw_splits;
-      if (f32) gemm<true, 3, true, true, false>(q.dw_tile, a, grid, st);
-      else if (q.two) launch_gemm<Sq<false, 2, true, true>, false>(a, grid, st);
-      else gemm<false, 1, true, true, false>(q.dw_tile, a, grid, st);
+      if (f32) gemm<6, true, true, false>(q.dw_tile, a, grid, st);
+      else if (q.planes == 2) launch_gemm<Sq<2, true, true>, false>(a, grid, st);
+      else gemm<1, true, true, false>(q.dw_tile, a, grid, st);
       if (a.slab) finish(q.dw_tile, a, a.I.n, nullptr, {}, st);
     }
     c.n = v1 - v0;

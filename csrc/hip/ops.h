@@ -65,23 +65,23 @@ std::vector<int64_t> linear_xent_sizes(int64_t rows, int64_t width, int64_t clas
 void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr_t bias, int bias_dt, uintptr_t labels,
                      int64_t ignore, int64_t rows, int64_t width, int64_t classes, int64_t vocab, int dt, uintptr_t ws,
                      uintptr_t xc, uintptr_t bias32, uintptr_t inv, uintptr_t lab, uintptr_t stat, uintptr_t dev,
-                     uintptr_t amax, uintptr_t loss, uintptr_t correct, uintptr_t n_out, uintptr_t stream);
+                     uintptr_t wp, uintptr_t loss, uintptr_t correct, uintptr_t n_out, uintptr_t stream);
 void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int64_t classes, int64_t vocab, int dt,
                      uintptr_t ws, uintptr_t xc, uintptr_t bias32, uintptr_t inv, uintptr_t lab, uintptr_t stat,
-                     uintptr_t dev, uintptr_t amax, uintptr_t gloss, uintptr_t dx, uintptr_t dw, int64_t ldd,
+                     uintptr_t dev, uintptr_t wp, uintptr_t gloss, uintptr_t dx, uintptr_t dw, int64_t ldd,
                      uintptr_t db, int grad_dt, int db_dt, bool accumulate, uintptr_t stream);
 
 // ---- Linear with an 8-bit input checkpoint (act8.hip) ----
-std::vector<int64_t> linear_act8_sizes(int64_t rows, int64_t width, int64_t out, int dt, bool copy);
+std::vector<int64_t> linear_act8_sizes(int64_t rows, int64_t width, int64_t out, int dt, bool copy, bool gelu);
 void act8_pack(uintptr_t x, int64_t ldx, int64_t rows, int64_t width, int dt, uintptr_t qp, uintptr_t qs,
                uintptr_t stream);
 void act8_values(uintptr_t qp, uintptr_t qs, int64_t rows, int64_t width, int dt, uintptr_t out, uintptr_t stream);
 void linear_act8_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr_t bias, int bias_dt, uintptr_t y,
                      uintptr_t qp, uintptr_t qs, int64_t rows, int64_t width, int64_t out, int dt, bool gelu, bool copy,
-                     uintptr_t amax, uintptr_t ws, uintptr_t stream);
+                     uintptr_t wp, uintptr_t ws, uintptr_t stream);
 void linear_act8_bwd(uintptr_t dy, int64_t ldy, uintptr_t w, int64_t ldw, uintptr_t qp, uintptr_t qs, uintptr_t dx,
                      bool dx_add, uintptr_t dw, int64_t ldd, uintptr_t db, int grad_dt, int db_dt, bool accumulate, int64_t rows,
-                     int64_t width, int64_t out, int dt, bool gelu, uintptr_t amax, uintptr_t ws, uintptr_t stream);
+                     int64_t width, int64_t out, int dt, bool gelu, uintptr_t wp, uintptr_t ws, uintptr_t stream);
 
 // ---- fused softmax cross-entropy (xent.hip) ----
 // logits [rows][ld] (bf16 / fp32, 16-byte rows), V <= ld valid classes; per-row lse / loss /

@@ -9,7 +9,7 @@ import torch
 from vodascheduler_amd.ops.linear_xent import linear_cross_entropy
 
 from test_linear_xent_gpu import _check, _inputs
-from xent_bounds import U
+from xent_bounds import U, formulas, within
 
 pytestmark = pytest.mark.gpu
 
@@ -95,3 +95,86 @@ def test_a_confident_row_s_loss_is_not_negative(dtype):
             x *= 2.0 ** (seed // 2)
         y = (x.float() @ w.float().t()).argmax(1)
         assert float(linear_cross_entropy(x, w, y)[0]) >= 0.0
+
+
+def _subset(x, w, b, y, C, keep):
+    """The formulas' (dx, dw, db) of some rows alone, in the mean over all of them, and their bounds less the
+    one term in them that is no fp32 error (2^-49 of each element of x, for each row)."""
+    rows, n = x.shape[0], keep.numel()
+    (_, _, _, dx, dw, db), (_, bdx, bdw, bdb) = formulas(x[keep], w, b, y[keep], C, -100, n / rows)
+    bdw[:C] -= 2.0 ** -49 / rows * x[keep].detach().double().abs().sum(0)
+    bdx -= 2.0 ** -49 / rows * w[:C].detach().double().abs().sum(0)
+    return (dx, dw, db), (bdx + 1e-35, bdw + 1e-35, bdb)
+
+
+@pytest.mark.parametrize("big", [1e10, 1e16, 2.0 ** 60, 1e30])
+@pytest.mark.parametrize("rows,K,C", [(20, 64, 300), (200, 203, 500), (600, 264, 1000)])
+def test_one_labelled_row_of_another_size(rows, K, C, big):
+    """fp32: its logits are far apart, so its softmax is one class; the other rows' gradients, and the weight's of
+    all other classes, are as ever."""
+    x, w, b, y = _inputs(rows, K, C, C, torch.float32, bias=True, seed=rows, ignored=0.0)
+    with torch.no_grad():
+        x[3] *= big
+    loss, _, n = linear_cross_entropy(x, w, y, b)
+    gx, gw, gb = torch.autograd.grad(loss, (x, w, b))
+    keep = torch.tensor([r for r in range(rows) if r != 3], device=DEV)
+    (dx, dw, db), (bdx, bdw, bdb) = _subset(x, w, b, y, C, keep)
+    within(gx[keep], dx, bdx, "dx")
+    z = x[3].detach().double() @ w.detach().double().t()
+    apart = (z.amax() - z) > 200  # certain: its softmax there is 0, in fp32 too
+    apart[y[3]] = False
+    assert int(apart.sum()) >= C - 3
+    within(gw[apart], dw[apart], bdw[apart], "dw")
+    within(gb[apart], db[apart], bdb[apart], "db")
+
+
+@pytest.mark.parametrize("big", [1e16, 1e30])
+def test_one_class_and_one_feature_of_another_size(big):
+    """fp32: weights of a class that its bias masks, a feature that no class reads."""
+    rows, K, C = 300, 72, 400
+    x, w, b, y = _inputs(rows, K, C, C, torch.float32, bias=True, ignored=0.1)
+    y = torch.where(y == 9, 10, y)
+    with torch.no_grad():
+        w[9] *= big
+        b[9] = float("-inf")
+        w[:, 5] = 0.0
+        x[:, 5] *= big
+        w[9, 5] = 0.0
+    loss, _, n = linear_cross_entropy(x, w, y, b)
+    gx, gw, gb = torch.autograd.grad(loss, (x, w, b))
+    with torch.no_grad():
+        w[9] = 0.0  # takes no part: any weights give the same
+    keep = (y >= 0).nonzero()[:, 0]
+    (dx, dw, db), (bdx, bdw, bdb) = _subset(x, w, b, y, C, keep)
+    scale = rows / keep.numel()
+    assert torch.isfinite(loss)
+    within(gx[keep], dx * scale, bdx * scale, "dx")
+    within(gw, dw * scale, bdw * scale, "dw")
+    within(gb, db * scale, bdb * scale, "db")
+
+
+@pytest.mark.parametrize("rows", [20, 300])
+def test_gradients_of_unlikely_classes(rows):
+    """fp32: classes that a bias makes unlikely (2^-40 to 2^-90 of the softmax) get gradients right to
+    their own size."""
+    K, C = 64, 400
+    x, w, b, y = _inputs(rows, K, C, C, torch.float32, bias=True, ignored=0.0)
+    y = y % 100
+    with torch.no_grad():
+        b[100:] -= torch.arange(300, device=DEV) * 0.1 + 28
+    loss, _, _ = linear_cross_entropy(x, w, y, b)
+    gx, gw, gb = torch.autograd.grad(loss, (x, w, b))
+    # bounds as the formulas', summed from the relative terms alone: the difference that _subset takes, of
+    # numbers near 2^-49 in fp64, is good to 2^-102 only, and these classes' terms lie below 2^-24 2^-90
+    X, W, B = (t.detach().double() for t in (x, w, b))
+    z = X @ W.t() + B
+    gap = z.amax(1, keepdim=True) - z
+    p = torch.softmax(z, 1)
+    G = p - torch.nn.functional.one_hot(y, C)
+    ez = (K + 4) * U * (X.abs() @ W.abs().t()) + 4 * U * (z.abs() + B.abs())
+    far = ez + ez.amax(1, keepdim=True)
+    dG = p * (far + 4 * U * gap + (C + 16) * U + (p * far).sum(1, keepdim=True)) + 3 * U * G.abs() + U * p
+    bound = (dG.t() @ X.abs() + (rows + 68) * U * (G.abs().t() @ X.abs())) / rows
+    want = G.t() @ X / rows
+    assert float(p[:, 100:].amax()) < 2.0 ** -30 and float(p[:, 399].amax()) < 2.0 ** -75
+    within(gw, want, bound + 9 * U * want.abs(), "dw")

@@ -14,8 +14,9 @@ BERT-base's FFN keeps 0.79 + 3.17 KB a token this way instead of 1.5 + 6 + 6 KB 
 least 2^-126) that keeps the block's largest finite value within 448, so the only rounding is e4m3's
 (what would round past fp32's range stays at 240 2^120); infinities and NaN come back as NaN.
 
-Types: bf16 or fp32 ``x`` and ``weight`` alike (fp32 at fp32 accuracy for finite inputs; an infinite one gives
-NaN or infinity where it takes part), ``bias`` of either.  Any sizes and row strides.  Gradients that the
+Types: bf16 or fp32 ``x`` and ``weight`` alike (fp32 at fp32 accuracy wherever the products stay
+finite: three bf16 planes hold any finite element by itself; an infinite one gives NaN or infinity where it
+takes part), ``bias`` of either.  Any sizes and row strides.  Gradients that the
 fused optimizer owns go straight into its flat buffer (ops/dense.py's contract).  Without a gradient of
 ``weight`` and without the GELU no checkpoint is kept.  Only first derivatives.  ``Act8Linear`` is the
 layer, with ``FusedLinear``'s parameters.
@@ -104,6 +105,11 @@ def _check_float(who: str, x: torch.Tensor) -> None:
         raise TypeError(f"{who}: fp32 or bf16, got {x.dtype}")
 
 
+def _planes(w: torch.Tensor) -> torch.Tensor:
+    """Workspace for the three planes of an fp32 weight."""
+    return torch.empty(6 * w.shape[0] * (-(-w.shape[1] // 8) * 8), dtype=torch.uint8, device=w.device)
+
+
 class _LinearAct8Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, gelu, sink_in, bias_handoff):
@@ -121,30 +127,30 @@ class _LinearAct8Fn(torch.autograd.Function):
             y = F.linear(F.gelu(wide, approximate="tanh") if gelu else wide, weight.float(),
                          None if bias is None else bias.float()).to(x.dtype)
             q, s = _pack_ref(x) if keep else (None, None)
-            ctx.save_for_backward(weight, q, s, None)
+            ctx.save_for_backward(weight, q, s)
             return y
         h = N.hip()
         with _on(dev):
             dt = N.dtype_code(x.dtype)
             # bf16 rows of whole aligned vectors go into the product as they are
             copy = bool(f32 or gelu or x.data_ptr() % 16 or x.stride(0) % 8 or K % 8)
-            nf, _, kq, _ = h.linear_act8_sizes(rows, K, out, dt, copy)
+            nf, _, kq, _ = h.linear_act8_sizes(rows, K, out, dt, copy, gelu)
             w = weight if f32 else _rows16(weight)
             ws = torch.empty(max(nf, 256), dtype=torch.uint8, device=dev)
             y = torch.empty(rows, out, dtype=x.dtype, device=dev)
             q = torch.empty(rows, kq, dtype=_F8, device=dev) if keep else None
             s = torch.empty(rows, kq // BLOCK, dtype=_E8, device=dev) if keep else None
-            amax = torch.empty(2048, dtype=torch.float32, device=dev) if f32 else None
+            planes = _planes(w) if f32 else None
             h.linear_act8_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), N.ptr(bias),
                               N.DT_F32 if bias is None else N.dtype_code(bias.dtype), y.data_ptr(), N.ptr(q),
-                              N.ptr(s), rows, K, out, dt, gelu, copy, N.ptr(amax), ws.data_ptr(), N.stream_of(x))
-        ctx.save_for_backward(weight, q, s, amax)
+                              N.ptr(s), rows, K, out, dt, gelu, copy, N.ptr(planes), ws.data_ptr(), N.stream_of(x))
+        ctx.save_for_backward(weight, q, s)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        weight, q, s, amax = ctx.saved_tensors
+        weight, q, s = ctx.saved_tensors
         rows, K, out = ctx.dims
         wp, bp = ctx.params
         gelu, dt = ctx.gelu, ctx.x_dtype
@@ -182,7 +188,7 @@ class _LinearAct8Fn(torch.autograd.Function):
         with _on(dev):
             if not f32:
                 dy = _rows16(dy)
-            _, nb, _, _ = h.linear_act8_sizes(rows, K, out, N.dtype_code(dt), True)
+            _, nb, _, _ = h.linear_act8_sizes(rows, K, out, N.dtype_code(dt), True, gelu)
             w = weight if f32 else _rows16(weight)
             if need_x:
                 dx = acc if acc is not None else torch.empty(rows, K, dtype=dt, device=dev)
@@ -198,12 +204,13 @@ class _LinearAct8Fn(torch.autograd.Function):
                 colsum_accumulate_(dy, db)
                 db = db[:out].to(bp.dtype)
             ws = torch.empty(max(nb, 256), dtype=torch.uint8, device=dev)
+            planes = _planes(w) if f32 and need_x else None
             if need_x or need_w:
                 h.linear_act8_bwd(dy.data_ptr(), dy.stride(0), w.data_ptr(), w.stride(0), N.ptr(q), N.ptr(s),
                                   N.ptr(dx), acc is not None, N.ptr(dw), dw.stride(0) if need_w else K,
                                   N.ptr(db) if need_w else 0, N.dtype_code(dw.dtype) if need_w else N.DT_F32,
                                   N.dtype_code(db.dtype) if db is not None else N.DT_F32, bool(direct), rows, K, out,
-                                  N.dtype_code(dt), gelu, N.ptr(amax), ws.data_ptr(), N.stream_of(dy))
+                                  N.dtype_code(dt), gelu, N.ptr(planes), ws.data_ptr(), N.stream_of(dy))
         if direct:
             _ready(wp)
             if need_b:

@@ -16,8 +16,8 @@ hipGraph-capturable).
   padding) reaches the loss or a gradient.  A loss with every row ignored is 0 (PyTorch: NaN).
 * ``weight`` rows from ``num_classes`` on are padding: outside the softmax, gradient zero.  A bias of
   -inf takes a class out.
-* Types: bf16 or fp32 ``x`` and ``weight`` alike, ``bias`` of either; fp32 runs at fp32 accuracy (two fp16
-  planes an operand) for finite inputs.  An infinite or NaN input of a labelled row or of a class's
+* Types: bf16 or fp32 ``x`` and ``weight`` alike, ``bias`` of either; fp32 runs at fp32 accuracy (three
+  bf16 planes an operand, which hold any finite element by itself) wherever the products stay finite.  An infinite or NaN input of a labelled row or of a class's
   weights makes the loss NaN or infinite.  Anything else is refused on a GPU.
 * Gradients of a weight and bias that the fused optimizer owns are summed straight into its flat
   buffer (ops/dense.py's contract), else returned.  Sums have a fixed order: the same call gives the
@@ -93,22 +93,23 @@ class _LinearXentFn(torch.autograd.Function):
             w = weight if f32 else _rows16(weight)
             ws = torch.empty(max(nf, 256), dtype=torch.uint8, device=dev)
             # what the backward needs, in one buffer, each part 256-byte aligned: x's compact rows, the
-            # padded bias, each row's place, the labels, (max, 1 / sum), the device scalars, w's maxima
+            # padded bias, each row's place, the labels, (max, 1 / sum), the device scalars
             at = [0]
-            for n in ((4 if f32 else 2) * rows * kp, 4 * vpad, 4 * rows, 4 * rows, 8 * rows, nd, 8192 if f32 else 0):
+            for n in ((6 if f32 else 2) * rows * kp, 4 * vpad, 4 * rows, 4 * rows, 8 * rows, nd):
                 at.append(at[-1] + -(-n // 256) * 256)
             keep = torch.empty(at[-1], dtype=torch.uint8, device=dev)
             p = keep.data_ptr()
             p = [p + a for a in at]
+            planes = torch.empty(6 * C * kp, dtype=torch.uint8, device=dev) if f32 else None
             loss = torch.empty((), dtype=torch.float32, device=dev)
             correct = torch.empty((), dtype=torch.int64, device=dev)
             n = torch.empty((), dtype=torch.int64, device=dev)
             h.linear_xent_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), N.ptr(bias),
                               N.DT_F32 if bias is None else N.dtype_code(bias.dtype), labels.data_ptr(), ignore, rows,
                               K, C, V, N.dtype_code(x.dtype), ws.data_ptr(), p[0], p[1], p[2], p[3], p[4], p[5],
-                              p[6], loss.data_ptr(), correct.data_ptr(), n.data_ptr(), N.stream_of(x))
+                              N.ptr(planes), loss.data_ptr(), correct.data_ptr(), n.data_ptr(), N.stream_of(x))
         ctx.save_for_backward(weight, keep)
-        ctx.at, ctx.dims, ctx.nb = at, (rows, K, C, V), nb
+        ctx.at, ctx.dims, ctx.nb, ctx.kp = at, (rows, K, C, V), nb, kp
         ctx.params = (weight, bias)
         ctx.x_dtype = x.dtype
         ctx.mark_non_differentiable(correct, n)
@@ -145,8 +146,9 @@ class _LinearXentFn(torch.autograd.Function):
                     if t is not None:
                         t[C:].zero_()
             ws = torch.empty(max(ctx.nb, 256), dtype=torch.uint8, device=dev)
+            planes = torch.empty(6 * C * ctx.kp, dtype=torch.uint8, device=dev) if f32 else None
             N.hip().linear_xent_bwd(w.data_ptr(), w.stride(0), rows, K, C, V, N.dtype_code(ctx.x_dtype), ws.data_ptr(),
-                                    p[0], p[1], p[2], p[3], p[4], p[5], p[6], gloss.data_ptr(), N.ptr(dx),
+                                    p[0], p[1], p[2], p[3], p[4], p[5], N.ptr(planes), gloss.data_ptr(), N.ptr(dx),
                                     N.ptr(dw), dw.stride(0) if need_w else K, N.ptr(db),
                                     N.dtype_code(dw.dtype) if need_w else N.DT_F32,
                                     N.dtype_code(db.dtype) if need_b else N.DT_F32, bool(direct), N.stream_of(weight))
