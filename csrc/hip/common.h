@@ -113,19 +113,19 @@ constexpr float kGeluC = 0.044715f;
 constexpr float kGeluA = -2.f * kGeluK * 1.4426950408889634f;
 constexpr float kGeluB = kGeluA * kGeluC;
 
-// exponent clamped at 64 so that e stays finite (s = 2^-64 then; e s = 1 - s exactly enough)
-__device__ __forceinline__ float gelu_exp(float h, float h2) {
-  return __builtin_amdgcn_exp2f(fminf(h * __builtin_fmaf(kGeluB, h2, kGeluA), 64.f));
+// For any finite h: where B h^2 is past fp32's range the exponential is infinite or 0, and s 0 or 1.
+__device__ __forceinline__ float gelu_tanh_f(float h) {
+  return h * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(h * __builtin_fmaf(kGeluB, h * h, kGeluA)));
 }
 
-__device__ __forceinline__ float gelu_tanh_f(float h) { return h * __builtin_amdgcn_rcpf(1.f + gelu_exp(h, h * h)); }
-
+// The slope at 9 is 1 to 2^-90 and at -9 0 to 2^-88, so h is clamped there: e stays finite and the cubic's terms
+// small.  The clamp drops a NaN; 0 h brings it back.
 __device__ __forceinline__ float gelu_tanh_grad(float h) {
-  const float h2 = h * h;
-  const float e = gelu_exp(h, h2);
+  const float c = __builtin_amdgcn_fmed3f(h, -9.f, 9.f), c2 = c * c;
+  const float e = __builtin_amdgcn_exp2f(c * __builtin_fmaf(kGeluB, c2, kGeluA));
   const float s = __builtin_amdgcn_rcpf(1.f + e);
   // s (1 - s) = e s^2: no cancellation as s -> 1
-  return __builtin_fmaf(2.f * kGeluK * h * e * s * s, __builtin_fmaf(3.f * kGeluC, h2, 1.f), s);
+  return __builtin_fmaf(2.f * kGeluK * c * e * s * s, __builtin_fmaf(3.f * kGeluC, c2, 1.f), __builtin_fmaf(0.f, h, s));
 }
 
 

@@ -53,7 +53,8 @@ def gelu_tanh_ref(h: torch.Tensor) -> torch.Tensor:
 
 def gelu_tanh_grad_ref(h: torch.Tensor) -> torch.Tensor:
     """d gelu_tanh / dh (fp32, or fp64 for fp64 input)."""
-    h = h if h.dtype == torch.float64 else h.float()
+    # past 20 it is 0 or 1 in fp64 too, while h^3 may be infinite
+    h = (h if h.dtype == torch.float64 else h.float()).clamp(-20, 20)
     c = math.sqrt(2.0 / math.pi)
     u = c * (h + 0.044715 * h ** 3)
     t = torch.tanh(u)
