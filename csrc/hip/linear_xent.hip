@@ -463,16 +463,18 @@ void launch_logits(LogitArgs& p, int tile, hipStream_t st) {
   auto go = [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     hipLaunchKernelGGL((xent_logits_kernel<T, BWD, PL>), grid, dim3(T::kThreads), 0, st, p);
+    check_launch();
   };
-  constexpr bool large = PL != 2;  // G in two planes comes with few rows only
-  if (tile == kFew) go(static_cast<Few<NP, false, false>*>(nullptr));
-  else if (!large || tile == kSq) go(static_cast<Sq<NP, false, false>*>(nullptr));
-  else if constexpr (large) {
-    if (tile == kBig) go(static_cast<Big<NP, false, false>*>(nullptr));
-    else if (tile == kDeep) go(static_cast<Deep<NP, false, false>*>(nullptr));
-    else go(static_cast<Wide<NP, false, false>*>(nullptr));
+  // bf16's G has two planes with few rows only, one with more than kFew and kSq are for
+  constexpr bool few = !(BWD && PL == 1), large = !(BWD && PL == 2);
+  if constexpr (few)
+    if (tile == kFew) return go(static_cast<Few<NP, false, false>*>(nullptr));
+  if constexpr (large) {
+    if (tile == kBig) return go(static_cast<Big<NP, false, false>*>(nullptr));
+    if (tile == kDeep) return go(static_cast<Deep<NP, false, false>*>(nullptr));
+    if (tile == kWide) return go(static_cast<Wide<NP, false, false>*>(nullptr));
   }
-  check_launch();
+  go(static_cast<Sq<NP, false, false>*>(nullptr));
 }
 
 }  // namespace
@@ -558,6 +560,21 @@ void check_xent(int64_t rows, int64_t width, int64_t classes, int64_t vocab) {
   // a launch holds less than 2^32 threads: 256 x 128 a workgroup of 256, eight outputs a thread of the finish
   VODA_CHECK(up(rows, 128) / 128 * (up(classes, 256) / 256) < (1 << 24), "linear_xent: rows x vocabulary too large");
   VODA_CHECK(rows * up(width, 8) <= (int64_t(1) << 34), "linear_xent: rows x width too large");
+}
+
+}  // namespace
+
+namespace {
+
+// G w, on one of the tiles that the plan takes for dx: kFew needs 32 rows at most, where bf16's G has two
+// planes, kWide 1024 at least, where it has one
+template <int NP>
+void dx_gemm(int tile, const GemmArgs& p, int64_t grid, hipStream_t st) {
+  if constexpr (NP != 1)
+    if (tile == kFew) return launch_gemm<Few<NP, false, true>, false>(p, grid, st);
+  if constexpr (NP != 2)
+    if (tile == kWide) return launch_gemm<Wide<NP, false, true>, false>(p, grid, st);
+  launch_gemm<Sq<NP, false, true>, false>(p, grid, st);
 }
 
 }  // namespace
@@ -716,10 +733,9 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
       x.J = {p.W.p + int64_t(v0) * p.W.ld, p.W.ld, p.W.plane, int(up(width, 8))};
       x.nk = v1 - v0;
       x.add = v0 > 0;
-      if (f32) gemm<6, false, true, false>(q.dx_tile, x, q.dx.grid, st);
-      else if (q.planes == 1) gemm<1, false, true, false>(q.dx_tile, x, q.dx.grid, st);
-      else if (q.dx_tile == kFew) launch_gemm<Few<2, false, true>, false>(x, q.dx.grid, st);
-      else launch_gemm<Sq<2, false, true>, false>(x, q.dx.grid, st);
+      if (f32) dx_gemm<6>(q.dx_tile, x, q.dx.grid, st);
+      else if (q.planes == 1) dx_gemm<1>(q.dx_tile, x, q.dx.grid, st);
+      else dx_gemm<2>(q.dx_tile, x, q.dx.grid, st);
     }
     if (dw) {
       GemmArgs a{};
