@@ -365,7 +365,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void xent_join_kernel(const float2
                                                                     int* __restrict__ csum, float* __restrict__ loss,
                                                                     int64_t* __restrict__ correct) {
   constexpr int kJoinGroups = 64 * kJoinWaves / kJoinRows, kQ = 64 / kJoinRows;
-  __shared__ float sm[kJoinGroups][kJoinRows], ss[kJoinGroups][kJoinRows], sl[kJoinGroups][kJoinRows];
+  __shared__ float sm[kJoinGroups][kJoinRows], ss[kJoinGroups][kJoinRows];
+  __shared__ int sl[kJoinGroups][kJoinRows];
   __shared__ int last;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int row = threadIdx.x % kJoinRows, grp = threadIdx.x / kJoinRows;
@@ -373,7 +374,9 @@ __global__ __launch_bounds__(64 * kJoinWaves) void xent_join_kernel(const float2
   const int i = blockIdx.x * kJoinRows + row;
   const bool live = i < n;
   const int yslot = live ? lab[i] / slot_cols : 0;
-  float m = -INFINITY, s = 0.f, before = -INFINITY;  // before: largest of the slots in front of the label's
+  const float z = live ? zlab[i] : 0.f;
+  float m = -INFINITY, s = 0.f;
+  int beaten = 0;  // a slot in front of the label's holds a logit as large
   if (live) {
 #pragma unroll 4
     for (int k = grp; k < slots; k += kJoinGroups) {
@@ -382,27 +385,27 @@ __global__ __launch_bounds__(64 * kJoinWaves) void xent_join_kernel(const float2
       const float at = nm == -INFINITY ? 0.f : nm;
       s = s * __builtin_amdgcn_exp2f((m - at) * kLog2e) + v.y * __builtin_amdgcn_exp2f((v.x - at) * kLog2e);
       m = nm;
-      if (k < yslot) before = fmaxf(before, v.x);
+      beaten |= k < yslot && v.x >= z;
     }
   }
   sm[grp][row] = m;
   ss[grp][row] = s;
-  sl[grp][row] = before;
+  sl[grp][row] = beaten;
   __syncthreads();
   if (wave == 0) {
     // kQ lanes a row, each a share of the groups
     const int q = lane / kJoinRows;
     m = -INFINITY;
-    before = -INFINITY;
+    beaten = 0;
 #pragma unroll
     for (int k = 0; k < kJoinGroups / kQ; ++k) {
       m = fmaxf(m, sm[kQ * k + q][row]);
-      before = fmaxf(before, sl[kQ * k + q][row]);
+      beaten |= sl[kQ * k + q][row];
     }
 #pragma unroll
     for (int o = kJoinRows; o < 64; o <<= 1) {
       m = fmaxf(m, __shfl_xor(m, o, 64));
-      before = fmaxf(before, __shfl_xor(before, o, 64));
+      beaten |= __shfl_xor(beaten, o, 64);
     }
     const float at = m == -INFINITY ? 0.f : m;
     s = 0.f;
@@ -414,11 +417,10 @@ __global__ __launch_bounds__(64 * kJoinWaves) void xent_join_kernel(const float2
     double l = 0.0;
     int ok = 0;
     if (live && q == 0) {
-      const float z = zlab[i];
       stat[i] = make_float2(m, 1.f / s);
       // (max - z) first: exact where the label's logit is the largest or near it
       l = double(m - z) + double(logf(s));
-      ok = z == m && before < z && !tie[i] && s == s;
+      ok = z == m && !beaten && !tie[i] && s == s;
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {

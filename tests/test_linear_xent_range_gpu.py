@@ -178,3 +178,20 @@ def test_gradients_of_unlikely_classes(rows):
     want = G.t() @ X / rows
     assert float(p[:, 100:].amax()) < 2.0 ** -30 and float(p[:, 399].amax()) < 2.0 ** -75
     within(gw, want, bound + 9 * U * want.abs(), "dw")
+
+
+@pytest.mark.parametrize("rows", [1, 3, 40, 200, 1100])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_first_of_nothing_but_masks(dtype, rows):
+    """Every class at -inf: no loss, and the first maximum is class 0, as argmax has it."""
+    x, w, b, y = _inputs(rows, 48, 700, 690, dtype, bias=True, ignored=0.1)
+    y = torch.where(y < 0, y, torch.where(torch.arange(rows, device=DEV) % 3 == 0, 0, y))
+    with torch.no_grad():
+        b[:] = float("-inf")
+    loss, correct, n = linear_cross_entropy(x, w, y, b, 690)
+    assert torch.isnan(loss) or int(n) == 0
+    assert int(correct) == int((y == 0).sum())
+    with torch.no_grad():  # one class left, behind several slots of masks
+        b[600] = 0.0
+    y = torch.where(y == 0, 600, torch.where(y == 600, 5, y))
+    assert int(linear_cross_entropy(x, w, y, b, 690)[1]) == int((y == 600).sum())
