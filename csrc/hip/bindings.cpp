@@ -46,7 +46,8 @@ PYBIND11_MODULE(_vodahip, m) {
   m.def("masked_softmax_bwd", &masked_softmax_bwd);
   m.def("xent_fwd", &xent_fwd);
   m.def("xent_bwd", &xent_bwd);
-  m.def("linear_xent_sizes", &linear_xent_sizes);
+  m.def("linear_xent_sizes", &linear_xent_sizes, py::arg("rows"), py::arg("width"), py::arg("classes"), py::arg("vocab"),
+        py::arg("f32"), py::arg("g_bytes") = int64_t(512) << 20);
   m.def("linear_xent_fwd", &linear_xent_fwd);
   m.def("linear_xent_bwd", &linear_xent_bwd);
   m.def("linear_act8_sizes", &linear_act8_sizes, py::arg("rows"), py::arg("width"), py::arg("out"), py::arg("dt"),

@@ -497,13 +497,13 @@ struct XentPlan {
   int64_t b_g, b_dx, b_dw, b_db;
 };
 
-constexpr int64_t kGBytes = int64_t(512) << 20;  // G of one piece of the vocabulary
 constexpr int kTwoRows = 128;
 // rows from which xent_count runs: the gather takes 6.2 / 9.2 / 15.9 / 42 us without it at 8192 / 16384 /
 // 32768 / 65536 rows of 64, 4.8 / 5.3 / 6.3 / 8.8 with it, and it takes 2.8 and a launch
 constexpr int kCountFrom = 12288;
 
-XentPlan xent_plan(int rows, int width, int classes, bool f32) {
+// g_bytes: most for G of one piece of the vocabulary (one piece has 256 columns at least)
+XentPlan xent_plan(int rows, int width, int classes, bool f32, int64_t g_bytes) {
   XentPlan q{};
   const int np = f32 ? 6 : 1;
   // bf16: one rounding of G to bf16 is one more of the same size as the gradients' own, and over many
@@ -533,7 +533,7 @@ XentPlan xent_plan(int rows, int width, int classes, bool f32) {
   at = 0;
   // pieces of equal width, so that none of them is a remainder that fills a few CUs
   const int64_t row_bytes = int64_t(rows) * 2 * q.planes;
-  const int64_t most = std::max<int64_t>(256, kGBytes / row_bytes / 256 * 256);
+  const int64_t most = std::max<int64_t>(256, g_bytes / row_bytes / 256 * 256);
   const int64_t pieces = (q.vpad + most - 1) / most;
   q.piece = int(up((q.vpad + pieces - 1) / pieces, 256));
   q.gtile = tile(q.piece);
@@ -555,13 +555,14 @@ XentPlan xent_plan(int rows, int width, int classes, bool f32) {
   return q;
 }
 
-void check_xent(int64_t rows, int64_t width, int64_t classes, int64_t vocab) {
+void check_xent(int64_t rows, int64_t width, int64_t classes, int64_t vocab, int64_t g_bytes) {
   VODA_CHECK(rows > 0 && rows <= (1 << 24), "linear_xent: 1 to 2^24 rows");
   VODA_CHECK(width > 0 && width <= (1 << 20), "linear_xent: width 1 to 2^20");
   VODA_CHECK(classes > 0 && classes <= vocab && vocab <= (1 << 24), "linear_xent: 1 <= classes <= vocabulary <= 2^24");
   // a launch holds less than 2^32 threads: 256 x 128 a workgroup of 256, eight outputs a thread of the finish
   VODA_CHECK(up(rows, 128) / 128 * (up(classes, 256) / 256) < (1 << 24), "linear_xent: rows x vocabulary too large");
   VODA_CHECK(rows * up(width, 8) <= (int64_t(1) << 34), "linear_xent: rows x width too large");
+  VODA_CHECK(g_bytes >= 0, "linear_xent: the workspace's limit is negative");
 }
 
 }  // namespace
@@ -583,9 +584,9 @@ void dx_gemm(int tile, const GemmArgs& p, int64_t grid, hipStream_t st) {
 
 // bytes of (forward workspace, backward workspace), and the widths of x's compact rows and of the
 // padded fp32 bias
-std::vector<int64_t> linear_xent_sizes(int64_t rows, int64_t width, int64_t classes, int64_t vocab, bool f32) {
-  check_xent(rows, width, classes, vocab);
-  const XentPlan q = xent_plan(int(rows), int(width), int(classes), f32);
+std::vector<int64_t> linear_xent_sizes(int64_t rows, int64_t width, int64_t classes, int64_t vocab, bool f32, int64_t g_bytes) {
+  check_xent(rows, width, classes, vocab, g_bytes);
+  const XentPlan q = xent_plan(int(rows), int(width), int(classes), f32, g_bytes);
   return {q.fwd_bytes, q.bwd_bytes, q.kp, q.vpad, int64_t(sizeof(XentDev))};
 }
 
@@ -595,13 +596,13 @@ void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
                      int64_t ignore, int64_t rows, int64_t width, int64_t classes, int64_t vocab, int dt, uintptr_t ws,
                      uintptr_t xc, uintptr_t bias32, uintptr_t inv, uintptr_t lab, uintptr_t stat, uintptr_t dev,
                      uintptr_t wp, uintptr_t loss, uintptr_t correct, uintptr_t n_out, uintptr_t stream) {
-  check_xent(rows, width, classes, vocab);
+  check_xent(rows, width, classes, vocab, 0);
   VODA_CHECK(dt == kF32 || dt == kBF16, "linear_xent: x must be fp32 or bf16");
   const bool f32 = dt == kF32;
   VODA_CHECK(f32 || (w % 16 == 0 && ldw % 8 == 0 && ldw >= up(width, 8)),
              "linear_xent: bf16 weight rows must be 16-byte aligned and whole 16-byte vectors");
   VODA_CHECK(xc % 16 == 0 && ws % 256 == 0 && wp % 16 == 0 && (wp || !f32), "linear_xent: workspaces must be aligned");
-  const XentPlan q = xent_plan(int(rows), int(width), int(classes), f32);
+  const XentPlan q = xent_plan(int(rows), int(width), int(classes), f32, 0);
   hipStream_t st = as_stream(stream);
   uint8_t* base = reinterpret_cast<uint8_t*>(ws);
   XentDev* d = reinterpret_cast<XentDev*>(dev);
@@ -664,12 +665,13 @@ void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
 }
 
 // dx [rows][width] contiguous in x's type; rows [0, classes) of dw [..][ldd] in ``grad_dt`` and of db in
-// ``db_dt`` (added to when ``accumulate``); each of dx, dw and db may be null.
+// ``db_dt`` (added to when ``accumulate``); each of dx, dw and db may be null.  ``g_bytes`` as in the
+// sizes.
 void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int64_t classes, int64_t vocab, int dt,
                      uintptr_t ws, uintptr_t xc, uintptr_t bias32, uintptr_t inv, uintptr_t lab, uintptr_t stat,
                      uintptr_t dev, uintptr_t wp, uintptr_t gloss, uintptr_t dx, uintptr_t dw, int64_t ldd,
-                     uintptr_t db, int grad_dt, int db_dt, bool accumulate, uintptr_t stream) {
-  check_xent(rows, width, classes, vocab);
+                     uintptr_t db, int grad_dt, int db_dt, bool accumulate, int64_t g_bytes, uintptr_t stream) {
+  check_xent(rows, width, classes, vocab, g_bytes);
   VODA_CHECK(dt == kF32 || dt == kBF16, "linear_xent: x must be fp32 or bf16");
   VODA_CHECK((grad_dt == kF32 || grad_dt == kBF16) && (db_dt == kF32 || db_dt == kBF16),
              "linear_xent: weight and bias gradients must be fp32 or bf16");
@@ -677,7 +679,7 @@ void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int6
   VODA_CHECK(f32 || (w % 16 == 0 && ldw % 8 == 0 && ldw >= up(width, 8)),
              "linear_xent: bf16 weight rows must be 16-byte aligned and whole 16-byte vectors");
   VODA_CHECK(xc % 16 == 0 && ws % 256 == 0 && wp % 16 == 0 && (wp || !f32), "linear_xent: workspaces must be aligned");
-  const XentPlan q = xent_plan(int(rows), int(width), int(classes), f32);
+  const XentPlan q = xent_plan(int(rows), int(width), int(classes), f32, g_bytes);
   hipStream_t st = as_stream(stream);
   uint8_t* base = reinterpret_cast<uint8_t*>(ws);
   XentDev* d = reinterpret_cast<XentDev*>(dev);

@@ -61,7 +61,8 @@ void layernorm_bwd(uintptr_t dy, uintptr_t x, uintptr_t mean, uintptr_t rstd, ui
                    uintptr_t dbias_in = 0);
 
 // ---- vocabulary head's loss without logits (linear_xent.hip) ----
-std::vector<int64_t> linear_xent_sizes(int64_t rows, int64_t width, int64_t classes, int64_t vocab, bool f32);
+std::vector<int64_t> linear_xent_sizes(int64_t rows, int64_t width, int64_t classes, int64_t vocab, bool f32,
+                                       int64_t g_bytes);
 void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr_t bias, int bias_dt, uintptr_t labels,
                      int64_t ignore, int64_t rows, int64_t width, int64_t classes, int64_t vocab, int dt, uintptr_t ws,
                      uintptr_t xc, uintptr_t bias32, uintptr_t inv, uintptr_t lab, uintptr_t stat, uintptr_t dev,
@@ -69,7 +70,7 @@ void linear_xent_fwd(uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, uintptr
 void linear_xent_bwd(uintptr_t w, int64_t ldw, int64_t rows, int64_t width, int64_t classes, int64_t vocab, int dt,
                      uintptr_t ws, uintptr_t xc, uintptr_t bias32, uintptr_t inv, uintptr_t lab, uintptr_t stat,
                      uintptr_t dev, uintptr_t wp, uintptr_t gloss, uintptr_t dx, uintptr_t dw, int64_t ldd,
-                     uintptr_t db, int grad_dt, int db_dt, bool accumulate, uintptr_t stream);
+                     uintptr_t db, int grad_dt, int db_dt, bool accumulate, int64_t g_bytes, uintptr_t stream);
 
 // ---- Linear with an 8-bit input checkpoint (act8.hip) ----
 std::vector<int64_t> linear_act8_sizes(int64_t rows, int64_t width, int64_t out, int dt, bool copy, bool gelu);

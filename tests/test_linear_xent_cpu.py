@@ -130,3 +130,16 @@ def test_the_workspace_is_bounded():
     h = _native.hip()
     mb = [h.linear_xent_sizes(8192, 2048, v, v, False)[1] / 2 ** 20 for v in (1 << 16, 1 << 18, 1 << 20)]
     assert mb[-1] < 1.2 * mb[0] and mb[-1] < 512 + 4 * 64 + 128
+
+
+def test_the_workspace_s_limit():
+    """G goes in pieces of at least 256 columns, of at most ``g_bytes`` otherwise."""
+    from vodascheduler_amd.ops import _native
+
+    h = _native.hip()
+    for f32, planes in ((False, 1), (True, 3)):
+        size = [h.linear_xent_sizes(1000, 64, 20000, 20000, f32, limit)[1] for limit in (0, 4 << 20, 512 << 20)]
+        assert size[0] < size[1] < size[2] and size[2] == h.linear_xent_sizes(1000, 64, 20000, 20000, f32)[1]
+        assert size[0] >= 1000 * 2 * planes * 256 and size[2] >= 1000 * 2 * planes * 20000
+    with pytest.raises(ValueError):
+        h.linear_xent_sizes(1000, 64, 20000, 20000, False, -1)

@@ -195,3 +195,46 @@ def test_the_first_of_nothing_but_masks(dtype, rows):
         b[600] = 0.0
     y = torch.where(y == 0, 600, torch.where(y == 600, 5, y))
     assert int(linear_cross_entropy(x, w, y, b, 690)[1]) == int((y == 600).sum())
+
+
+@pytest.mark.parametrize("dtype,flat", [(d, f) for d in TYPES for f in (None, torch.float32, torch.bfloat16)
+                                        if (d, f) != (torch.float32, torch.bfloat16)])
+@pytest.mark.parametrize("rows", [20, 300, 700])
+def test_pieces_of_the_vocabulary(dtype, rows, flat, monkeypatch):
+    """Three pieces, the last of 188 columns, classes < vocabulary: dx gathers over them, dw and db go
+    piece by piece to their rows, returned or onto what a flat gradient holds."""
+    from vodascheduler_amd.ops import linear_xent
+    from vodascheduler_amd.utils.flat import FlatGroup, grad_of
+
+    monkeypatch.setattr(linear_xent, "G_BYTES", 0)
+    K, V, C = 72, 730, 700
+    x, w, b, y = _inputs(rows, K, V, C, dtype, bias=True, seed=rows)
+    if flat is None:
+        _check(x, w, b, y, C)
+        return
+    want, bound = formulas(x, w, b, y, C, -100)
+    w, b = torch.nn.Parameter(w.detach()), torch.nn.Parameter(b.detach())
+    group = FlatGroup([w, b], grad_dtype=flat)  # noqa: F841  (owns the gradients)
+    for t in (w, b):
+        grad_of(t).fill_(0.5)
+    loss = linear_cross_entropy(x, w, y, b, C)[0]
+    monkeypatch.setattr(linear_xent, "G_BYTES", 1 << 20)  # the backward keeps to the forward's limit
+    loss.backward()
+    within(x.grad, want[3], bound[1], "dx")
+    half = torch.finfo(flat).eps / 2
+    for t, r, d in ((w, want[4], bound[2]), (b, want[5], bound[3])):
+        within(grad_of(t), r + 0.5, d + half * (r + 0.5).abs() + 2.0 ** -24, "flat gradient")
+        assert torch.equal(grad_of(t)[C:], torch.full_like(grad_of(t)[C:], 0.5))
+
+
+def test_the_number_of_pieces(monkeypatch):
+    """One piece, two or three: the forward, which has none, keeps its bits, and the gradients their bounds."""
+    from vodascheduler_amd.ops import linear_xent
+
+    for dtype, rows in ((torch.bfloat16, 300), (torch.float32, 300), (torch.bfloat16, 40)):
+        x, w, b, y = _inputs(rows, 72, 730, 700, dtype, bias=True)
+        losses = []
+        for limit in (512 << 20, 512 * rows * 2 * 3, 0):
+            monkeypatch.setattr(linear_xent, "G_BYTES", limit)
+            losses.append(_check(x, w, b, y, 700)[0])
+        assert torch.equal(losses[0], losses[1]) and torch.equal(losses[0], losses[2])

@@ -7,10 +7,12 @@ It returns the same ``(loss, correct, n_valid)``: the mean loss over the labelle
 those whose first-maximum class is the label, and their count, all device tensors (no host sync,
 hipGraph-capturable).
 
-* The forward keeps two numbers a row (for the sum of its exponentials); the backward computes the
-  logits again, piece by piece of the vocabulary, in a workspace of at most 512 MB (or one piece of 256
-  columns), and gives ``x``, ``weight`` and ``bias`` their gradients.  BERT-base's MLM head over 8192
-  positions would keep 0.5 GB of bf16 logits and as much gradient.
+* The forward keeps two numbers a row, and the labelled rows of ``x`` together (in a buffer of all rows' size:
+  how many are labelled stays on the device; fp32: three planes, 6 bytes an element), with the bias in fp32.
+  The backward computes the logits again, piece by piece of the vocabulary, and leaves their gradient in a
+  workspace of at most ``G_BYTES`` (512 MB; one piece has at least 256 columns); beside it stand the split sums
+  of dx and dw and, in fp32, the planes of ``weight``.  BERT-base's MLM head over 8192 positions would keep
+  0.5 GB of bf16 logits and as much gradient.
 * A row whose label is ``ignore_index`` or lies outside [0, num_classes) is left out before any
   product: it costs nothing, its gradient is exactly zero, and nothing that it holds (NaN, uninitialised
   padding) reaches the loss or a gradient.  A loss with every row ignored is 0 (PyTorch: NaN).
@@ -37,6 +39,11 @@ from torch.autograd.function import once_differentiable
 from ..utils.flat import flat_grad
 from . import _native as N
 from .dense import _direct, _ready
+
+
+# most for G of one piece of the vocabulary in the backward.  Smaller pieces take more time: at 512 / 256 / 128 / 64 MB
+# a translation batch (10240 x 256 x 15000) ran in 477 / 513 / 576 / 695 us
+G_BYTES = 512 << 20
 
 
 def _valid(labels: torch.Tensor, classes: int, ignore_index: int) -> torch.Tensor:
@@ -89,7 +96,7 @@ class _LinearXentFn(torch.autograd.Function):
         f32 = x.dtype == torch.float32
         dev = x.device
         with _on(dev):
-            nf, nb, kp, vpad, nd = h.linear_xent_sizes(rows, K, C, V, f32)
+            nf, nb, kp, vpad, nd = h.linear_xent_sizes(rows, K, C, V, f32, G_BYTES)
             w = weight if f32 else _rows16(weight)
             ws = torch.empty(max(nf, 256), dtype=torch.uint8, device=dev)
             # what the backward needs, in one buffer, each part 256-byte aligned: x's compact rows, the
@@ -110,7 +117,7 @@ class _LinearXentFn(torch.autograd.Function):
                               N.ptr(planes), loss.data_ptr(), correct.data_ptr(), n.data_ptr(), N.stream_of(x))
         ctx.save_for_backward(weight, keep)
         ctx.at, ctx.dims, ctx.nb, ctx.kp = at, (rows, K, C, V), nb, kp
-        ctx.params = (weight, bias)
+        ctx.params, ctx.g_bytes = (weight, bias), G_BYTES
         ctx.x_dtype = x.dtype
         ctx.mark_non_differentiable(correct, n)
         ctx.set_materialize_grads(False)  # no zero gradients for the two counts
@@ -151,7 +158,8 @@ class _LinearXentFn(torch.autograd.Function):
                                     p[0], p[1], p[2], p[3], p[4], p[5], N.ptr(planes), gloss.data_ptr(), N.ptr(dx),
                                     N.ptr(dw), dw.stride(0) if need_w else K, N.ptr(db),
                                     N.dtype_code(dw.dtype) if need_w else N.DT_F32,
-                                    N.dtype_code(db.dtype) if need_b else N.DT_F32, bool(direct), N.stream_of(weight))
+                                    N.dtype_code(db.dtype) if need_b else N.DT_F32, bool(direct), ctx.g_bytes,
+                                    N.stream_of(weight))
         if direct:
             if need_w:
                 _ready(wp)
