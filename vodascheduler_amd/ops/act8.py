@@ -124,8 +124,9 @@ class _LinearAct8Fn(torch.autograd.Function):
         keep = ctx.needs_input_grad[1] or gelu and ctx.needs_input_grad[0]
         if not x.is_cuda:
             wide = x.float()
-            y = F.linear(F.gelu(wide, approximate="tanh") if gelu else wide, weight.float(),
-                         None if bias is None else bias.float()).to(x.dtype)
+            with torch.autocast("cpu", enabled=False):
+                y = F.linear(F.gelu(wide, approximate="tanh") if gelu else wide, weight.float(),
+                             None if bias is None else bias.float()).to(x.dtype)
             q, s = _pack_ref(x) if keep else (None, None)
             ctx.save_for_backward(weight, q, s)
             return y
@@ -172,15 +173,16 @@ class _LinearAct8Fn(torch.autograd.Function):
         if not dy.is_cuda:
             c = None if q is None else _unpack_ref(q, s, K, torch.float32)
             g = dy.float()
-            if need_x:
-                dx = g @ weight.float()
-                if gelu:
-                    dx = dx * gelu_tanh_grad_ref(c)
-                dx = dx.to(dt) if acc is None else (dx + acc.float()).to(dt)
-            if need_w:
-                dw = (g.t() @ (F.gelu(c, approximate="tanh") if gelu else c)).to(weight.dtype)
-            if need_b:
-                db = g.sum(0).to(bp.dtype)
+            with torch.autocast("cpu", enabled=False):
+                if need_x:
+                    dx = g @ weight.float()
+                    if gelu:
+                        dx = dx * gelu_tanh_grad_ref(c)
+                    dx = dx.to(dt) if acc is None else (dx + acc.float()).to(dt)
+                if need_w:
+                    dw = (g.t() @ (F.gelu(c, approximate="tanh") if gelu else c)).to(weight.dtype)
+                if need_b:
+                    db = g.sum(0).to(bp.dtype)
             return dx, dw, db, None, None, None
         dev = dy.device
         f32 = dt == torch.float32
@@ -243,7 +245,8 @@ def linear_act8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
     # (a reshape that changes nothing would still be a node of the backward)
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if x2.shape[0] == 0:
-        return F.linear(F.gelu(x, approximate="tanh") if act else x, weight, None if bias is None else bias.to(x.dtype))
+        with torch.autocast(dev.type, enabled=False):
+            return F.linear(F.gelu(x, approximate="tanh") if act else x, weight, None if bias is None else bias.to(x.dtype))
     if x2.stride(1) != 1:
         x2 = x2.contiguous()
     if weight.stride(1) != 1:

@@ -59,8 +59,9 @@ def linear_cross_entropy_ref(x: torch.Tensor, weight: torch.Tensor, labels: torc
     x, labels = x.reshape(-1, x.shape[-1]), labels.reshape(-1)
     rows = _valid(labels, C, ignore_index).nonzero()[:, 0]
     y = labels[rows]
-    z = F.linear(x[rows].to(dt), weight[:C].to(dt), None if bias is None else bias[:C].to(dt))
-    loss = F.cross_entropy(z, y, reduction="sum") / max(1, rows.numel())
+    with torch.autocast(x.device.type, enabled=False):
+        z = F.linear(x[rows].to(dt), weight[:C].to(dt), None if bias is None else bias[:C].to(dt))
+        loss = F.cross_entropy(z, y, reduction="sum") / max(1, rows.numel())
     correct = (z.detach().argmax(1) == y).sum()
     return loss, correct, torch.tensor(rows.numel(), device=x.device)
 
@@ -193,6 +194,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     ``num_classes`` classes against integer ``labels`` (one a row of x); see the module docstring."""
     C = weight.shape[0] if num_classes is None else int(num_classes)
     _check(x, weight, labels, bias, C)
+    dev = x.device
     if x.dtype != weight.dtype and torch.is_autocast_enabled(x.device.type):
         x = x.to(weight.dtype)
     # (a reshape that changes nothing would still be a node of the backward)
@@ -206,7 +208,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     if bias is not None and bias.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"linear_cross_entropy: bias must be fp32 or bf16, got {bias.dtype}")
     if x2.shape[0] == 0:  # no rows: a zero that still has (zero) gradients
-        loss = F.linear(x2.float(), weight.float(), None if bias is None else bias.float()).sum()
+        with torch.autocast(dev.type, enabled=False):
+            loss = F.linear(x2.float(), weight.float(), None if bias is None else bias.float()).sum()
         return loss, labels.new_zeros((), dtype=torch.int64), labels.new_zeros((), dtype=torch.int64)
     if x2.stride(1) != 1:
         x2 = x2.contiguous()
