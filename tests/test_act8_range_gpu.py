@@ -3,6 +3,8 @@ arithmetic on its own terms, whatever else a row, a column or the tensor holds."
 import pytest
 import torch
 
+from vodascheduler_amd.ops.act8 import linear_act8
+
 from act8_bounds import U, checkpoint, gelu, slope
 from test_act8_gpu import _inputs, _run
 from xent_bounds import within
@@ -109,3 +111,26 @@ def test_the_largest_and_smallest_numbers():
     assert torch.isfinite(y).all()
     assert ((y[:, 0] - x[:, 0]).abs() <= 2 * U * top).all() and ((y[:, 1] - x[:, 0] / 2).abs() <= U * top).all()
     assert ((y[:, 2] - 1).abs() <= 4 * U).all()
+
+
+@pytest.mark.parametrize("need", [n for n in ((i & 1, i & 2, i & 4) for i in range(1, 8))])
+@pytest.mark.parametrize("act", [None, "gelu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_each_gradient_whatever_else_is_asked_for(dtype, act, need):
+    """dx and dw keep their bits.  db is summed with dw, or by itself in another order: each sum of 50 terms
+    within 50 2^-24 of their sizes, and a rounding to the type."""
+    ins = _inputs(50, 64, 72, dtype, bias=True)
+    dy = ins[3]
+    full = dict(zip("xwb", _run(*ins, act)[1:]))
+    leaves = {nm: t.detach().requires_grad_(bool(k)) for nm, t, k in zip("xwb", ins, need)}
+    y = linear_act8(*leaves.values(), act)
+    asked = {nm: t for nm, t in leaves.items() if t.requires_grad}
+    got = dict(zip(asked, torch.autograd.grad(y, list(asked.values()), dy)))
+    assert set(got) == {nm for nm, k in zip("xwb", need) if k}
+    for nm, g in got.items():
+        r = full[nm]
+        if nm != "b" or "w" in got:
+            assert torch.equal(g, r), nm
+        else:
+            off = 2 * 50 * U * dy.double().abs().sum(0) + torch.finfo(dtype).eps * r.double().abs()
+            assert ((g.double() - r.double()).abs() <= off).all()
