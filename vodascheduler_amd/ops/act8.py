@@ -81,7 +81,7 @@ def act8_pack(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def act8_unpack(q: torch.Tensor, scale: torch.Tensor, width: int, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values a checkpoint stands for, [.., width] (exact in bf16 too, for values bf16 reaches)."""
-    if q.dtype != _F8 or scale.dtype != _E8 or q.shape[:-1] != scale.shape[:-1] or q.device != scale.device:
+    if q.dim() < 1 or q.dtype != _F8 or scale.dtype != _E8 or q.shape[:-1] != scale.shape[:-1] or q.device != scale.device:
         raise ValueError("act8_unpack: q and scale are not a checkpoint of act8_pack")
     if q.shape[-1] != BLOCK * scale.shape[-1] or not 0 < width <= q.shape[-1] or width <= q.shape[-1] - BLOCK:
         raise ValueError(f"act8_unpack: width {width} of a checkpoint {tuple(q.shape)}, {tuple(scale.shape)}")
