@@ -175,7 +175,7 @@ def _check(x, weight, labels, bias, C) -> None:
         raise ValueError(f"linear_cross_entropy: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not multiply")
     if labels.numel() != x.numel() // max(1, x.shape[-1]):
         raise ValueError(f"linear_cross_entropy: {labels.numel()} labels for x {tuple(x.shape)}")
-    if labels.dtype.is_floating_point or labels.dtype == torch.bool:
+    if labels.dtype.is_floating_point or labels.dtype.is_complex or labels.dtype == torch.bool:
         raise TypeError(f"linear_cross_entropy: labels must be integers, got {labels.dtype}")
     if bias is not None and tuple(bias.shape) != (weight.shape[0],):
         raise ValueError(f"linear_cross_entropy: bias {tuple(bias.shape)} for weight {tuple(weight.shape)}")
