@@ -213,8 +213,9 @@ typedef __attribute__((address_space(3))) void c64_lds_void;
 
 // LDS[m0 + 16 * lane] = global[gptr] (inline asm: hipcc must not see an LDS write in flight,
 // or it would guard every LDS read of the row with a wait on it)
+// s_nop: the load may read M0 one wait state after its write, and in here the compiler puts none.
 __device__ __forceinline__ void c64_dma16(const void* gptr, uint32_t lds_addr) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gptr), "s"(lds_addr) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gptr), "s"(lds_addr) : "memory", "m0");
 }
 
 // one row of `pieces` 16-byte pieces from global `src` to LDS `dst`, 1 KB per wave-instruction,

@@ -50,8 +50,10 @@ struct Operand {
   int n;          // rows i (>= 1)
 };
 
+// LDS[m0 + 16 * lane] = global[gptr].  s_nop: the load may read M0 one wait state after its write, and in here
+// the compiler puts none.
 __device__ __forceinline__ void dma16(const void* gptr, uint32_t lds_addr) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gptr), "s"(lds_addr) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gptr), "s"(lds_addr) : "memory", "m0");
 }
 
 template <int N>

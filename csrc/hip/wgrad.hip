@@ -306,8 +306,9 @@ __global__ __launch_bounds__(kWgThreads, 2) void wgrad_kernel(WgradArgs p) {
 // that hipcc does not see an LDS write in flight: it would otherwise guard the next
 // ds_read_b64_tr_b16 with s_waitcnt vmcnt(0) and drain the whole ring every stage.  The
 // ring's completion is tracked by hand (wg_wait_vm) and published by the barrier.
+// s_nop: the load may read M0 one wait state after its write, and in here the compiler puts none.
 __device__ __forceinline__ void wg_dma16(const void* gptr, uint32_t lds_addr) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gptr), "s"(lds_addr) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gptr), "s"(lds_addr) : "memory", "m0");
 }
 
 template <int N>
