@@ -722,7 +722,7 @@ inline int whole_rows(uintptr_t p, int64_t ld, bool bf16) { return p % 16 == 0 &
 //   kBig  256 x 128, two workgroups a CU: one's epilogue runs beside the other's products;
 //   kSq   128 x 128, two a CU;
 //   kDeep 128 x 128, one a CU on a ring twice as deep, where there are not two: nothing else hides the
-//         loads' latency (2 us a stage) then.  [1001 x 331] . [331 x 1348] in fp32 36 -> 20 us, but
+//         loads' latency (2 us a stage) then.  [1001 x 331] . [331 x 1348] in fp32 36 -> 23 us, but
 //         [8192 x 2304]^T . [8192 x 768] in bf16, which splits into two a CU, 50 -> 64;
 //   kFew  128 x 32 (row operands), for a handful of rows, whose products only stream the weights.
 template <int NP, bool IT, bool JT> using Wide = Tile<NP, IT, JT, 2, 4, 4, 2, 64, 2>;
@@ -753,9 +753,9 @@ inline int choose_tile(int64_t ni, int64_t nj, int64_t nk, int np, bool col_i, b
   // over a long reduction); over a short one kWide's epilogue, which nothing hides, costs more than that
   if (w >= 192 && nk * np >= 1536 && (w + 255) / 256 * 10 <= (b + 255) / 256 * 6) return kWide;
   if (b >= 256) return kBig;
-  // a split reduction fills the chip with the largest tile too, at twice kSq's slabs: with 1820 to 3456 steps
-  // a split it won ([8704 x 15000]^T . [8704 x 256] in bf16 and qkv's gradients in fp32, 448 -> 438 and 411 ->
-  // 401 us a pass), with 900 to 1150 it lost (qkv's in bf16, 164 -> 172)
+  // a split reduction fills the chip with the largest tile too, at twice kSq's slabs: with 1820 to 6912 steps
+  // a split it won ([8704 x 15000]^T . [8704 x 256] in bf16 and qkv's gradients in fp32, 448 -> 438 and 615 ->
+  // 565 us a pass), with 900 to 1150 it lost (qkv's in bf16, 164 -> 172)
   if (split) {
     const int64_t s = split_of(kWide).of(w, nk);
     if (w * s >= 192 && nk / s * np >= 1536) return kWide;
