@@ -15,7 +15,7 @@ least 2^-126) that keeps the block's largest finite value within 448, so the onl
 (what would round past fp32's range stays at 240 2^120); infinities and NaN come back as NaN.
 
 Types: bf16 or fp32 ``x`` and ``weight`` alike (fp32 at fp32 accuracy wherever the products stay
-finite: three bf16 planes hold any finite element by itself; an infinite one gives NaN or infinity where it
+finite: three bf16 planes hold an element of 2^-110 or more by itself, whatever stands beside it; an infinite one gives NaN or infinity where it
 takes part), ``bias`` of either.  Any sizes and row strides.  Gradients that the
 fused optimizer owns go straight into its flat buffer (ops/dense.py's contract).  Without a gradient of
 ``weight`` and without the GELU no checkpoint is kept.  Only first derivatives.  ``Act8Linear`` is the

@@ -19,7 +19,8 @@ hipGraph-capturable).
 * ``weight`` rows from ``num_classes`` on are padding: outside the softmax, gradient zero.  A bias of
   -inf takes a class out.
 * Types: bf16 or fp32 ``x`` and ``weight`` alike, ``bias`` of either; fp32 runs at fp32 accuracy (three
-  bf16 planes an operand, which hold any finite element by itself) wherever the products stay finite.  An infinite or NaN input of a labelled row or of a class's
+  bf16 planes an operand, which hold an element of 2^-110 or more by itself, whatever stands beside it) wherever
+  the products stay finite.  An infinite or NaN input of a labelled row or of a class's
   weights makes the loss NaN or infinite, and such a row counts as not correct.  Anything else is refused on a GPU.
 * Gradients of a weight and bias that the fused optimizer owns are summed straight into its flat
   buffer (ops/dense.py's contract), else returned.  Sums have a fixed order: the same call gives the
